@@ -505,6 +505,99 @@ int ftc_backend_kv_read(ftc_backend* be, int64_t layer, int64_t pos0, int64_t n,
 int ftc_backend_kv_write(ftc_backend* be, int64_t layer, int64_t pos0, int64_t n, const float* k,
                          const float* v);
 
+/* ------------------------------------------------------------ paged KV cache
+ *
+ * One layer's cache of many sequences, in pages of page_size positions: a
+ * sequence owns whole pages in any order, named by a page table, so requests
+ * of any length share one pool and a common prefix can share pages.  The
+ * reference keeps one fp32 buffer per sequence (ft/include/ft/kv_cache.h:12-20,
+ * ftc_backend_kv_alloc here). */
+
+/* Element type of a cache beside FTC_F16 and FTC_BF16: 8-bit codes with one
+ * fp32 scale d per position and KV head (row of head_dim values):
+ *   d = max|x| / 127 (rounded to fp32),  code = x / d rounded to the nearest
+ *   integer, ties to even,  value = d * code.
+ * A row of zeros has d = 0; a row that holds an infinity or a NaN gets
+ * d = NaN and reads back as NaN. */
+#define FTC_KV_Q8 64
+
+typedef struct ftc_kv_pages {
+    int dtype;                 /* FTC_F16, FTC_BF16 or FTC_KV_Q8 */
+    int64_t n_pages;           /* pages in the pool */
+    int64_t page_size;         /* positions per page: 16, 32, 64, 128 or 256 */
+    int64_t n_head_kv;         /* 1..1024 */
+    int64_t head_dim;          /* 64, 128 or 256 */
+    void* k;                   /* device: page p at p * page_stride elements, */
+    void* v;                   /*   [n_head_kv][page_size][head_dim] inside */
+    int64_t page_stride;       /* elements; its bytes a multiple of 16 */
+    float* k_scale;            /* FTC_KV_Q8: device, page p at p * scale_stride, */
+    float* v_scale;            /*   [n_head_kv][page_size] inside (else NULL) */
+    int64_t scale_stride;      /* floats, a multiple of 4 */
+} ftc_kv_pages;
+
+/* The rows of one call: sequence s has the rows [start[s], start[s + 1]) of
+ * the n_tokens rows, which are its last positions: row i of it is position
+ * kv_len[s] - (start[s + 1] - start[s]) + i.  Position j lives in page
+ * page_table[s * table_stride + j / page_size], slot j % page_size; a page
+ * id outside [0, n_pages) is not mapped, and neither is a position past the
+ * table or a negative one.  Rows at or after start[n_seqs] (padding of a
+ * captured graph) are neither read nor written.  start, kv_len and the table
+ * are DEVICE arrays, read when the kernels run, so a captured call follows
+ * their values; 0 <= start[s] <= start[s + 1] <= n_tokens. */
+typedef struct ftc_page_batch {
+    int64_t n_seqs;            /* 0..2048 */
+    int64_t n_tokens;          /* rows of x, q and out */
+    int64_t max_new;           /* most rows of any sequence (0: unknown); only picks kernels */
+    const int32_t* start;      /* device [n_seqs + 1] */
+    const int32_t* kv_len;     /* device [n_seqs]: positions after this call's rows */
+    const int32_t* page_table; /* device [n_seqs][table_stride] */
+    int64_t table_cols;        /* pages per sequence in the table */
+    int64_t table_stride;      /* >= table_cols */
+} ftc_page_batch;
+
+/* Store the batch's new K and V rows (x_dtype FTC_F32, FTC_F16 or FTC_BF16;
+ * [n_tokens][x_stride], the head's head_dim values at kv_head * head_dim) at
+ * their positions: rounded to the 16-bit type, or quantised.  Rows at
+ * positions that are not mapped are dropped.  When two rows of a call name
+ * one slot, what it holds afterwards is not specified.  The engine's KV
+ * write, ft/src/engine.cpp:553-559, for a batch of sequences.
+ * Pointers 16-byte aligned, x_stride * element size a multiple of 16. */
+int ftc_kv_pages_write(const ftc_kv_pages* pages, const ftc_page_batch* batch, const void* k_new,
+                       const void* v_new, int x_dtype, int64_t x_stride, void* stream);
+
+/* The same rows out of the cache, in out_dtype (FTC_F32, FTC_F16 or
+ * FTC_BF16; one rounding of the value): what ftc_kv_pages_write stored, or,
+ * with start spanning whole sequences, their snapshot (ft/src/engine.cpp:
+ * 630-645).  Rows at positions that are not mapped are zero. */
+int ftc_kv_pages_read(const ftc_kv_pages* pages, const ftc_page_batch* batch, void* k_out,
+                      void* v_out, int out_dtype, int64_t out_stride, void* stream);
+
+/* Bytes of workspace ftc_attention_pages needs (0: none, or bad arguments).
+ * They depend on the device, the cache's and q's types and head layout and
+ * n_tokens, not on the sequences. */
+size_t ftc_attention_pages_workspace_bytes(const ftc_kv_pages* pages, const ftc_page_batch* batch,
+                                           int64_t n_head, int q_dtype);
+
+/* Causal grouped-query attention of the batch's rows over the pages:
+ * Engine::Impl::attn (ft/src/engine.cpp:137-177) for many sequences, one or
+ * many new tokens each.  A row at position p sees position j when j <= p, j
+ * is mapped, and, with window > 0, p - j < window or j < n_sink (the first
+ * n_sink positions stay visible).  Scores are scale * q . k, a row that sees
+ * nothing gives zeros, and what stands at positions that a row does not see
+ * (NaN, infinities) does not reach it.  q and out: [n_tokens][stride] of
+ * q_dtype, head h at h * head_dim; query head h reads KV head
+ * h / (n_head / n_head_kv).  q_dtype is FTC_F32 with any cache, or FTC_F16
+ * with an FTC_F16 or FTC_KV_Q8 cache, or FTC_BF16 with an FTC_BF16 or
+ * FTC_KV_Q8 cache.  The K and V rows of this call must be in the cache
+ * already (ftc_kv_pages_write before it on the stream).  scale > 0.
+ * Pointers 16-byte aligned, strides times the element size multiples of 16.
+ * ws: ftc_attention_pages_workspace_bytes, 256-byte aligned; calls that may
+ * overlap on the GPU need a workspace each. */
+int ftc_attention_pages(const ftc_kv_pages* pages, const ftc_page_batch* batch, const void* q,
+                        int q_dtype, int64_t q_stride, int64_t n_head, float scale,
+                        int64_t window, int64_t n_sink, void* out, int64_t out_stride, void* ws,
+                        size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

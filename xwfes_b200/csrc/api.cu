@@ -132,6 +132,13 @@ int attention_check(int64_t M, int64_t n_head, int64_t n_head_kv, int64_t head_d
                     const char* who);
 int rope(float* x, int64_t M, int64_t heads, int64_t head_dim, int64_t base, double theta,
          int neox, cudaStream_t st);
+int kv_pages_rows(const ftc_kv_pages* c, const ftc_page_batch* b, const void* k, const void* v,
+                  int dtype, int64_t stride, bool write, cudaStream_t st);
+size_t attention_pages_workspace_bytes(const ftc_kv_pages* c, const ftc_page_batch* b,
+                                       int64_t n_head, int q_dtype);
+int attention_pages(const ftc_kv_pages* c, const ftc_page_batch* b, const void* q, int q_dtype,
+                    int64_t q_stride, int64_t n_head, float scale, int64_t window, int64_t n_sink,
+                    void* out, int64_t out_stride, void* ws, size_t ws_bytes, cudaStream_t st);
 
 // status readers of the translation units whose kernels use bounded waits
 int devstat_gemv_q4k(int clear);
@@ -872,6 +879,40 @@ int ftc_attention(const float* q, int64_t M, int64_t n_head, int64_t n_head_kv, 
 int ftc_rope(float* x, int64_t M, int64_t heads, int64_t head_dim, int64_t base, double theta,
              int neox, void* stream) {
     int rc = rope(x, M, heads, head_dim, base, theta, neox, (cudaStream_t)stream);
+    return rc ? rc : ok();
+}
+
+int ftc_kv_pages_write(const ftc_kv_pages* pages, const ftc_page_batch* batch, const void* k_new,
+                       const void* v_new, int x_dtype, int64_t x_stride, void* stream) {
+    if (inject_fail("ftc_kv_pages_write"))
+        return set_error(FTC_E_INJECTED, "ftc_kv_pages_write: injected failure");
+    int rc = kv_pages_rows(pages, batch, k_new, v_new, x_dtype, x_stride, true,
+                           (cudaStream_t)stream);
+    return rc ? rc : ok();
+}
+
+int ftc_kv_pages_read(const ftc_kv_pages* pages, const ftc_page_batch* batch, void* k_out,
+                      void* v_out, int out_dtype, int64_t out_stride, void* stream) {
+    if (inject_fail("ftc_kv_pages_read"))
+        return set_error(FTC_E_INJECTED, "ftc_kv_pages_read: injected failure");
+    int rc = kv_pages_rows(pages, batch, k_out, v_out, out_dtype, out_stride, false,
+                           (cudaStream_t)stream);
+    return rc ? rc : ok();
+}
+
+size_t ftc_attention_pages_workspace_bytes(const ftc_kv_pages* pages, const ftc_page_batch* batch,
+                                           int64_t n_head, int q_dtype) {
+    return attention_pages_workspace_bytes(pages, batch, n_head, q_dtype);
+}
+
+int ftc_attention_pages(const ftc_kv_pages* pages, const ftc_page_batch* batch, const void* q,
+                        int q_dtype, int64_t q_stride, int64_t n_head, float scale,
+                        int64_t window, int64_t n_sink, void* out, int64_t out_stride, void* ws,
+                        size_t ws_bytes, void* stream) {
+    if (inject_fail("ftc_attention_pages"))
+        return set_error(FTC_E_INJECTED, "ftc_attention_pages: injected failure");
+    int rc = attention_pages(pages, batch, q, q_dtype, q_stride, n_head, scale, window, n_sink, out,
+                             out_stride, ws, ws_bytes, (cudaStream_t)stream);
     return rc ? rc : ok();
 }
 

@@ -75,6 +75,11 @@ SIGNATURES = {
     "ftc_attention": (C.c_int, [_p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p,
                                 C.c_size_t, _p]),
     "ftc_rope": (C.c_int, [_p, _i64, _i64, _i64, _i64, C.c_double, C.c_int, _p]),
+    "ftc_kv_pages_write": (C.c_int, [_p, _p, _p, _p, C.c_int, _i64, _p]),
+    "ftc_kv_pages_read": (C.c_int, [_p, _p, _p, _p, C.c_int, _i64, _p]),
+    "ftc_attention_pages_workspace_bytes": (C.c_size_t, [_p, _p, _i64, C.c_int]),
+    "ftc_attention_pages": (C.c_int, [_p, _p, _p, C.c_int, _i64, _i64, C.c_float, _i64, _i64, _p,
+                                      _i64, _p, C.c_size_t, _p]),
     "ftc_backend_kv_alloc": (C.c_int, [_p, _i64, _i64, _i64]),
     "ftc_backend_attention": (C.c_int, [_p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p,
                                         C.c_int, _p]),
@@ -94,6 +99,19 @@ class ExpertChunkJob(C.Structure):
     _fields_ = [("x", _p), ("out", _p), ("gate", _p), ("up", _p), ("down", _p),
                 ("dtype", C.c_int), ("M", _i64), ("K", _i64), ("IC", _i64),
                 ("gate_up_row_stride", C.c_size_t), ("down_row_stride", C.c_size_t)]
+
+
+class KvPagesDesc(C.Structure):
+    """``ftc_kv_pages``: one layer's paged KV cache."""
+    _fields_ = [("dtype", C.c_int), ("n_pages", _i64), ("page_size", _i64), ("n_head_kv", _i64),
+                ("head_dim", _i64), ("k", _p), ("v", _p), ("page_stride", _i64), ("k_scale", _p),
+                ("v_scale", _p), ("scale_stride", _i64)]
+
+
+class PageBatchDesc(C.Structure):
+    """``ftc_page_batch``: the rows and page table of one call."""
+    _fields_ = [("n_seqs", _i64), ("n_tokens", _i64), ("max_new", _i64), ("start", _p),
+                ("kv_len", _p), ("page_table", _p), ("table_cols", _i64), ("table_stride", _i64)]
 
 
 class MoeDesc(C.Structure):
@@ -255,6 +273,222 @@ def rope(x, heads, head_dim, base, theta, neox, stream=None):
     check(lib().ftc_rope(x.data_ptr(), x.shape[0], heads, head_dim, base, float(theta),
                          1 if neox else 0, _stream(stream)), "ftc_rope")
     return x
+
+
+KV_Q8 = 64  # FTC_KV_Q8 in include/ftc.h
+
+_ROW_TYPES = {}  # torch dtype -> FTC type of q / x / out rows (filled on first use)
+_KV_TYPES = {}   # torch dtype -> FTC type of a paged cache
+
+
+def _torch_types():
+    import torch
+    if not _KV_TYPES:
+        _ROW_TYPES.update({torch.float32: F.F32, torch.float16: F.F16, torch.bfloat16: F.BF16})
+        _KV_TYPES.update({torch.float16: F.F16, torch.bfloat16: F.BF16, torch.int8: KV_Q8})
+    return torch
+
+
+class KvPages:
+    """One layer's paged KV cache (``ftc_kv_pages``) over CUDA tensors.
+
+    ``k`` / ``v``: [n_pages, n_head_kv, page_size, head_dim] float16, bfloat16
+    or int8 (8-bit codes; then ``k_scale`` / ``v_scale`` are fp32 [n_pages,
+    n_head_kv, page_size]); dense inside a page, any page stride.
+    page_size 16 .. 256 (a power of two), head_dim 64, 128 or 256."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        _torch_types()
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _KV_TYPES:
+            raise ValueError("KvPages: k and v must be [n_pages, n_head_kv, page_size, head_dim] "
+                             "of one type, float16, bfloat16 or int8")
+        n, h, p, d = k.shape
+        q8 = _KV_TYPES[k.dtype] == KV_Q8
+        if k.stride() != v.stride() or k.stride()[1:] != (p * d, d, 1):
+            raise ValueError("KvPages: pages must be dense and k and v of one page stride")
+        if (k_scale is not None, v_scale is not None) != (q8, q8):
+            raise ValueError("KvPages: k_scale and v_scale go with int8 codes, and only with them")
+        for t in (k_scale, v_scale) if q8 else ():
+            if str(t.dtype) != "torch.float32" or t.shape != (n, h, p) or \
+                    t.stride() != k_scale.stride() or t.stride()[1:] != (p, 1):
+                raise ValueError("KvPages: scales must be fp32 [n_pages, n_head_kv, page_size], "
+                                 "dense inside a page")
+        tensors = [t for t in (k, v, k_scale, v_scale) if t is not None]
+        if any(not t.is_cuda or t.device != k.device for t in tensors):
+            raise ValueError("KvPages: all tensors on one CUDA device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_head_kv, self.page_size, self.head_dim = h, p, d
+        self.device = k.device
+        # a pool of one page has no meaningful stride between pages
+        ps, ss = (k.stride(0) if n > 1 else h * p * d), 0
+        if q8:
+            ss = k_scale.stride(0) if n > 1 else h * p
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        self.desc = KvPagesDesc(_KV_TYPES[k.dtype], n, p, h, d, k.data_ptr(), v.data_ptr(), ps,
+                                ptr(k_scale), ptr(v_scale), ss)
+        self._ref = C.byref(self.desc)
+
+    @classmethod
+    def empty(cls, n_pages, n_head_kv, page_size, head_dim, dtype="KV_Q8", device="cuda"):
+        """A new pool of ``n_pages`` pages (contents unspecified); ``dtype``
+        "F16", "BF16" or "KV_Q8"."""
+        torch = _torch_types()
+        t = {"F16": torch.float16, "BF16": torch.bfloat16, "KV_Q8": torch.int8}.get(
+            dtype.upper() if isinstance(dtype, str) else None)
+        if t is None:
+            raise ValueError('KvPages: dtype must be "F16", "BF16" or "KV_Q8"')
+        shape = (n_pages, n_head_kv, page_size, head_dim)
+        kv = [torch.empty(shape, dtype=t, device=device) for _ in range(2)]
+        sc = [torch.empty(shape[:3], dtype=torch.float32, device=device) for _ in range(2)] \
+            if t == torch.int8 else []
+        return cls(*kv, *sc)
+
+
+class PageBatch:
+    """The rows of a call on a paged cache (``ftc_page_batch``): int32 CUDA
+    tensors ``start`` [n_seqs + 1] (sequence s has rows start[s] ..
+    start[s + 1]), ``kv_len`` [n_seqs] (positions after this call's rows) and
+    ``page_table`` [n_seqs, cols].  ``n_tokens``: rows of the call's tensors;
+    ``max_new``: most rows of any sequence, 0 when unknown (it only picks
+    kernels).  The values are read on the device when the kernels run."""
+
+    def __init__(self, start, kv_len, page_table, n_tokens, max_new=0):
+        torch = _torch_types()
+        for t, dim in ((start, 1), (kv_len, 1), (page_table, 2)):
+            if t.dtype != torch.int32 or t.dim() != dim or not t.is_cuda or \
+                    t.device != start.device or (t.numel() and t.stride(-1) != 1):
+                raise ValueError("PageBatch: int32 tensors start [n_seqs + 1], kv_len [n_seqs] "
+                                 "and page_table [n_seqs, cols] on one CUDA device")
+        n = kv_len.shape[0]
+        if start.shape[0] != n + 1 or page_table.shape[0] != n:
+            raise ValueError("PageBatch: start has n_seqs + 1 entries, page_table n_seqs rows")
+        cols = page_table.shape[1]
+        self.start, self.kv_len, self.page_table = start, kv_len, page_table
+        self.n_tokens, self.device = n_tokens, start.device
+        self.desc = PageBatchDesc(n, n_tokens, max_new, start.data_ptr(), kv_len.data_ptr(),
+                                  page_table.data_ptr(), cols,
+                                  page_table.stride(0) if n > 1 else cols)
+        self._ref = C.byref(self.desc)
+
+
+class _PagedLaunch:
+    """Device guard and stream of a paged call: the current stream of the
+    cache's device unless one is given (a torch stream or its address)."""
+
+    def __init__(self, device, stream):
+        import torch
+        self._guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index \
+            else None
+        self._given = stream
+        self._device = device
+
+    def __enter__(self):
+        import torch
+        if self._guard is not None:
+            self._guard.__enter__()
+        if self._given is None:
+            self.stream, self.ctx = torch.cuda.current_stream(self._device).cuda_stream, None
+            return self
+        s = self._given
+        if isinstance(s, int):
+            s = torch.cuda.ExternalStream(s, device=self._device) if s else \
+                torch.cuda.default_stream(self._device)
+        # buffers made here belong to the stream that the kernels run on
+        self.stream, self.ctx = s.cuda_stream, torch.cuda.stream(s)
+        self.ctx.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def _paged_rows(x, pages, batch, width, what):
+    """(FTC type, row stride) of rows [n_tokens, width] (or [n_tokens, heads,
+    head_dim]); rows may be wider apart than they are long."""
+    if x.dim() == 3:
+        x = x.view(x.shape[0], x.shape[1] * x.shape[2])
+    if x.dtype not in _ROW_TYPES or x.dim() != 2 or x.shape[1] != width or \
+            x.shape[0] != batch.n_tokens or x.device != pages.device or \
+            (x.shape[0] and x.stride(1) != 1):
+        raise ValueError(f"{what}: rows must be [{batch.n_tokens}, {width}] float32, float16 or "
+                         "bfloat16 on the cache's device, values of a row next to each other")
+    return _ROW_TYPES[x.dtype], x.stride(0) if x.shape[0] > 1 else width
+
+
+def _paged_args(pages, batch, what):
+    if batch.device != pages.device:
+        raise ValueError(f"{what}: cache and batch on different devices")
+
+
+def kv_pages_write(pages, k_new, v_new, batch, stream=None):
+    """Store the batch's new K and V rows ([n_tokens, n_head_kv * head_dim]
+    fp32, fp16 or bf16) in the paged cache, rounded or quantised to its type
+    (ftc_kv_pages_write)."""
+    _paged_args(pages, batch, "kv_pages_write")
+    width = pages.n_head_kv * pages.head_dim
+    t, ld = _paged_rows(k_new, pages, batch, width, "kv_pages_write")
+    if (t, ld) != _paged_rows(v_new, pages, batch, width, "kv_pages_write"):
+        raise ValueError("kv_pages_write: k_new and v_new must have one type and row stride")
+    with _PagedLaunch(pages.device, stream) as on:
+        check(lib().ftc_kv_pages_write(pages._ref, batch._ref, k_new.data_ptr(), v_new.data_ptr(),
+                                       t, ld, on.stream), "ftc_kv_pages_write")
+
+
+def kv_pages_read(pages, batch, k_out=None, v_out=None, out_dtype="F32", stream=None):
+    """The batch's rows out of the paged cache (ftc_kv_pages_read): (k, v)
+    [n_tokens, n_head_kv * head_dim] in ``out_dtype`` ("F32", "F16" or "BF16";
+    the type of k_out when given).  Rows of padding keep what they held."""
+    torch = _torch_types()
+    _paged_args(pages, batch, "kv_pages_read")
+    width = pages.n_head_kv * pages.head_dim
+    with _PagedLaunch(pages.device, stream) as on:
+        if k_out is None or v_out is None:
+            if k_out is not None or v_out is not None:
+                raise ValueError("kv_pages_read: give both k_out and v_out, or none")
+            dt = getattr(torch, _TORCH_OUT[F.dtype_id(out_dtype)])
+            k_out = torch.empty((batch.n_tokens, width), dtype=dt, device=pages.device)
+            v_out = torch.empty_like(k_out)
+        t, ld = _paged_rows(k_out, pages, batch, width, "kv_pages_read")
+        if (t, ld) != _paged_rows(v_out, pages, batch, width, "kv_pages_read"):
+            raise ValueError("kv_pages_read: k_out and v_out must have one type and row stride")
+        check(lib().ftc_kv_pages_read(pages._ref, batch._ref, k_out.data_ptr(), v_out.data_ptr(),
+                                      t, ld, on.stream), "ftc_kv_pages_read")
+    return k_out, v_out
+
+
+def attention_pages(q, n_head, pages, batch, window=0, n_sink=0, scale=None, out=None, ws=None,
+                    stream=None):
+    """Causal grouped-query attention of the batch's rows over the paged cache
+    (ftc_attention_pages): q [n_tokens, n_head * head_dim] fp32, fp16 or bf16;
+    returns out of q's type.  ``window`` > 0: a row sees the last ``window``
+    positions up to its own, and the first ``n_sink``.  ``scale`` defaults to
+    1 / sqrt(head_dim).  ``ws``: uint8 workspace (allocated when None)."""
+    torch = _torch_types()
+    _paged_args(pages, batch, "attention_pages")
+    width = n_head * pages.head_dim
+    t, ld = _paged_rows(q, pages, batch, width, "attention_pages")
+    if scale is None:
+        scale = pages.head_dim ** -0.5
+    with _PagedLaunch(pages.device, stream) as on:
+        if out is None:
+            out = torch.empty((batch.n_tokens, width), dtype=q.dtype, device=pages.device)
+        to, ldo = _paged_rows(out, pages, batch, width, "attention_pages")
+        if to != t:
+            raise ValueError("attention_pages: out must have q's type")
+        need = lib().ftc_attention_pages_workspace_bytes(pages._ref, batch._ref, n_head, t)
+        if ws is None and need:
+            ws = torch.empty(need, dtype=torch.uint8, device=pages.device)
+        if ws is not None and (ws.device != pages.device or not ws.is_contiguous()):
+            raise ValueError("attention_pages: ws must be contiguous on the cache's device")
+        check(lib().ftc_attention_pages(
+            pages._ref, batch._ref, q.data_ptr(), t, ld, n_head, scale, window, n_sink,
+            out.data_ptr(), ldo, ws.data_ptr() if ws is not None else None,
+            ws.numel() * ws.element_size() if ws is not None else 0, on.stream),
+            "ftc_attention_pages")
+    return out
 
 
 _TORCH_OUT = {F.F32: "float32", F.BF16: "bfloat16", F.F16: "float16"}
