@@ -57,6 +57,13 @@ def attention(q, n_head, pages, table, start, kv_len, window=0, n_sink=0, scale=
         operand type (f16, or bf16 over a bf16 cache);
       * the weighted sum and the sum of weights: the same two roundings per
         16 positions, plus one for each of up to 64 joined parts;
+      * f16 weights (all but over a bf16 cache) lie on a grid that ends in steps
+        of 2^-24.  The kernels hold them 2^up times the weight relative to the
+        row's largest (14 for fp32 q, at least 6 for 16-bit q), times V's
+        scale relative to at most twice the largest one: each is off by at
+        most half a step, 2^-25, of 2^-up * 2 max|v| on top of its relative
+        error, and the sum of weights is at least 1 in these units, so n
+        positions add n * 2^-(24 + up) * max|v|;
       * one rounding of the result to q's type."""
     hd, nkv, page = pages.head_dim, pages.n_head_kv, pages.page_size
     n_pages = pages.k.shape[0]
@@ -68,6 +75,8 @@ def attention(q, n_head, pages, table, start, kv_len, window=0, n_sink=0, scale=
     pieces = 3 if q.dtype == torch.float32 else 1
     u_p = 2.0 ** -22 if q.dtype == torch.float32 else \
         EPS_HALF[torch.bfloat16 if pages.k.dtype == torch.bfloat16 else torch.float16]
+    floor = 0.0 if pages.k.dtype == torch.bfloat16 else \
+        2.0 ** -(24 + (14 if q.dtype == torch.float32 else 6))
     tab = table.cpu()
     for s in range(len(kv_len)):
         n = start[s + 1] - start[s]
@@ -107,8 +116,9 @@ def attention(q, n_head, pages, table, start, kv_len, window=0, n_sink=0, scale=
             e = a * (2.0 ** -22 + (hd // 16) * pieces * 2.0 ** -22 + 6 * 2.0 ** -24)
             acc = ((len(ok) + 15) // 16 * pieces + 64) * 2.0 ** -22
             wabs = torch.nan_to_num(w, 0, 0) @ torch.nan_to_num(vh.abs(), 0, 0, 0)
+            vmax = torch.nan_to_num(vh.abs(), 0, 0, 0).max() if len(ok) else 0.0
             bound[start[s]:start[s + 1], h] = (2 * e + u_p + acc) * wabs + \
-                EPS_HALF[q.dtype] * o.abs() + 1e-30
+                floor * len(ok) * vmax + EPS_HALF[q.dtype] * o.abs() + 1e-30
     if q.dtype == torch.float16:
         bound += 2.0 ** -25  # half a step of its subnormals
     return out.view(T, -1), bound.view(T, -1)

@@ -145,6 +145,9 @@ int devstat_gemv_q4k(int clear);
 int devstat_gemv_imma(int clear);
 int devstat_gemm_q4k(int clear);
 int devstat_peer_ar(int clear);
+int devstat_pages_f16(int clear);
+int devstat_pages_bf16(int clear);
+int devstat_pages_q8(int clear);
 
 }  // namespace ftc
 
@@ -789,7 +792,8 @@ int ftc_device_status(void* stream, int* status) {
     FTC_REQUIRE(status, FTC_E_INVALID, "ftc_device_status: null status");
     FTC_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
     int v = 0;
-    for (int (*rd)(int) : {devstat_gemv_q4k, devstat_gemv_imma, devstat_gemm_q4k, devstat_peer_ar}) {
+    for (int (*rd)(int) : {devstat_gemv_q4k, devstat_gemv_imma, devstat_gemm_q4k, devstat_peer_ar,
+                           devstat_pages_f16, devstat_pages_bf16, devstat_pages_q8}) {
         const int s = rd(1);
         FTC_REQUIRE(s >= 0, FTC_E_CUDA, "ftc_device_status: cannot read the status word");
         v |= s;

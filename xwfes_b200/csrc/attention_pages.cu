@@ -1,107 +1,223 @@
 // attention_pages.cu -- causal grouped-query attention of a ragged batch of
 // new rows over a paged KV cache, with an optional sliding window and sink
 // positions (Engine::Impl::attn, ft/src/engine.cpp:137-177, for many
-// sequences).
-//
-// One warp per (row, query head): the visible positions one after another,
-// an online softmax (running maximum m and sum l, the accumulator rescaled
-// when m grows), head_dim / 32 values per lane.
-#include <cuda_bf16.h>
+// sequences): argument checks, the choice of kernels, the workspace and the
+// joining of cut tiles.
+#include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
+#include <mutex>
 
-#include "kv_pages.cuh"
+#include "attention_pages.cuh"
 
 namespace ftc {
+namespace paged {
+
+int launch_f16(const PagedJob& j, int q_dtype);
+int launch_bf16(const PagedJob& j, int q_dtype);
+int launch_q8(const PagedJob& j, int q_dtype);
+PagedSet geom_f16(int64_t hd, int q_dtype, int cls);
+PagedSet geom_bf16(int64_t hd, int q_dtype, int cls);
+PagedSet geom_q8(int64_t hd, int q_dtype, int cls);
+
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float to_f(T x) {
-    if constexpr (std::is_same<T, __half>::value) return __half2float(x);
-    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __bfloat162float(x);
-    else return (float)x;
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+                cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
 }
 
-template <typename T>
-__device__ __forceinline__ T from_f(float x) {
-    if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
-    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __float2bfloat16_rn(x);
-    else return x;
+}  // namespace
+
+// The pool as [page][KV head and slot][head_dim], boxes of up to 128 bytes by
+// one page's share of a key chunk.
+int page_map(CUtensorMap* m, const void* base, const ftc_kv_pages* c, int key_step) {
+    auto enc = encode_fn();
+    FTC_REQUIRE(enc, FTC_E_CUDA, "ftc_attention_pages: cuTensorMapEncodeTiled unavailable");
+    const bool q8 = c->dtype == FTC_KV_Q8;
+    const int es = q8 ? 1 : 2;
+    const int64_t row = c->head_dim * es;
+    const cuuint64_t dims[3] = {(cuuint64_t)c->head_dim, (cuuint64_t)(c->n_head_kv * c->page_size),
+                                (cuuint64_t)c->n_pages};
+    const cuuint64_t strides[2] = {(cuuint64_t)row, (cuuint64_t)(c->page_stride * es)};
+    const int64_t boxb = row < 128 ? row : 128;
+    const cuuint32_t box[3] = {(cuuint32_t)(boxb / es),
+                               (cuuint32_t)std::min<int64_t>(c->page_size, key_step), 1};
+    const cuuint32_t ones[3] = {1, 1, 1};
+    const CUresult r =
+        enc(m,
+            q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+               : c->dtype == FTC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            3, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            boxb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    FTC_REQUIRE(r == CUDA_SUCCESS, FTC_E_CUDA, "ftc_attention_pages: page tensor map rejected");
+    return FTC_OK;
 }
 
-struct PagedArgs {
-    PageView b;
-    const void *q, *k, *v;
-    const float *ks, *vs;
-    void* out;
-    int64_t q_stride, out_stride;
-    int n_head, gqa;
-    int window, n_sink;
-    float scale;
+}  // namespace paged
+
+namespace {
+
+using namespace paged;
+
+// Where a set of tiles keeps its pieces.
+struct JoinSet {
+    const CutTile* cut;
+    const float2* stat;
+    const float* part;
+    int G, TR;
 };
 
-template <typename X, typename C, int HD>
-__global__ void __launch_bounds__(128) paged_simple(const PagedArgs a) {
+struct JoinArgs {
+    JoinSet set[2];
+    int blocks0;  // blocks of set 0
+    void* out;
+    int64_t out_stride;
+    int gqa;
+};
+
+constexpr int kJoinWarps = 8;
+
+// A warp per row of a cut tile: the pieces in order (the CTA that holds the
+// tile's start has the first in its slot 1, the CTAs after it theirs in slot
+// 0), out = sum_k O_k 2^(M_k - M) / sum_k l_k 2^(M_k - M).
+template <typename X, int HD>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join(const JoinArgs a) {
+    const int which = (int)blockIdx.x >= a.blocks0;
+    const JoinSet& s = a.set[which];
+    const int per = (s.TR + kJoinWarps - 1) / kJoinWarps;  // blocks per CTA of the set
+    const int blk = blockIdx.x - (which ? a.blocks0 : 0);
+    const int b = blk / per;
+    const int r = (blk - b * per) * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const CutTile ct = s.cut[b];
+    if (ct.pieces == 0 || r >= ct.rows) return;
+    auto slot = [&](int k) { return 2 * (int64_t)(b + k) + (k == 0 ? 1 : 0); };
+    float M = -INFINITY;
+    for (int k = lane; k < ct.pieces; k += 32) M = fmaxf(M, s.stat[slot(k) * s.TR + r].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float R = M == -INFINITY ? 0.f : M;
     constexpr int E = HD / 32;
-    const int h = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int t = blockIdx.y + 65535 * blockIdx.z;
-    if (h >= a.n_head || t >= a.b.n_tokens) return;
-    int s = 0;
-    while (s < a.b.n_seqs && a.b.start[s + 1] <= t) ++s;
-    if (s >= a.b.n_seqs) return;
-    int r0, n;
-    seq_rows(a.b, s, r0, n);
-    if (t < r0 || t >= r0 + n) return;
-    const int p = seq_len(a.b, s) - n + (t - r0);
-    const int kvh = h / a.gqa;
-    float q[E], acc[E] = {};
-    const X* qr = static_cast<const X*>(a.q) + (int64_t)t * a.q_stride + (int64_t)h * HD;
-#pragma unroll
-    for (int i = 0; i < E; ++i) q[i] = to_f(qr[lane + 32 * i]) * a.scale;
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j <= p; ++j) {
-        if (a.window > 0 && p - j >= a.window && j >= a.n_sink) {
-            j = p - a.window;
-            continue;
+    float acc[E] = {}, l = 0.f;
+    for (int k0 = 0; k0 < ct.pieces; k0 += 32) {
+        float w = 0.f, wl = 0.f;
+        if (k0 + lane < ct.pieces) {
+            const float2 st = s.stat[slot(k0 + lane) * s.TR + r];
+            w = ex2(st.x - R);
+            wl = st.y * w;
         }
-        const int page = page_of(a.b, s, j);
-        if (page < 0) continue;
-        const int64_t row = (int64_t)kvh * a.b.page_size + (j & (a.b.page_size - 1));
-        const int64_t off = page * a.b.page_stride + row * HD;
-        const C* kr = static_cast<const C*>(a.k) + off;
-        const C* vr = static_cast<const C*>(a.v) + off;
-        float d = 0.f;
+        const int n = min(32, ct.pieces - k0);
+#pragma unroll 8
+        for (int k = 0; k < n; ++k) {
+            const float wk = __shfl_sync(0xffffffffu, w, k);
+            l += __shfl_sync(0xffffffffu, wl, k);
+            const float* p = s.part + (slot(k0 + k) * s.TR + r) * HD + E * lane;
+            float x[E];
+            if constexpr (E == 2) {
+                const float2 v = *reinterpret_cast<const float2*>(p);
+                x[0] = v.x, x[1] = v.y;
+            } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) d = fmaf(q[i], to_f(kr[lane + 32 * i]), d);
+                for (int i = 0; i < E; i += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(p + i);
+                    x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+                }
+            }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        float vsc = 1.f;
-        if constexpr (sizeof(C) == 1) {
-            d *= a.ks[page * a.b.scale_stride + row];
-            vsc = a.vs[page * a.b.scale_stride + row];
+            for (int i = 0; i < E; ++i) acc[i] = fmaf(x[i], wk, acc[i]);
         }
-        const float mn = fmaxf(m, d), al = expf(m - mn), e = expf(d - mn);
-        l = l * al + e;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < E; ++i) acc[i] = fmaf(e * vsc, to_f(vr[lane + 32 * i]), acc[i] * al);
     }
-    X* o = static_cast<X*>(a.out) + (int64_t)t * a.out_stride + (int64_t)h * HD;
+    const int pr = ct.r0 + r, t = pr / a.gqa, h = ct.kvh * a.gqa + pr - t * a.gqa;
+    X* o = static_cast<X*>(a.out) + (int64_t)(ct.row + t) * a.out_stride + (int64_t)h * HD +
+           E * lane;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int i = 0; i < E; ++i) o[lane + 32 * i] = from_f<X>(l == 0.f ? 0.f : acc[i] / l);
+    for (int i = 0; i < E; i += 2) {
+        if constexpr (sizeof(X) == 4)
+            *reinterpret_cast<float2*>(o + i) = make_float2(acc[i] * inv, acc[i + 1] * inv);
+        else *reinterpret_cast<uint32_t*>(o + i) = pack<X>(acc[i] * inv, acc[i + 1] * inv);
+    }
 }
 
-template <typename X, typename C>
-int launch(const PagedArgs& a, int64_t head_dim, cudaStream_t st) {
-    const dim3 grid((unsigned)((a.n_head + 3) / 4),
-                    (unsigned)(a.b.n_tokens < 65535 ? a.b.n_tokens : 65535),
-                    (unsigned)((a.b.n_tokens + 65534) / 65535));
-    if (head_dim == 64) paged_simple<X, C, 64><<<grid, 128, 0, st>>>(a);
-    else if (head_dim == 128) paged_simple<X, C, 128><<<grid, 128, 0, st>>>(a);
-    else paged_simple<X, C, 256><<<grid, 128, 0, st>>>(a);
-    FTC_CUDA(cudaGetLastError());
+template <typename X, int HD>
+int launch_join(const JoinArgs& a, int blocks, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kJoinWarps * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_join<X, HD>, a);
+    if (e != cudaSuccess) return cuda_error(e, "launch paged_join");
     return FTC_OK;
+}
+
+template <typename X>
+int join_hd(const JoinArgs& a, int blocks, int64_t hd, cudaStream_t st) {
+    return hd == 64    ? launch_join<X, 64>(a, blocks, st)
+           : hd == 128 ? launch_join<X, 128>(a, blocks, st)
+                       : launch_join<X, 256>(a, blocks, st);
+}
+
+// The launches of a call: which sequences (by packed rows) go to which class.
+// Decode sequences, 16 rows or fewer, and chunks differ too much for one
+// shape; a batch that may hold both gets two launches.
+struct CallPlan {
+    int n = 0;
+    int cls[2], min_rows[2], max_rows[2];
+    PagedSet set[2];
+    size_t off[2], bytes = 0;
+};
+
+size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+
+CallPlan call_plan(const ftc_kv_pages* c, const ftc_page_batch* b, int64_t n_head, int q_dtype) {
+    CallPlan p;
+    const int64_t gqa = n_head / c->n_head_kv;
+    const int64_t most = b->max_new > 0 ? std::min(b->max_new, b->n_tokens) : b->n_tokens;
+    const int64_t rows = most * gqa;
+    auto add = [&](int cls, int lo, int hi) {
+        p.cls[p.n] = cls;
+        p.min_rows[p.n] = lo;
+        p.max_rows[p.n] = hi;
+        p.set[p.n] = c->dtype == FTC_F16    ? geom_f16(c->head_dim, q_dtype, cls)
+                     : c->dtype == FTC_BF16 ? geom_bf16(c->head_dim, q_dtype, cls)
+                                            : geom_q8(c->head_dim, q_dtype, cls);
+        const PagedSet& s = p.set[p.n];
+        p.off[p.n] = p.bytes;
+        const size_t slots = 2 * (size_t)s.G * s.TR;
+        p.bytes += up256(s.G * sizeof(CutTile)) + up256(slots * sizeof(float2)) +
+                   up256(slots * (size_t)c->head_dim * sizeof(float));
+        ++p.n;
+    };
+    const int big = rows <= 64 ? 1 : 2;
+    if (rows <= 16) {
+        add(0, 1, INT_MAX);
+    } else if (b->n_seqs == 1) {
+        add(big, 1, INT_MAX);
+    } else {
+        if (gqa <= 16) add(0, 1, 16);
+        add(big, gqa <= 16 ? 17 : 1, INT_MAX);
+    }
+    return p;
 }
 
 int check(const ftc_kv_pages* c, const ftc_page_batch* b, int64_t n_head, int q_dtype,
@@ -111,6 +227,8 @@ int check(const ftc_kv_pages* c, const ftc_page_batch* b, int64_t n_head, int q_
     if (rc) return rc;
     FTC_REQUIRE(n_head >= 1 && n_head <= 8192 && n_head % c->n_head_kv == 0, FTC_E_INVALID,
                 w + ": n_head must be a multiple of n_head_kv, at most 8192");
+    FTC_REQUIRE(b->n_tokens * (n_head / c->n_head_kv) <= (1 << 30), FTC_E_UNSUPPORTED,
+                w + ": too many rows for one launch");
     FTC_REQUIRE(q_dtype == FTC_F32 || q_dtype == FTC_F16 || q_dtype == FTC_BF16, FTC_E_UNSUPPORTED,
                 w + ": q must be F32, F16 or BF16");
     FTC_REQUIRE(q_dtype == FTC_F32 || c->dtype == FTC_KV_Q8 || c->dtype == q_dtype,
@@ -124,14 +242,16 @@ size_t attention_pages_workspace_bytes(const ftc_kv_pages* c, const ftc_page_bat
                                        int64_t n_head, int q_dtype) {
     PageView v;
     if (check(c, b, n_head, q_dtype, "ftc_attention_pages_workspace_bytes", &v)) return 0;
-    return 0;
+    if (b->n_seqs == 0 || b->n_tokens == 0) return 0;
+    return call_plan(c, b, n_head, q_dtype).bytes;
 }
 
 int attention_pages(const ftc_kv_pages* c, const ftc_page_batch* b, const void* q, int q_dtype,
                     int64_t q_stride, int64_t n_head, float scale, int64_t window, int64_t n_sink,
                     void* out, int64_t out_stride, void* ws, size_t ws_bytes, cudaStream_t st) {
-    PagedArgs a;
-    const int rc = check(c, b, n_head, q_dtype, "ftc_attention_pages", &a.b);
+    PagedJob j;
+    PagedArgs& a = j.a;
+    int rc = check(c, b, n_head, q_dtype, "ftc_attention_pages", &a.b);
     if (rc) return rc;
     FTC_REQUIRE(scale > 0.f && std::isfinite(scale), FTC_E_INVALID,
                 "ftc_attention_pages: scale must be positive and finite");
@@ -148,13 +268,11 @@ int attention_pages(const ftc_kv_pages* c, const ftc_page_batch* b, const void* 
                 FTC_E_INVALID,
                 "ftc_attention_pages: strides must cover n_head * head_dim and be multiples of 16 "
                 "bytes");
-    const size_t need = attention_pages_workspace_bytes(c, b, n_head, q_dtype);
-    FTC_REQUIRE(ws_bytes >= need && (need == 0 || (ws && (uintptr_t)ws % 256 == 0)), FTC_E_INVALID,
+    const CallPlan plan = call_plan(c, b, n_head, q_dtype);
+    FTC_REQUIRE(ws && ws_bytes >= plan.bytes && (uintptr_t)ws % 256 == 0, FTC_E_INVALID,
                 "ftc_attention_pages: workspace smaller than ftc_attention_pages_workspace_bytes "
                 "or not 256-byte aligned");
     a.q = q;
-    a.k = c->k;
-    a.v = c->v;
     a.ks = c->k_scale;
     a.vs = c->v_scale;
     a.out = out;
@@ -164,16 +282,40 @@ int attention_pages(const ftc_kv_pages* c, const ftc_page_batch* b, const void* 
     a.gqa = (int)(n_head / c->n_head_kv);
     a.window = window > INT_MAX ? 0 : (int)window;
     a.n_sink = n_sink > INT_MAX ? INT_MAX : (int)n_sink;
-    a.scale = scale;
-    if (q_dtype == FTC_F32)
-        return c->dtype == FTC_F16    ? launch<float, __half>(a, c->head_dim, st)
-               : c->dtype == FTC_BF16 ? launch<float, __nv_bfloat16>(a, c->head_dim, st)
-                                      : launch<float, int8_t>(a, c->head_dim, st);
-    if (q_dtype == FTC_F16)
-        return c->dtype == FTC_F16 ? launch<__half, __half>(a, c->head_dim, st)
-                                   : launch<__half, int8_t>(a, c->head_dim, st);
-    return c->dtype == FTC_BF16 ? launch<__nv_bfloat16, __nv_bfloat16>(a, c->head_dim, st)
-                                : launch<__nv_bfloat16, int8_t>(a, c->head_dim, st);
+    a.c = (float)((double)scale * 1.4426950408889634);
+    FTC_REQUIRE(a.c > 0.f && std::isfinite(a.c), FTC_E_INVALID,
+                "ftc_attention_pages: scale out of range");
+    j.c = c;
+    j.st = st;
+    JoinArgs jn = {};
+    jn.out = out;
+    jn.out_stride = out_stride;
+    jn.gqa = a.gqa;
+    int blocks = 0;
+    for (int i = 0; i < plan.n; ++i) {
+        const PagedSet& s = plan.set[i];
+        uint8_t* base = static_cast<uint8_t*>(ws) + plan.off[i];
+        const size_t slots = 2 * (size_t)s.G * s.TR;
+        a.cut = reinterpret_cast<CutTile*>(base);
+        a.stat = reinterpret_cast<float2*>(base + up256(s.G * sizeof(CutTile)));
+        a.part = reinterpret_cast<float*>(base + up256(s.G * sizeof(CutTile)) +
+                                          up256(slots * sizeof(float2)));
+        a.min_rows = plan.min_rows[i];
+        a.max_rows = plan.max_rows[i];
+        a.second = i > 0;
+        j.set = s;
+        j.cls = plan.cls[i];
+        rc = c->dtype == FTC_F16    ? launch_f16(j, q_dtype)
+             : c->dtype == FTC_BF16 ? launch_bf16(j, q_dtype)
+                                    : launch_q8(j, q_dtype);
+        if (rc) return rc;
+        jn.set[i] = {a.cut, a.stat, a.part, s.G, s.TR};
+        blocks += s.G * ((s.TR + kJoinWarps - 1) / kJoinWarps);
+        if (i == 0) jn.blocks0 = blocks;
+    }
+    return q_dtype == FTC_F32   ? join_hd<float>(jn, blocks, c->head_dim, st)
+           : q_dtype == FTC_F16 ? join_hd<__half>(jn, blocks, c->head_dim, st)
+                                : join_hd<__nv_bfloat16>(jn, blocks, c->head_dim, st);
 }
 
 }  // namespace ftc
