@@ -211,8 +211,8 @@ CallPlan call_plan(const ftc_kv_pages* c, const ftc_page_batch* b, int64_t n_hea
     const int big = rows <= 64 ? 1 : 2;
     if (rows <= 16) {
         add(0, 1, INT_MAX);
-    } else if (b->n_seqs == 1) {
-        add(big, 1, INT_MAX);
+    } else if (b->n_seqs == 1 || (b->max_new > 0 && b->n_tokens == b->n_seqs * b->max_new)) {
+        add(big, 1, INT_MAX);  // sequences of one size
     } else {
         if (gqa <= 16) add(0, 1, 16);
         add(big, gqa <= 16 ? 17 : 1, INT_MAX);

@@ -64,8 +64,9 @@ struct Cfg {
     static constexpr int XB = NG > 1 ? (NG / 2) * MW * 32 * (HD / 2 + 4) * 4 : 0;
     static constexpr int kFixed = 1024 /* alignment */ + QB + XB + 1024 /* barriers, flags */;
     static constexpr int SLOT_ALL = SLOT + (kQ8 ? 2 * KS * 4 : 0);
-    // two CTAs per SM where each still has slots in flight beside the held ones
-    static constexpr int OCC = NW <= 4 && (112 * 1024 - kFixed) / SLOT_ALL >= NG + 4 ? 2 : 1;
+    // two CTAs per SM where each still has slots in flight beside the held
+    // ones, and where 168 registers hold the accumulator (head_dim < 256)
+    static constexpr int OCC = NW <= 4 && HD < 256 && (112 * 1024 - kFixed) / SLOT_ALL >= NG + 4 ? 2 : 1;
     static constexpr int kFit = ((OCC == 2 ? 112 : 224) * 1024 - kFixed) / SLOT_ALL;
     static constexpr int NSLOT = kFit < 24 ? kFit : 24;
     static_assert(NSLOT >= NG + 1, "ring holds every group's slot and one in flight");
@@ -172,6 +173,8 @@ __device__ __forceinline__ float2 load2(const X* p) {
     if constexpr (sizeof(X) == 4) return *reinterpret_cast<const float2*>(p);
     else return unpack<X>(*reinterpret_cast<const uint32_t*>(p));
 }
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
 
 // 16-byte chunk `c` of row `r` in a box tile of K or V.
 template <class F>
@@ -358,6 +361,7 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
             // codes a lane's four are neighbours (one word of the cache row)
             const int kl = F::kQ8 ? 4 * t4 : 2 * t4, kh = F::kQ8 ? 4 * t4 + 2 : 2 * t4 + 8;
             int e0 = 0, e1 = 0;
+            float fa0 = 1.f, fb0 = 1.f, fa1 = 1.f, fb1 = 1.f;
             if constexpr (F::kRowScale) {
                 uint32_t m0 = 0, m1 = 0;
 #pragma unroll
@@ -383,8 +387,10 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                 // the row's largest value lands in [2^14, 2^15)
                 if (m0 > 0 && m0 < 0x7F800000u) e0 = (int)(m0 >> 23) - 141;
                 if (m1 > 0 && m1 < 0x7F800000u) e1 = (int)(m1 >> 23) - 141;
-                c0 = fmaxf(scalbnf(a.c, e0), 1e-38f);
-                c1 = fmaxf(scalbnf(a.c, e1), 1e-38f);
+                fa0 = pow2(-e0 / 2), fb0 = pow2(-e0 - -e0 / 2);
+                fa1 = pow2(-e1 / 2), fb1 = pow2(-e1 - -e1 / 2);
+                c0 = fmaxf(a.c * pow2(e0 / 2) * pow2(e0 - e0 / 2), 1e-38f);
+                c1 = fmaxf(a.c * pow2(e1 / 2) * pow2(e1 - e1 / 2), 1e-38f);
             }
             if (grp == 0) {
 #pragma unroll
@@ -392,11 +398,11 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                     float2 x0 = make_float2(0.f, 0.f), y0 = x0, x1 = x0, y1 = x0;
                     if (va) x0 = load2(qa + 16 * i + kl), y0 = load2(qa + 16 * i + kh);
                     if (vb) x1 = load2(qb + 16 * i + kl), y1 = load2(qb + 16 * i + kh);
-                    if constexpr (F::kRowScale) {
-                        x0.x = scalbnf(x0.x, -e0), x0.y = scalbnf(x0.y, -e0);
-                        y0.x = scalbnf(y0.x, -e0), y0.y = scalbnf(y0.y, -e0);
-                        x1.x = scalbnf(x1.x, -e1), x1.y = scalbnf(x1.y, -e1);
-                        y1.x = scalbnf(y1.x, -e1), y1.y = scalbnf(y1.y, -e1);
+                    if constexpr (F::kRowScale) {  // 2^-e as two factors in range
+                        x0.x = x0.x * fa0 * fb0, x0.y = x0.y * fa0 * fb0;
+                        y0.x = y0.x * fa0 * fb0, y0.y = y0.y * fa0 * fb0;
+                        x1.x = x1.x * fa1 * fb1, x1.y = x1.y * fa1 * fb1;
+                        y1.x = y1.x * fa1 * fb1, y1.y = y1.y * fa1 * fb1;
                     }
                     uint32_t r0[NP], r1[NP], r2[NP], r3[NP];
                     split<OT, NP>(x0.x, x0.y, r0);
@@ -440,38 +446,48 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
             const uint32_t vs_addr = ks_addr + KS * F::ROWB;
 
             // ---- scores: KS / 8 tiles of 8 keys
-            float S[KS / 8][4];
+            // (k outside, so that a piece of q is read once for all of them)
+            float S[KS / 8][4], lo[F::kF32 ? KS / 8 : 1][4];
 #pragma unroll
             for (int n = 0; n < KS / 8; ++n) {
-                float h0[4] = {}, h1[4] = {}, lo[4] = {};
+                S[n][0] = S[n][1] = S[n][2] = S[n][3] = 0.f;
+                if constexpr (F::kF32) lo[n][0] = lo[n][1] = lo[n][2] = lo[n][3] = 0.f;
+            }
 #pragma unroll
-                for (int c4 = 0; c4 < F::ROWB / 64; ++c4) {
-                    uint32_t r[4];
-                    ldsm4(r, ks_addr + chunk_off<F>(8 * n + (lane & 7), 4 * c4 + (lane >> 3)));
-                    constexpr int STEPS = F::kQ8 ? 4 : 2;  // k-steps in four chunks
+            for (int c4 = 0; c4 < F::ROWB / 64; ++c4) {
+                constexpr int STEPS = F::kQ8 ? 4 : 2;  // k-steps in four chunks
+                uint32_t r[KS / 8][4];
 #pragma unroll
-                    for (int st = 0; st < STEPS; ++st) {
+                for (int n = 0; n < KS / 8; ++n)
+                    ldsm4(r[n], ks_addr + chunk_off<F>(8 * n + (lane & 7), 4 * c4 + (lane >> 3)));
+#pragma unroll
+                for (int st = 0; st < STEPS; ++st) {
+                    const uint4* qf = sQ + (mt * NP * (HD / 16) + c4 * STEPS + st) * 32 + lane;
+                    uint4 qv[NP];
+#pragma unroll
+                    for (int q = 0; q < NP; ++q) qv[q] = qf[q * (HD / 16) * 32];
+#pragma unroll
+                    for (int n = 0; n < KS / 8; ++n) {
                         uint32_t b0, b1;
                         if constexpr (F::kQ8) {
-                            const uint32_t u = r[st] ^ 0x80808080u;
+                            const uint32_t u = r[n][st] ^ 0x80808080u;
                             b0 = codes2<0x4140>(u);
                             b1 = codes2<0x4342>(u);
                         } else {
-                            b0 = r[2 * st];
-                            b1 = r[2 * st + 1];
+                            b0 = r[n][2 * st];
+                            b1 = r[n][2 * st + 1];
                         }
-                        const int i = c4 * STEPS + st;
-                        const uint4* qf = sQ + (mt * NP * (HD / 16) + i) * 32 + lane;
-                        if (F::kF32 && (i & 1)) mma16816<F::kHalf>(h1, qf[0], b0, b1);
-                        else mma16816<F::kHalf>(h0, qf[0], b0, b1);
+                        mma16816<F::kHalf>(S[n], qv[0], b0, b1);
 #pragma unroll
-                        for (int n2 = 1; n2 < NP; ++n2)
-                            mma16816<F::kHalf>(lo, qf[n2 * (HD / 16) * 32], b0, b1);
+                        for (int q = 1; q < NP; ++q) mma16816<F::kHalf>(lo[n], qv[q], b0, b1);
                     }
                 }
+            }
+            if constexpr (F::kF32) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    S[n][i] = F::kF32 ? (h0[i] + h1[i]) + lo[i] : h0[i];
+                for (int n = 0; n < KS / 8; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) S[n][i] += lo[n][i];
             }
 
             // ---- the 8-bit scales of this lane's keys
@@ -496,10 +512,10 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const int Ek = min(max((int)(__float_as_uint(top) >> 23) - 126, -126), 126);
                 if (Ek > E) {
-                    mul = E - Ek < -126 ? 0.f : __int_as_float((127 + E - Ek) << 23);
+                    mul = E - Ek < -126 ? 0.f : pow2(E - Ek);
                     E = Ek;
                 }
-                const float f = __int_as_float((127 - E) << 23);
+                const float f = pow2(-E);
 #pragma unroll
                 for (int n = 0; n < KS / 8; ++n) vsc[n][0] *= f, vsc[n][1] *= f;
             }
@@ -677,7 +693,7 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
 
         // ---- join the groups, halving their number per round
         if constexpr (F::kQ8) {
-            const float f = __int_as_float((127 + E) << 23);
+            const float f = pow2(E);
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -853,12 +869,11 @@ PagedSet geom_cfg() {
 }
 
 // The class's shape: 4 warps on 16 rows, 4 warps of 16 rows, and 8 warps of
-// 16 rows where 128 rows of q pieces leave room for the ring.
+// 16 rows (head_dim 256: 4, nine warps leave a thread too few registers).
 template <typename X, typename C, int HD, class Fn>
 auto with_class(int cls, Fn fn) {
     using std::integral_constant;
-    constexpr int np = Cfg<X, C, HD, 1, 4>::NP;
-    constexpr int big = 8 * np * (HD / 16) * 512 <= 128 * 1024 ? 8 : 4;
+    constexpr int big = HD < 256 ? 8 : 4;
     return cls == 0   ? fn(integral_constant<int, 1>(), integral_constant<int, 4>())
            : cls == 1 ? fn(integral_constant<int, 4>(), integral_constant<int, 4>())
                       : fn(integral_constant<int, big>(), integral_constant<int, big>());
