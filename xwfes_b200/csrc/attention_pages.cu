@@ -42,7 +42,9 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 // The pool as [page][KV head and slot][head_dim], boxes of up to 128 bytes by
 // one page's share of a key chunk.
-int page_map(CUtensorMap* m, const void* base, const ftc_kv_pages* c, int key_step) {
+// plain8: rows of 8-bit codes stay as they lie (they are converted, not fed to
+// matrix loads).
+int page_map(CUtensorMap* m, const void* base, const ftc_kv_pages* c, int key_step, bool plain8) {
     auto enc = encode_fn();
     FTC_REQUIRE(enc, FTC_E_CUDA, "ftc_attention_pages: cuTensorMapEncodeTiled unavailable");
     const bool q8 = c->dtype == FTC_KV_Q8;
@@ -61,7 +63,8 @@ int page_map(CUtensorMap* m, const void* base, const ftc_kv_pages* c, int key_st
                : c->dtype == FTC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
             3, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            boxb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            q8 && plain8 ? CU_TENSOR_MAP_SWIZZLE_NONE
+            : boxb == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     FTC_REQUIRE(r == CUDA_SUCCESS, FTC_E_CUDA, "ftc_attention_pages: page tensor map rejected");
     return FTC_OK;
@@ -273,6 +276,7 @@ int attention_pages(const ftc_kv_pages* c, const ftc_page_batch* b, const void* 
                 "ftc_attention_pages: workspace smaller than ftc_attention_pages_workspace_bytes "
                 "or not 256-byte aligned");
     a.q = q;
+    a.v = c->v;
     a.ks = c->k_scale;
     a.vs = c->v_scale;
     a.out = out;

@@ -832,7 +832,7 @@ struct PagedJob {
     cudaStream_t st;
 };
 
-int page_map(CUtensorMap* m, const void* base, const ftc_kv_pages* c, int key_step);
+int page_map(CUtensorMap* m, const void* base, const ftc_kv_pages* c, int key_step, bool plain8);
 
 // Shortest range of chunks worth a CTA of its own, in rounds of its groups.
 constexpr int kLeastRounds = 2;
@@ -845,7 +845,8 @@ int launch_cfg(const PagedJob& j) {
                          "cudaFuncSetAttribute(paged_mma)");
     if (rc) return rc;
     CUtensorMap tk, tv;
-    if ((rc = page_map(&tk, j.c->k, j.c, F::KS)) || (rc = page_map(&tv, j.c->v, j.c, F::KS)))
+    if ((rc = page_map(&tk, j.c->k, j.c, F::KS, false)) ||
+        (rc = page_map(&tv, j.c->v, j.c, F::KS, false)))
         return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)j.set.G);
@@ -866,44 +867,6 @@ template <typename X, typename C, int HD, int MW, int NW>
 PagedSet geom_cfg() {
     using F = Cfg<X, C, HD, MW, NW>;
     return {F::OCC * device_sms(), F::TR};
-}
-
-// The class's shape: 4 warps on 16 rows, 4 warps of 16 rows, and 8 warps of
-// 16 rows (head_dim 256: 4, nine warps leave a thread too few registers).
-template <typename X, typename C, int HD, class Fn>
-auto with_class(int cls, Fn fn) {
-    using std::integral_constant;
-    constexpr int big = HD < 256 ? 8 : 4;
-    return cls == 0   ? fn(integral_constant<int, 1>(), integral_constant<int, 4>())
-           : cls == 1 ? fn(integral_constant<int, 4>(), integral_constant<int, 4>())
-                      : fn(integral_constant<int, big>(), integral_constant<int, big>());
-}
-
-template <typename X, typename C, int HD>
-int launch_class(const PagedJob& j) {
-    return with_class<X, C, HD>(j.cls, [&](auto mw, auto nw) {
-        return launch_cfg<X, C, HD, decltype(mw)::value, decltype(nw)::value>(j);
-    });
-}
-
-template <typename X, typename C, int HD>
-PagedSet geom_class(int cls) {
-    return with_class<X, C, HD>(cls, [&](auto mw, auto nw) {
-        return geom_cfg<X, C, HD, decltype(mw)::value, decltype(nw)::value>();
-    });
-}
-
-template <typename X, typename C>
-int launch_hd(const PagedJob& j) {
-    return j.c->head_dim == 64    ? launch_class<X, C, 64>(j)
-           : j.c->head_dim == 128 ? launch_class<X, C, 128>(j)
-                                  : launch_class<X, C, 256>(j);
-}
-
-template <typename X, typename C>
-PagedSet geom_hd(int64_t hd, int cls) {
-    return hd == 64 ? geom_class<X, C, 64>(cls)
-                    : hd == 128 ? geom_class<X, C, 128>(cls) : geom_class<X, C, 256>(cls);
 }
 
 }  // namespace paged

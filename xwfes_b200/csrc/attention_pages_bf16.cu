@@ -1,5 +1,5 @@
 // attention_pages_bf16.cu -- the paged attention kernels over a bf16 cache.
-#include "attention_pages.cuh"
+#include "paged_classes.cuh"
 
 namespace ftc {
 

@@ -1,5 +1,5 @@
 // attention_pages_q8.cu -- the paged attention kernels over an 8-bit cache.
-#include "attention_pages.cuh"
+#include "paged_classes.cuh"
 
 namespace ftc {
 

@@ -1,0 +1,815 @@
+// attention_pages_tc.cuh -- the paged attention of long chunks with 16-bit
+// queries on the tcgen05 tensor cores.
+//
+// A tile is 256 packed rows, two stages of 128; its keys come 128 at a time.
+// Per stage and key tile, S = Q K^T (128 x 128) and O += P V (128 x head_dim)
+// accumulate in tensor memory: S 128 columns, the weights P written over it as
+// 16-bit A operand, O head_dim columns.  One thread issues all MMAs,
+//   S0(0) S1(0) | PV0(j) S0(j+1) PV1(j) S1(j+1) | ...
+// so that the tensor cores work on one stage while the other's softmax runs.
+// The MMAs of one thread run in order, which is what makes S(j+1) after PV(j)
+// safe on the same columns, and what lets the softmax warps rescale O: when
+// S(j) has arrived, PV(j-1) is done and PV(j) waits for this stage's P.
+// Rescaling is lazy: the reference maximum only moves when a score passes it by
+// 2^8, which f16 weights leave room for (they sit 2^7 up).
+//
+// Warps: 0 brings K and V by TMA, one box per page (V as it lies in the cache:
+// positions by head_dim, the MN-major B operand of PV); 1 issues MMAs; 4-7 and
+// 8-11 are the softmax of the two stages, a thread per row; 12-15 turn 8-bit
+// codes into f16 tiles, and in tiles where some row's mask hides something they
+// take V elements that are not finite out (0 x inf would reach every row),
+// which the rows that see them get back at the end.  8-bit scales stay in fp32:
+// K's multiplies S, V's multiplies P, relative to its running maximum 2^E.
+//
+// What bounds it: per key tile and stage pair the tensor cores need 4 x 512
+// clocks at head_dim 128, and the exponentials, 16 a clock, as many.
+#pragma once
+
+#include <climits>
+
+#include "attention_pages.cuh"
+
+namespace ftc {
+namespace paged {
+
+template <typename X_, typename C_, int HD_>
+struct TcCfg {
+    using X = X_;
+    using C = C_;
+    static constexpr int HD = HD_, TR = 256, KS = 128;
+    static constexpr bool kQ8 = sizeof(C) == 1;
+    using OT = typename std::conditional<std::is_same<C, __nv_bfloat16>::value, __nv_bfloat16,
+                                         __half>::type;
+    static constexpr bool kHalf = std::is_same<OT, __half>::value;
+    static constexpr bool kRowScale = kHalf && !std::is_same<X, __half>::value;
+    static constexpr int SUB = KS * 128;           // 64 dimensions of 128 rows
+    static constexpr int TILE = SUB * (HD / 64);   // K or V tile, 16-bit
+    static constexpr int QB = 2 * TILE;
+    static constexpr int NSL = kQ8 ? (HD == 128 ? 3 : 4) : (HD == 128 ? 4 : 6);
+    static constexpr int RAW = kQ8 ? KS * HD : 0;
+    static constexpr int NR = kQ8 ? 3 : 1;
+    static constexpr int NSC = 3;
+    static constexpr int OFF_RING = 0;
+    static constexpr int OFF_Q = OFF_RING + NSL * TILE;
+    static constexpr int OFF_RAW = OFF_Q + QB;
+    static constexpr int OFF_SC = OFF_RAW + (kQ8 ? NR * RAW : 0);
+    static constexpr int OFF_BAR = OFF_SC + NSC * (kQ8 ? 2 * KS * 4 : 0);
+    static constexpr int SMEM = OFF_BAR + 1024 + 1024;
+    static constexpr int THREADS = 512;
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+    static_assert(NSL * TILE >= Plan<TR, KS>::kSmem, "the plan's prefix sums fit in the ring");
+};
+
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+    return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+}
+__device__ __forceinline__ float f2lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float f2hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t f2add(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t f2mul(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t f2fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// Loads done: ties the registers to the wait, so that no use moves above it.
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                   "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+        "%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,"
+        "%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(
+            taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+// Shared-memory descriptor of V as MN-major B operand, 128-byte swizzle: 64
+// dimensions (128 bytes) of a position side by side, positions 128 bytes
+// apart; leading offset = from one 64 dimensions to the next, stride offset =
+// from 8 positions to the next 8.
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(const void* tile, uint32_t lead) {
+    const uint64_t addr = smem_u32(tile);
+    uint64_t d = 0;
+    d |= (addr >> 4) & 0x3FFFull;
+    d |= (uint64_t)(lead >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= 1ull << 46;
+    d |= 2ull << 61;
+    return d;
+}
+
+__device__ __forceinline__ bool one_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+    if (*dead) return false;
+    if (mbar_wait(bar, parity)) return true;
+    *dead = 1;
+    return false;
+}
+
+// V elements that are not finite, of the positions that a row sees, added to
+// 32 dimensions of its sum.
+template <class F>
+__device__ __noinline__ void add_odd(const PagedArgs& a, const PlanPos& p,
+                                     const TileWork<F::TR, F::KS>& tw, int m, int pos, int d0,
+                                     uint32_t (&s)[32]) {
+    using OT = typename F::OT;
+    for (int j = 0; j < m; ++j) {
+        const int key0 = tw.key0(p.i + j);
+        for (int key = key0; key < key0 + F::KS && key <= pos; ++key) {
+            const int pg = page_of(a.b, p.s, key);
+            if (pg < 0 || !(a.window == 0 || pos - key < a.window || key < a.n_sink)) continue;
+            const uint32_t* v = reinterpret_cast<const uint32_t*>(
+                static_cast<const OT*>(a.v) + (int64_t)pg * a.b.page_stride +
+                ((int64_t)p.kvh * a.b.page_size + (key & (a.b.page_size - 1))) * F::HD + d0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float2 x = unpack<OT>(v[i]);
+                if (!(fabsf(x.x) < INFINITY))
+                    s[2 * i] = __float_as_uint(__uint_as_float(s[2 * i]) + x.x);
+                if (!(fabsf(x.y) < INFINITY))
+                    s[2 * i + 1] = __float_as_uint(__uint_as_float(s[2 * i + 1]) + x.y);
+            }
+        }
+    }
+}
+
+template <class F>
+__global__ void __launch_bounds__(F::THREADS, 1)
+paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+         const __grid_constant__ PagedArgs a, int least) {
+    using X = typename F::X;
+    using C = typename F::C;
+    using OT = typename F::OT;
+    constexpr int HD = F::HD, TR = F::TR, KS = F::KS;
+    using P = Plan<TR, KS>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sRing = smem + F::OFF_RING;
+    uint8_t* sQ = smem + F::OFF_Q;
+    uint8_t* sRaw = smem + F::OFF_RAW;
+    float* sScale = reinterpret_cast<float*>(smem + F::OFF_SC);  // [NSC][K, V][128]
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + F::OFF_BAR);  // 16-bit tiles landed
+    uint64_t* ready = full + F::NSL;     // tile is an operand (converted, cleaned)
+    uint64_t* empty = ready + F::NSL;    // its MMAs are done
+    uint64_t* raw_full = empty + F::NSL;
+    uint64_t* raw_empty = raw_full + F::NR;
+    uint64_t* sc_full = raw_empty + F::NR;  // flags and scales of a key tile
+    uint64_t* sc_empty = sc_full + F::NSC;
+    uint64_t* q_full = sc_empty + F::NSC;  // [2]
+    uint64_t* s_full = q_full + 2;
+    uint64_t* p_full = s_full + 2;
+    uint64_t* o_full = p_full + 2;
+    uint64_t* o_empty = o_full + 2;
+    uint64_t* drain = o_empty + 2;
+    volatile int* dead = reinterpret_cast<volatile int*>(drain + 1);
+    volatile int* odd = dead + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(dead) + 2);
+    int* sFlag = const_cast<int*>(dead) + 4;  // [NSC]
+    PlanPos* sPos = reinterpret_cast<PlanPos*>(sFlag + 4);
+    int64_t* sPre = reinterpret_cast<int64_t*>(sRing);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < F::NSL; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&ready[i], 4);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < F::NR; ++i) {
+            mbar_init(&raw_full[i], 1);
+            mbar_init(&raw_empty[i], 4);
+        }
+        for (int i = 0; i < F::NSC; ++i) {
+            mbar_init(&sc_full[i], 1);
+            mbar_init(&sc_empty[i], 12);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], 4);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_full[i], 1);
+            mbar_init(&o_empty[i], 4);
+        }
+        mbar_init(drain, 1);
+        *dead = 0;
+        *odd = 0;
+        mbar_fence_init();
+    }
+    if (!a.second) grid_dependency_wait();  // as paged_mma
+    grid_launch_dependents();
+    __syncthreads();
+
+    const int64_t W = P::scan(a, sPre);
+    const int64_t L = plan_share(W, (int)gridDim.x, 1, least);
+    const int64_t u0 = (int64_t)blockIdx.x * L;
+    if (u0 >= W) {
+        if (threadIdx.x == 0) a.cut[blockIdx.x].pieces = 0;
+        if (a.second) grid_dependency_wait();
+        return;
+    }
+    const int total = (int)min(L, W - u0);
+    if (warp == 0) {
+        const PlanPos p = P::locate(a, sPre, u0);
+        if (lane == 0) *sPos = p;
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    fence_proxy_async_smem();  // the prefix sums are done with: the ring may be filled
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    PlanPos p = *sPos;
+
+    if (warp == 0) {
+        // -------------------------------------------------------- producer
+        if (lane == 0) {
+            prefetch_tensormap(&tk);
+            prefetch_tensormap(&tv);
+        }
+        const int box = min(a.b.page_size, KS), boxes = KS / box;
+        constexpr int NBOX = F::kQ8 ? 1 : HD / 64;  // 128-byte columns
+        uint32_t it = 0;
+        for (int left = total; left > 0 && !*dead;) {
+            const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
+            const int m = min(tw.count - p.i, left);
+            for (int j = 0; j < m; ++j, ++it) {
+                const int key0 = tw.key0(p.i + j);
+                const int id = lane < boxes ? page_of(a.b, p.s, key0 + lane * box) : -1;
+                const unsigned on = __ballot_sync(0xffffffffu, id >= 0);
+                const int y = p.kvh * a.b.page_size + (key0 & (a.b.page_size - 1));
+                const int ss = it % F::NSC;
+                if (!ring_wait(&sc_empty[ss], ((it / F::NSC) & 1) ^ 1, dead)) break;
+                if (lane == 0) {
+                    int flag = 0;  // a bit per 16 positions
+                    for (int b = 0; b < boxes; ++b)
+                        if ((on >> b) & 1) flag |= ((1 << (box / 16)) - 1) << (b * box / 16);
+                    sFlag[ss] = flag;
+                    if constexpr (F::kQ8)
+                        mbar_arrive_expect_tx(&sc_full[ss], __popc(on) * 2 * box * 4);
+                    else mbar_arrive(&sc_full[ss]);
+                }
+                __syncwarp();
+                if constexpr (F::kQ8) {
+                    if (id >= 0) {
+                        const int64_t src = (int64_t)id * a.b.scale_stride + y;
+                        bulk_copy(sScale + (ss * 2 + 0) * KS + lane * box, a.ks + src, box * 4,
+                                  &sc_full[ss]);
+                        bulk_copy(sScale + (ss * 2 + 1) * KS + lane * box, a.vs + src, box * 4,
+                                  &sc_full[ss]);
+                    }
+                }
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    const uint32_t t = 2 * it + kv;
+                    uint64_t* bar;
+                    uint8_t* dst;
+                    if constexpr (F::kQ8) {
+                        const int s = t % F::NR;
+                        if (!ring_wait(&raw_empty[s], ((t / F::NR) & 1) ^ 1, dead)) break;
+                        bar = &raw_full[s];
+                        dst = sRaw + s * F::RAW;
+                        if (lane == 0) mbar_arrive_expect_tx(bar, F::RAW);
+                    } else {
+                        const int s = t % F::NSL;
+                        if (!ring_wait(&empty[s], ((t / F::NSL) & 1) ^ 1, dead)) break;
+                        bar = &full[s];
+                        dst = sRing + s * F::TILE;
+                        if (lane == 0) mbar_arrive_expect_tx(bar, F::TILE);
+                    }
+                    __syncwarp();
+                    const int b = lane / NBOX, col = lane % NBOX;
+                    const int pg = __shfl_sync(0xffffffffu, id, b);
+                    if (b < boxes)  // past the last page: zeros
+                        tma_box(dst + col * F::SUB + b * box * (F::kQ8 ? HD : 128),
+                                kv ? &tv : &tk, col * 64, y, pg < 0 ? a.b.n_pages : pg, bar);
+                    __syncwarp();
+                }
+                if (*dead) break;
+            }
+            left -= m;
+            if (left > 0) P::next_tile(a, p);
+        }
+        if (*dead && lane == 0) {  // let issued copies land before the CTA leaves
+            for (int i = 0; i < F::NSC; ++i) {
+                mbar_wait(&sc_full[i], 0);
+                mbar_wait(&sc_full[i], 1);
+            }
+            for (int i = 0; i < (F::kQ8 ? F::NR : F::NSL); ++i) {
+                uint64_t* b = F::kQ8 ? &raw_full[i] : &full[i];
+                mbar_wait(b, 0);
+                mbar_wait(b, 1);
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------- MMA
+        if (lane == 0) {
+            constexpr uint32_t fmt = F::kHalf ? 0u : 1u;
+            constexpr uint32_t id_s = idesc_f16(fmt, 128, KS);
+            constexpr uint32_t id_o = idesc_f16(fmt, 128, HD) | (1u << 16);  // B is MN-major
+            uint32_t it = 0, np[2] = {0, 0}, no[2] = {0, 0};  // no: segments of a stage
+            auto operand = [&](uint32_t t) -> uint8_t* {
+                const int s = t % F::NSL;
+                uint64_t* b = F::kQ8 || (t & 1) ? &ready[s] : &full[s];
+                // ready of a 16-bit ring only counts V tiles (odd t, even NSL)
+                if (!one_wait(b, (t / F::NSL) & 1, dead)) return nullptr;
+                tc_fence_after();
+                return sRing + s * F::TILE;
+            };
+            auto scores = [&](int i, const uint8_t* kt) {
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const uint64_t dq = smem_desc_k_sw128(sQ + i * F::TILE + (k / 4) * F::SUB);
+                    const uint64_t dk = smem_desc_k_sw128(kt + (k / 4) * F::SUB);
+                    umma_f16_ss(tmem + i * 128, dq + 2 * (k % 4), dk + 2 * (k % 4), id_s, k != 0);
+                }
+                umma_commit(&s_full[i]);
+            };
+            for (int left = total; left > 0 && !*dead;) {
+                const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
+                const int m = min(tw.count - p.i, left);
+                const int stages = p.n * a.gqa - p.t * TR > 128 ? 2 : 1;
+                const uint8_t* kt = operand(2 * it);
+                if (!kt) break;
+                for (int i = 0; i < stages; ++i) {
+                    if (!one_wait(&q_full[i], no[i] & 1, dead)) break;
+                    tc_fence_after();
+                    scores(i, kt);
+                }
+                umma_commit(&empty[2 * it % F::NSL]);
+                for (int j = 0; j < m; ++j) {
+                    const uint8_t* vt = nullptr;
+                    kt = nullptr;
+                    for (int i = 0; i < stages; ++i) {
+                        if (!one_wait(&p_full[i], np[i]++ & 1, dead)) break;
+                        if (i == 0 && !(vt = operand(2 * (it + j) + 1))) break;
+                        if (j == 0 && !one_wait(&o_empty[i], (no[i] & 1) ^ 1, dead)) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = 0; k < KS / 16; ++k)
+                            umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k,
+                                        smem_desc_mn_sw128(vt + k * 2048, F::SUB), id_o,
+                                        j != 0 || k != 0);
+                        if (j + 1 < m) {
+                            if (i == 0 && !(kt = operand(2 * (it + j + 1)))) break;
+                            scores(i, kt);
+                        } else {
+                            umma_commit(&o_full[i]);
+                            ++no[i];
+                        }
+                    }
+                    if (*dead) break;
+                    umma_commit(&empty[(2 * (it + j) + 1) % F::NSL]);
+                    if (j + 1 < m) umma_commit(&empty[2 * (it + j + 1) % F::NSL]);
+                }
+                if (*dead) break;
+                it += m;
+                left -= m;
+                if (left > 0) P::next_tile(a, p);
+            }
+            if (*dead) {  // nothing of this CTA may be in flight when it leaves
+                umma_commit(drain);
+                mbar_wait(drain, 0);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 12) {
+        // --------------------------------------------- operand preparation
+        const int w = warp - 12;
+        uint32_t it = 0;
+        for (int left = total; left > 0;) {
+            const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
+            const int m = min(tw.count - p.i, left);
+            for (int j = 0; j < m; ++j, ++it) {
+                const int ss = it % F::NSC;
+                ring_wait(&sc_full[ss], (it / F::NSC) & 1, dead);
+                const int flag = sFlag[ss];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sc_empty[ss]);
+                if constexpr (F::kQ8) {
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const uint32_t t = 2 * it + kv;
+                        const int rs = t % F::NR, s = t % F::NSL;
+                        if (!ring_wait(&raw_full[rs], (t / F::NR) & 1, dead)) continue;
+                        if (!ring_wait(&empty[s], ((t / F::NSL) & 1) ^ 1, dead)) continue;
+                        const uint8_t* src = sRaw + rs * F::RAW;
+                        uint8_t* dst = sRing + s * F::TILE;
+                        constexpr int LPR = HD / 16;        // lanes per row
+                        constexpr int RPI = 32 / LPR;       // rows per step
+                        const int c = lane % LPR;           // 16 codes of a row
+                        const bool swap = (c >> 2) & 1;     // other bank half first
+#pragma unroll 4
+                        for (int r = w * 32 + lane / LPR; r < w * 32 + 32; r += RPI) {
+                            const uint4 u = *reinterpret_cast<const uint4*>(src + r * HD + 16 * c);
+                            const uint32_t x0 = u.x ^ 0x80808080u, x1 = u.y ^ 0x80808080u;
+                            const uint32_t x2 = u.z ^ 0x80808080u, x3 = u.w ^ 0x80808080u;
+                            const uint4 lo = make_uint4(codes2<0x4140>(x0), codes2<0x4342>(x0),
+                                                        codes2<0x4140>(x1), codes2<0x4342>(x1));
+                            const uint4 hi = make_uint4(codes2<0x4140>(x2), codes2<0x4342>(x2),
+                                                        codes2<0x4140>(x3), codes2<0x4342>(x3));
+                            uint8_t* row = dst + (c >> 2) * F::SUB + r * 128;
+                            const int ch = 2 * (c & 3);
+                            *reinterpret_cast<uint4*>(row + (((ch + swap) ^ (r & 7)) << 4)) =
+                                swap ? hi : lo;
+                            *reinterpret_cast<uint4*>(row + (((ch + !swap) ^ (r & 7)) << 4)) =
+                                swap ? lo : hi;
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(&ready[s]);
+                            mbar_arrive(&raw_empty[rs]);
+                        }
+                    }
+                } else {
+                    const uint32_t t = 2 * it + 1;
+                    const int s = t % F::NSL;
+                    if (!ring_wait(&full[s], (t / F::NSL) & 1, dead)) continue;
+                    const int key0 = tw.key0(p.i + j);
+                    const bool whole = flag == 0xFF && key0 + KS - 1 <= tw.p_first &&
+                                       (a.window == 0 || tw.p_last - key0 < a.window ||
+                                        key0 + KS - 1 < a.n_sink);
+                    if (!whole) {
+                        constexpr uint32_t kInf = F::kHalf ? 0x7C007C00u : 0x7F807F80u;
+                        constexpr uint32_t kOne = F::kHalf ? 0x04000400u : 0x00800080u;
+                        uint4* v = reinterpret_cast<uint4*>(sRing + s * F::TILE);
+#pragma unroll 4
+                        for (int q = w * 32 + lane; q < F::TILE / 16; q += 128) {
+                            uint4 u = v[q];
+                            uint32_t* x = reinterpret_cast<uint32_t*>(&u);
+                            uint32_t z = 0;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) z |= (x[i] & kInf) + kOne;
+                            if (z & 0x80008000u) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const uint32_t b = ((x[i] & kInf) + kOne) & 0x80008000u;
+                                    x[i] &= ~((b & 0x8000u ? 0xFFFFu : 0u) |
+                                              (b & 0x80000000u ? 0xFFFF0000u : 0u));
+                                }
+                                v[q] = u;
+                                *odd = 1;
+                            }
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive(&ready[s]);
+                }
+            }
+            left -= m;
+            if (left > 0) P::next_tile(a, p);
+        }
+    } else if (warp >= 4) {
+        // --------------------------------------------------------- softmax
+        const int st = warp >= 8 ? 1 : 0;
+        const int r = (warp & 3) * 32 + lane;  // row of the stage, TMEM lane
+        const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + st * 128;
+        const uint32_t tO = tS - st * 128 + 256 + st * 128;
+        uint32_t it = 0, ns = 0, no = 0;
+        bool owner = false;
+        for (int left = total; left > 0;) {
+            const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
+            const int m = min(tw.count - p.i, left);
+            const bool cut_l = p.i > 0, cut_r = p.i + m < tw.count;
+            const int rows = p.n * a.gqa;
+            const bool active = rows - p.t * TR > st * 128;
+            const int pr = p.t * TR + st * 128 + r;  // packed row
+            const bool live = pr < rows;
+            const int tok = live ? pr / a.gqa : 0;
+            const int h = p.kvh * a.gqa + pr - tok * a.gqa;
+            const int pos = live ? p.len - p.n + tok : -1;
+            const int64_t off = (int64_t)(p.row + tok) * a.out_stride + (int64_t)h * HD;
+            float c = a.c;
+
+            // q row into the K-major operand tile
+            if (active) {
+                const X* q = static_cast<const X*>(a.q) + (int64_t)(p.row + tok) * a.q_stride +
+                             (int64_t)h * HD;
+                uint8_t* dst = sQ + st * F::TILE + r * 128;
+                int e = 0;
+                if constexpr (F::kRowScale) {
+                    uint32_t top = 0;
+                    if (live) {
+#pragma unroll
+                        for (int k = 0; k < HD / 8; ++k) {
+                            const uint4 u = reinterpret_cast<const uint4*>(q)[k];
+                            top = max(top, max(max((u.x << 16) & 0x7FFF0000u, u.x & 0x7FFF0000u),
+                                               max((u.y << 16) & 0x7FFF0000u, u.y & 0x7FFF0000u)));
+                            top = max(top, max(max((u.z << 16) & 0x7FFF0000u, u.z & 0x7FFF0000u),
+                                               max((u.w << 16) & 0x7FFF0000u, u.w & 0x7FFF0000u)));
+                        }
+                    }
+                    // the row's largest value lands in [2^14, 2^15)
+                    if (top > 0 && top < 0x7F800000u) e = (int)(top >> 23) - 141;
+                    c = fmaxf(a.c * pow2(e / 2) * pow2(e - e / 2), 1e-38f);
+                }
+                const float fa = pow2(-e / 2), fb = pow2(-e - -e / 2);
+#pragma unroll
+                for (int k = 0; k < HD / 8; ++k) {
+                    uint4 u = live ? reinterpret_cast<const uint4*>(q)[k] : make_uint4(0, 0, 0, 0);
+                    if constexpr (F::kRowScale) {
+                        uint32_t* x = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 v = unpack<X>(x[i]);
+                            x[i] = pack<OT>(v.x * fa * fb, v.y * fa * fb);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(dst + (k / 8) * F::SUB + (((k % 8) ^ (r & 7)) << 4)) =
+                        u;
+                }
+                fence_proxy_async_smem();
+            }
+            __syncwarp();
+            if (active && lane == 0) mbar_arrive(&q_full[st]);
+
+            // positions of this warp's rows, for the mask tests
+            const int wr = p.t * TR + st * 128 + (warp & 3) * 32;
+            const int p_lo = p.len - p.n + min(wr, rows - 1) / a.gqa;
+            const int p_hi = p.len - p.n + min(wr + 31, rows - 1) / a.gqa;
+            constexpr float kUp = F::kHalf ? 7.f : 0.f;
+            float M = -INFINITY;  // reference maximum (log2)
+            int E = F::kQ8 ? -90 : 0;
+            uint64_t l2 = 0;      // two partial sums of weights
+            for (int j = 0; j < m; ++j, ++it) {
+                const int ss = it % F::NSC;
+                ring_wait(&sc_full[ss], (it / F::NSC) & 1, dead);
+                if (active && ring_wait(&s_full[st], ns++ & 1, dead)) {
+                    tc_fence_after();
+                    const int key0 = tw.key0(p.i + j);
+                    const int flag = sFlag[ss];
+                    const float4* ksc = reinterpret_cast<const float4*>(sScale + ss * 2 * KS);
+                    const float4* vsc = ksc + KS / 4;
+                    const bool whole = flag == 0xFF && key0 + KS - 1 <= p_lo &&
+                                       (a.window == 0 || p_hi - key0 < a.window ||
+                                        key0 + KS - 1 < a.n_sink);
+                    // ---- the row's maximum (masked scores go back as -inf)
+                    float mx = -INFINITY;
+                    uint32_t s[32];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        tmem_ld_32x32b_x32(tS + 32 * q, s);
+                        tmem_ld_done(s);
+                        if (!whole) {
+                            const int hi = pos - key0 - 32 * q;
+                            const int lo = a.window > 0 ? hi - a.window + 1 : INT_MIN;
+                            const int sk = a.n_sink - key0 - 32 * q;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const bool on = (flag >> (2 * q + i / 16)) & 1;
+                                if (!(on && i <= hi && (i >= lo || i < sk)))
+                                    s[i] = 0xFF800000u;
+                            }
+                            tmem_st_x32(tS + 32 * q, s);
+                        }
+                        float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const uint32_t* u = s + i;
+                            float v0 = __uint_as_float(s[i]), v1 = __uint_as_float(s[i + 1]);
+                            float v2 = __uint_as_float(s[i + 2]), v3 = __uint_as_float(s[i + 3]);
+                            if constexpr (F::kQ8) {
+                                const float4 k4 = ksc[8 * q + i / 4];
+                                const uint64_t a2 = f2mul(f2(v0, v1), f2(k4.x, k4.y));
+                                const uint64_t b2 = f2mul(f2(v2, v3), f2(k4.z, k4.w));
+                                v0 = f2lo(a2), v1 = f2hi(a2), v2 = f2lo(b2), v3 = f2hi(b2);
+                                if (!whole) {  // hidden, whatever the scale there
+                                    if (u[0] == 0xFF800000u) v0 = -INFINITY;
+                                    if (u[1] == 0xFF800000u) v1 = -INFINITY;
+                                    if (u[2] == 0xFF800000u) v2 = -INFINITY;
+                                    if (u[3] == 0xFF800000u) v3 = -INFINITY;
+                                }
+                            }
+                            m0 = fmaxf(m0, fmaxf(v0, v1));
+                            m1 = fmaxf(m1, fmaxf(v2, v3));
+                        }
+                        mx = fmaxf(mx, fmaxf(m0, m1));
+                    }
+                    if (!whole) tmem_st_wait();
+                    mx *= c;
+                    int Et = E;
+                    if constexpr (F::kQ8) {
+                        // V's largest scale in this tile, of positions some row may see
+                        float top = 0.f;
+                        const float4 v4 = vsc[lane];
+                        if ((flag >> (lane / 4)) & 1) {
+                            const int k = key0 + 4 * lane;
+                            if (k <= tw.p_last) top = fabsf(v4.x);
+                            if (k + 1 <= tw.p_last) top = fmaxf(top, fabsf(v4.y));
+                            if (k + 2 <= tw.p_last) top = fmaxf(top, fabsf(v4.z));
+                            if (k + 3 <= tw.p_last) top = fmaxf(top, fabsf(v4.w));
+                        }
+                        uint32_t tb = __float_as_uint(top);
+                        if (tb > 0x7F800000u) tb = 0;  // a NaN scale says nothing
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1)
+                            tb = max(tb, __shfl_xor_sync(0xffffffffu, tb, o));
+                        Et = max(E, min((int)(tb >> 23) - 126, 126));
+                    }
+                    if (__any_sync(0xffffffffu, mx > M + 8.f || Et > E)) {
+                        const float N = fmaxf(M, mx);
+                        // (0 while nothing was seen; the accumulator is not set before j = 1)
+                        const float f = M == -INFINITY ? 0.f : ex2(M - N + (float)(E - Et));
+                        M = N;
+                        E = Et;
+                        l2 = f2mul(l2, f2(f, f));
+                        if (j > 0) {
+#pragma unroll
+                            for (int q = 0; q < HD / 32; ++q) {
+                                tmem_ld_32x32b_x32(tO + 32 * q, s);
+                                tmem_ld_done(s);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    s[i] = __float_as_uint(__uint_as_float(s[i]) * f);
+                                tmem_st_x32(tO + 32 * q, s);
+                            }
+                        }
+                    }
+                    // ---- weights 2^(z - D), packed over the scores
+                    const float D = kUp - (M == -INFINITY ? 0.f : M) - (float)(F::kQ8 ? E : 0);
+                    const uint64_t c2 = f2(c, c), d2 = f2(D, D);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        tmem_ld_32x32b_x32(tS + 32 * q, s);
+                        tmem_ld_done(s);
+                        uint32_t w[16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            uint64_t z0 = f2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                            uint64_t z1 = f2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                            if constexpr (F::kQ8) {
+                                const float4 k4 = ksc[8 * q + i / 4];
+                                z0 = f2mul(z0, f2(k4.x, k4.y));
+                                z1 = f2mul(z1, f2(k4.z, k4.w));
+                                if (!whole) {  // -inf times a scale of a hidden position
+                                    z0 = f2(s[i] == 0xFF800000u ? -INFINITY : f2lo(z0),
+                                            s[i + 1] == 0xFF800000u ? -INFINITY : f2hi(z0));
+                                    z1 = f2(s[i + 2] == 0xFF800000u ? -INFINITY : f2lo(z1),
+                                            s[i + 3] == 0xFF800000u ? -INFINITY : f2hi(z1));
+                                }
+                            }
+                            z0 = f2fma(z0, c2, d2);
+                            z1 = f2fma(z1, c2, d2);
+                            float w0 = ex2(f2lo(z0)), w1 = ex2(f2hi(z0));
+                            float w2 = ex2(f2lo(z1)), w3 = ex2(f2hi(z1));
+                            l2 = f2add(l2, f2add(f2(w0, w1), f2(w2, w3)));
+                            if constexpr (F::kQ8) {
+                                const float4 v4 = vsc[8 * q + i / 4];
+                                if (!whole) {
+                                    w0 = w0 == 0.f ? 0.f : w0 * v4.x;
+                                    w1 = w1 == 0.f ? 0.f : w1 * v4.y;
+                                    w2 = w2 == 0.f ? 0.f : w2 * v4.z;
+                                    w3 = w3 == 0.f ? 0.f : w3 * v4.w;
+                                } else {
+                                    const uint64_t y0 = f2mul(f2(w0, w1), f2(v4.x, v4.y));
+                                    const uint64_t y1 = f2mul(f2(w2, w3), f2(v4.z, v4.w));
+                                    w0 = f2lo(y0), w1 = f2hi(y0), w2 = f2lo(y1), w3 = f2hi(y1);
+                                }
+                            }
+                            w[i / 2] = pack<OT>(w0, w1);
+                            w[i / 2 + 1] = pack<OT>(w2, w3);
+                        }
+                        tmem_st_x16(tS + 16 * q, w);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[st]);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sc_empty[ss]);
+            }
+
+            // ---- the finished rows, or this piece of them
+            if (active && ring_wait(&o_full[st], no++ & 1, dead)) {
+                tc_fence_after();
+                const bool piece = cut_l || cut_r;
+                const float l = f2lo(l2) + f2hi(l2);
+                const float inv = piece ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                const int64_t pslot = 2 * (int64_t)blockIdx.x + (cut_l ? 0 : 1);
+                float* part = a.part + (pslot * TR + st * 128 + r) * HD;
+                if (piece)
+                    a.stat[pslot * TR + st * 128 + r] =
+                        make_float2(M + (float)(F::kQ8 ? E : 0), l);
+                X* o = static_cast<X*>(a.out) + off;
+#pragma unroll
+                for (int q = 0; q < HD / 32; ++q) {
+                    uint32_t s[32];
+                    tmem_ld_32x32b_x32(tO + 32 * q, s);
+                    tmem_ld_done(s);
+                    if (!F::kQ8 && *odd && live)
+                        add_odd<F>(a, p, tw, m, pos, 32 * q, s);
+                    if (piece) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4*>(part + 32 * q + i) =
+                                make_uint4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+                    } else if (live) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint32_t y[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                y[k] = pack<X>(__uint_as_float(s[i + 2 * k]) * inv,
+                                               __uint_as_float(s[i + 2 * k + 1]) * inv);
+                            *reinterpret_cast<uint4*>(o + 32 * q + i) =
+                                make_uint4(y[0], y[1], y[2], y[3]);
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&o_empty[st]);
+            }
+            if (cut_r && !cut_l) {
+                owner = true;
+                if (threadIdx.x == 128) {
+                    const int64_t end = u0 + (total - left) + tw.count;
+                    CutTile ct;
+                    ct.pieces = (int)((end - 1) / L - blockIdx.x) + 1;
+                    ct.row = p.row;
+                    ct.kvh = p.kvh;
+                    ct.r0 = p.t * TR;
+                    ct.rows = min(rows - p.t * TR, TR);
+                    a.cut[blockIdx.x] = ct;
+                }
+            }
+            left -= m;
+            if (left > 0) P::next_tile(a, p);
+        }
+        if (!owner && threadIdx.x == 128) a.cut[blockIdx.x].pieces = 0;
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, 512);
+    if (a.second) grid_dependency_wait();
+}
+
+template <typename X, typename C, int HD>
+int launch_tc(const PagedJob& j) {
+    using F = TcCfg<X, C, HD>;
+    auto fn = paged_tc<F>;
+    int rc = opt_in_smem(reinterpret_cast<const void*>(fn), F::SMEM,
+                         "cudaFuncSetAttribute(paged_tc)");
+    if (rc) return rc;
+    CUtensorMap tk, tv;
+    if ((rc = page_map(&tk, j.c->k, j.c, F::KS, true)) ||
+        (rc = page_map(&tv, j.c->v, j.c, F::KS, true)))
+        return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)j.set.G);
+    cfg.blockDim = dim3(F::THREADS);
+    cfg.dynamicSmemBytes = F::SMEM;
+    cfg.stream = j.st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tk, tv, j.a, 2);
+    if (e != cudaSuccess) return cuda_error(e, "launch paged_tc");
+    return FTC_OK;
+}
+
+}  // namespace paged
+}  // namespace ftc

@@ -1,0 +1,60 @@
+// paged_classes.cuh -- the kernel of each class of sequences, for every type.
+#pragma once
+
+#include "attention_pages_tc.cuh"
+
+namespace ftc {
+namespace paged {
+
+// Class 2 runs on tcgen05 with 16-bit queries: fp32 ones need their sums kept
+// out of the matrix unit's accumulator, and head_dim 256 its tensor memory.
+template <typename X, int HD>
+constexpr bool kTc = sizeof(X) == 2 && HD < 256;
+
+// The class's shape elsewhere: 4 warps on 16 rows, 4 warps of 16 rows, and 8
+// warps of 16 rows (head_dim 256: 4, nine warps leave a thread too few
+// registers).
+template <typename X, typename C, int HD, class Fn>
+auto with_class(int cls, Fn fn) {
+    using std::integral_constant;
+    constexpr int big = HD < 256 ? 8 : 4;
+    return cls == 0   ? fn(integral_constant<int, 1>(), integral_constant<int, 4>())
+           : cls == 1 ? fn(integral_constant<int, 4>(), integral_constant<int, 4>())
+                      : fn(integral_constant<int, big>(), integral_constant<int, big>());
+}
+
+template <typename X, typename C, int HD>
+int launch_class(const PagedJob& j) {
+    if constexpr (kTc<X, HD>) {
+        if (j.cls == 2) return launch_tc<X, C, HD>(j);
+    }
+    return with_class<X, C, HD>(j.cls, [&](auto mw, auto nw) {
+        return launch_cfg<X, C, HD, decltype(mw)::value, decltype(nw)::value>(j);
+    });
+}
+
+template <typename X, typename C, int HD>
+PagedSet geom_class(int cls) {
+    if constexpr (kTc<X, HD>) {
+        if (cls == 2) return {device_sms(), TcCfg<X, C, HD>::TR};
+    }
+    return with_class<X, C, HD>(cls, [&](auto mw, auto nw) {
+        return geom_cfg<X, C, HD, decltype(mw)::value, decltype(nw)::value>();
+    });
+}
+
+template <typename X, typename C>
+int launch_hd(const PagedJob& j) {
+    return j.c->head_dim == 64    ? launch_class<X, C, 64>(j)
+           : j.c->head_dim == 128 ? launch_class<X, C, 128>(j)
+                                  : launch_class<X, C, 256>(j);
+}
+
+template <typename X, typename C>
+PagedSet geom_hd(int64_t hd, int cls) {
+    return hd == 64 ? geom_class<X, C, 64>(cls)
+                    : hd == 128 ? geom_class<X, C, 128>(cls) : geom_class<X, C, 256>(cls);
+}
+
+}  // namespace paged
+}  // namespace ftc

@@ -31,6 +31,7 @@ struct CutTile {
 struct PagedArgs {
     PageView b;
     const void* q;
+    const void* v;         // the V pool
     void* out;
     const float *ks, *vs;  // 8-bit scales
     int64_t q_stride, out_stride;
