@@ -125,24 +125,33 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join(const JoinArgs a) 
             wl = st.y * w;
         }
         const int n = min(32, ct.pieces - k0);
-#pragma unroll 8
-        for (int k = 0; k < n; ++k) {
-            const float wk = __shfl_sync(0xffffffffu, w, k);
-            l += __shfl_sync(0xffffffffu, wl, k);
-            const float* p = s.part + (slot(k0 + k) * s.TR + r) * HD + E * lane;
-            float x[E];
-            if constexpr (E == 2) {
-                const float2 v = *reinterpret_cast<const float2*>(p);
-                x[0] = v.x, x[1] = v.y;
-            } else {
+        for (int k1 = 0; k1 < n; k1 += 4) {
+            float x[4][E];  // four pieces in flight
 #pragma unroll
-                for (int i = 0; i < E; i += 4) {
-                    const float4 v = *reinterpret_cast<const float4*>(p + i);
-                    x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) x[k][i] = 0.f;
+                if (k1 + k >= n) continue;
+                const float* p = s.part + (slot(k0 + k1 + k) * s.TR + r) * HD + E * lane;
+                if constexpr (E == 2) {
+                    const float2 v = *reinterpret_cast<const float2*>(p);
+                    x[k][0] = v.x, x[k][1] = v.y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < E; i += 4) {
+                        const float4 v = *reinterpret_cast<const float4*>(p + i);
+                        x[k][i] = v.x, x[k][i + 1] = v.y, x[k][i + 2] = v.z, x[k][i + 3] = v.w;
+                    }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < E; ++i) acc[i] = fmaf(x[i], wk, acc[i]);
+            for (int k = 0; k < 4; ++k) {
+                const float wk = __shfl_sync(0xffffffffu, w, k1 + k);
+                if (k1 + k >= n) break;
+                l += __shfl_sync(0xffffffffu, wl, k1 + k);
+#pragma unroll
+                for (int i = 0; i < E; ++i) acc[i] = fmaf(x[k][i], wk, acc[i]);
+            }
         }
     }
     const int pr = ct.r0 + r, t = pr / a.gqa, h = ct.kvh * a.gqa + pr - t * a.gqa;
@@ -181,8 +190,8 @@ int join_hd(const JoinArgs& a, int blocks, int64_t hd, cudaStream_t st) {
 }
 
 // The launches of a call: which sequences (by packed rows) go to which class.
-// Decode sequences, 16 rows or fewer, and chunks differ too much for one
-// shape; a batch that may hold both gets two launches.
+// Decode sequences and chunks differ too much for one shape; a batch that may
+// hold both gets two launches.
 struct CallPlan {
     int n = 0;
     int cls[2], min_rows[2], max_rows[2];
@@ -211,14 +220,14 @@ CallPlan call_plan(const ftc_kv_pages* c, const ftc_page_batch* b, int64_t n_hea
                    up256(slots * (size_t)c->head_dim * sizeof(float));
         ++p.n;
     };
-    const int big = rows <= 64 ? 1 : 2;
-    if (rows <= 16) {
-        add(0, 1, INT_MAX);
-    } else if (b->n_seqs == 1 || (b->max_new > 0 && b->n_tokens == b->n_seqs * b->max_new)) {
-        add(big, 1, INT_MAX);  // sequences of one size
+    auto cls_of = [](int64_t r) { return r <= 8 ? 0 : r <= 16 ? 1 : r <= 64 ? 2 : 3; };
+    const int big = cls_of(rows), one = cls_of(gqa);
+    if (big <= 1 || one >= 2 || b->n_seqs == 1 ||
+        (b->max_new > 0 && b->n_tokens == b->n_seqs * b->max_new)) {
+        add(big, 1, INT_MAX);  // few rows, or sequences of one size
     } else {
-        if (gqa <= 16) add(0, 1, 16);
-        add(big, gqa <= 16 ? 17 : 1, INT_MAX);
+        add(one, 1, one == 0 ? 8 : 16);
+        add(big, one == 0 ? 9 : 17, INT_MAX);
     }
     return p;
 }

@@ -42,11 +42,14 @@
 namespace ftc {
 namespace paged {
 
-template <typename X, typename C, int HD_, int MW_, int NW_>
+template <typename X_, typename C_, int HD_, int NT_, int MW_, int NW_>
 struct Cfg {
-    static constexpr int HD = HD_, MW = MW_, NW = NW_;
-    static constexpr int NG = NW / MW;  // warp groups
-    static constexpr int TR = 16 * MW;  // packed rows per tile
+    using X = X_;
+    using C = C_;
+    static constexpr int HD = HD_, NT = NT_, MW = MW_, NW = NW_;
+    static constexpr int NG = NW / MW;      // warp groups
+    static constexpr int WR = 8 * NT;       // packed rows per warp
+    static constexpr int TR = WR * MW;      // packed rows per tile
     using OT = typename std::conditional<std::is_same<C, __nv_bfloat16>::value, __nv_bfloat16,
                                          __half>::type;
     static constexpr bool kF32 = sizeof(X) == 4, kQ8 = sizeof(C) == 1;
@@ -60,22 +63,28 @@ struct Cfg {
     // slots of about 8 KB: each of the NW warps holds one while it computes
     static constexpr int KS = 64 * ROWB <= 8192 ? 32 : 16;
     static constexpr int SLOT = 2 * KS * ROWB;
-    static constexpr int QB = MW * NP * (HD / 16) * 512;
-    static constexpr int XB = NG > 1 ? (NG / 2) * MW * 32 * (HD / 2 + 4) * 4 : 0;
-    static constexpr int kFixed = 1024 /* alignment */ + QB + XB + 1024 /* barriers, flags */;
+    static constexpr int NQB = MW == 1 ? 2 : 1;        // q buffers
+    static constexpr int QB1 = MW * NT * NP * (HD / 16) * 256;
+    static constexpr int QB = NQB * QB1;
+    static constexpr int PER = HD / 4 * NT + 4 * NT;   // floats a lane hands over in a join
+    static constexpr int XB = NG > 1 ? (NG / 2) * MW * 32 * PER * 4 : 0;
+    static constexpr int CTL = 1536;                   // barriers, flags, row factors
+    static constexpr int kFixed = 1024 /* alignment */ + QB + XB + CTL;
     static constexpr int SLOT_ALL = SLOT + (kQ8 ? 2 * KS * 4 : 0);
-    // two CTAs per SM where each still has slots in flight beside the held
-    // ones, and where 168 registers hold the accumulator (head_dim < 256)
-    static constexpr int OCC = NW <= 4 && HD < 256 && (112 * 1024 - kFixed) / SLOT_ALL >= NG + 4 ? 2 : 1;
-    static constexpr int kFit = ((OCC == 2 ? 112 : 224) * 1024 - kFixed) / SLOT_ALL;
-    static constexpr int NSLOT = kFit < 24 ? kFit : 24;
+    // CTAs per SM: as many as leave a thread its registers (the accumulator is
+    // HD / 4 * NT of them) and the ring slots in flight beside the held ones
+    static constexpr int fit(int occ) { return (224 * 1024 / occ - kFixed) / SLOT_ALL; }
+    static constexpr int OCC = NW <= 4 && NT == 1 && HD < 256 && fit(3) >= NG + 2 ? 3
+                               : NW <= 4 && NT * HD <= 256 && fit(2) >= NG + 2    ? 2
+                                                                                  : 1;
+    static constexpr int NSLOT = fit(OCC) < 24 ? fit(OCC) : 24;
     static_assert(NSLOT >= NG + 1, "ring holds every group's slot and one in flight");
     static constexpr int OFF_RING = 0;
     static constexpr int OFF_SCALE = OFF_RING + NSLOT * SLOT;
     static constexpr int OFF_Q = OFF_SCALE + (kQ8 ? NSLOT * 2 * KS * 4 : 0);
     static constexpr int OFF_X = OFF_Q + QB;
     static constexpr int OFF_BAR = OFF_X + XB;
-    static constexpr int SMEM = OFF_BAR + 1024 + 1024;
+    static constexpr int SMEM = OFF_BAR + CTL + 1024;
     static_assert(NSLOT * SLOT >= Plan<TR, KS>::kSmem, "the plan's prefix sums fit in the ring");
     static constexpr int THREADS = (NW + 1) * 32;
 };
@@ -111,18 +120,38 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 
+// 8 x 8 matrix of 16-bit elements, one row per four lanes, transposed.
+__device__ __forceinline__ uint32_t movm_t(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src)
+                 : "memory");
+}
+
+// Arrives on `bar` (counted in its phase) when this thread's cp.async so far
+// have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+
 template <bool kHalf>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
     if constexpr (kHalf)
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
             "{%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
             "{%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // Bytes i and j of w (codes + 128) as two f16 codes: 0x64uu is 1024 + u, and
@@ -169,6 +198,12 @@ __device__ __forceinline__ void split(float a, float b, uint32_t (&out)[NP]) {
 }
 
 template <typename X>
+__device__ __forceinline__ float load1(const X* p) {
+    if constexpr (std::is_same<X, __half>::value) return __half2float(*p);
+    else return __bfloat162float(*p);
+}
+
+template <typename X>
 __device__ __forceinline__ float2 load2(const X* p) {
     if constexpr (sizeof(X) == 4) return *reinterpret_cast<const float2*>(p);
     else return unpack<X>(*reinterpret_cast<const uint32_t*>(p));
@@ -185,10 +220,37 @@ __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
 }
 
 __device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-    if (*dead) return false;
+    if (__any_sync(0xffffffffu, *dead != 0)) return false;
     if (mbar_wait_warp(bar, parity)) return true;
     *dead = 1;
     return false;
+}
+
+// Waits until the producer has begun chunk k in its slot.  A slot's uses go to
+// the groups in turn, so a group that is ahead may come to its use while the
+// one before it, another group's, has not landed: the barrier's parity would
+// then answer for the use before that.  Once the tag says k, the barrier is in
+// this use's phase.
+__device__ __forceinline__ bool tag_wait(volatile int* tag, int k, volatile int* dead) {
+    const int lane = threadIdx.x & 31;
+    uint64_t t0 = 0;
+    for (uint32_t i = 0;; ++i) {
+        if (__all_sync(0xffffffffu, *tag == k)) return true;
+        if (__any_sync(0xffffffffu, *dead != 0)) return false;
+        if ((i & 255u) == 255u) {
+            int late = 0;
+            if (lane == 0) {
+                const uint64_t now = global_ns();
+                if (t0 == 0) t0 = now;
+                else late = now - t0 > kWaitLimitNs;
+            }
+            if (__shfl_sync(0xffffffffu, late, 0)) {
+                if (lane == 0) record_timeout();
+                *dead = 1;
+                return false;
+            }
+        }
+    }
 }
 
 struct Vis {
@@ -198,39 +260,118 @@ struct Vis {
     }
 };
 
-template <typename X, class F>
-__device__ __forceinline__ void store4(const PagedArgs& a, float4 v, int64_t off) {
-    X* o = static_cast<X*>(a.out) + off;
-    if constexpr (sizeof(X) == 4) *reinterpret_cast<float4*>(o) = v;
-    else *reinterpret_cast<uint2*>(o) = make_uint2(pack<X>(v.x, v.y), pack<X>(v.z, v.w));
+// Where the packed row pr of a tile's sequence comes from and goes to.
+struct RowRef {
+    int tok, head;
+    __device__ __forceinline__ RowRef(const PagedArgs& a, const PlanPos& p, int pr) {
+        tok = pr / a.gqa;
+        head = p.kvh * a.gqa + pr - tok * a.gqa;
+    }
+};
+
+// One warp's rows of q as B operands: pieces to sQ, score factors to sC.
+template <class F>
+__device__ __forceinline__ void prepare_q(const PagedArgs& a, const PlanPos& p, int pr0, uint2* sQ,
+                                          float* sC) {
+    using X = typename F::X;
+    using OT = typename F::OT;
+    constexpr int HD = F::HD, NP = F::NP;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    const int rows = p.n * a.gqa;
+    // the order of the 16 k of an instruction is free: with 8-bit codes a
+    // lane's four are neighbours (one word of the cache row)
+    const int kl = F::kQ8 ? 4 * t4 : 2 * t4, kh = F::kQ8 ? 4 * t4 + 2 : 2 * t4 + 8;
+#pragma unroll
+    for (int n = 0; n < F::NT; ++n) {
+        const int pr = pr0 + 8 * n + g;
+        const bool live = pr < rows;
+        const RowRef r(a, p, live ? pr : 0);
+        const X* q = static_cast<const X*>(a.q) + (int64_t)(p.row + r.tok) * a.q_stride +
+                     (int64_t)r.head * HD;
+        float2 x[HD / 16], y[HD / 16];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+            x[i] = y[i] = make_float2(0.f, 0.f);
+            if (live) x[i] = load2(q + 16 * i + kl), y[i] = load2(q + 16 * i + kh);
+        }
+        float fa = 1.f, fb = 1.f, c = a.c;
+        if constexpr (F::kRowScale) {
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i)
+                top = max(max(max(top, __float_as_uint(fabsf(x[i].x))),
+                              __float_as_uint(fabsf(x[i].y))),
+                          max(__float_as_uint(fabsf(y[i].x)), __float_as_uint(fabsf(y[i].y))));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // the row's largest value lands in [2^14, 2^15); 2^-e as two
+            // factors that are in range
+            const int e = top > 0 && top < 0x7F800000u ? (int)(top >> 23) - 141 : 0;
+            fa = pow2(-e / 2), fb = pow2(-e - -e / 2);
+            c = fmaxf(a.c * pow2(e / 2) * pow2(e - e / 2), 1e-38f);
+        }
+        if (t4 == 0) sC[8 * n + g] = c;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+            if constexpr (F::kRowScale) {
+                x[i].x = x[i].x * fa * fb, x[i].y = x[i].y * fa * fb;
+                y[i].x = y[i].x * fa * fb, y[i].y = y[i].y * fa * fb;
+            }
+            uint32_t b0[NP], b1[NP];
+            split<OT, NP>(x[i].x, x[i].y, b0);
+            split<OT, NP>(y[i].x, y[i].y, b1);
+#pragma unroll
+            for (int q2 = 0; q2 < NP; ++q2)
+                sQ[((n * NP + q2) * (HD / 16) + i) * 32 + lane] = make_uint2(b0[q2], b1[q2]);
+        }
+    }
 }
 
-template <typename X, typename C, class F>
+template <typename X, class F>
+__device__ __forceinline__ void store1(X* o, float v) {
+    if constexpr (sizeof(X) == 4) *o = v;
+    else if constexpr (std::is_same<X, __half>::value) *o = __float2half_rn(v);
+    else *o = __float2bfloat16_rn(v);
+}
+
+template <class F>
 __global__ void __launch_bounds__(F::THREADS, F::OCC)
 paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
           const __grid_constant__ PagedArgs a, int least) {
-    constexpr int HD = F::HD, MW = F::MW, NG = F::NG, NP = F::NP, KS = F::KS, TR = F::TR;
-    constexpr int NT = HD / 8;  // output tiles of 8 dimensions
+    using X = typename F::X;
+    using C = typename F::C;
     using OT = typename F::OT;
+    constexpr int HD = F::HD, NT = F::NT, MW = F::MW, NG = F::NG, NP = F::NP, KS = F::KS;
+    constexpr int TR = F::TR, DT = HD / 16, KT = KS / 16;  // 16-dimension and 16-key tiles
     using P = Plan<TR, KS>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* sScale = reinterpret_cast<float*>(smem + F::OFF_SCALE);
-    uint4* sQ = reinterpret_cast<uint4*>(smem + F::OFF_Q);
     float* sX = reinterpret_cast<float*>(smem + F::OFF_X);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + F::OFF_BAR);
     uint64_t* empty = full + F::NSLOT;
-    volatile int* dead = reinterpret_cast<volatile int*>(empty + F::NSLOT);
-    int* sFlag = const_cast<int*>(dead) + 4;                       // [NSLOT] mapped halves
-    PlanPos* sPos = reinterpret_cast<PlanPos*>(sFlag + 32);
+    uint64_t* q_full = empty + F::NSLOT;  // [2]
+    uint64_t* q_empty = q_full + 2;
+    volatile int* dead = reinterpret_cast<volatile int*>(q_empty + 2);
+    int* sFlag = const_cast<int*>(dead) + 4;  // [NSLOT] mapped halves
+    volatile int* sTag = sFlag + 24;          // [NSLOT] chunk in the slot
+    PlanPos* sPos = reinterpret_cast<PlanPos*>(sFlag + 48);
+    float* sC = reinterpret_cast<float*>(sPos + 1);  // [NQB][TR]
+    static_assert(F::NSLOT * 16 + 32 + 16 + 192 + (int)sizeof(PlanPos) + F::NQB * TR * 4 <= F::CTL,
+                  "control block");
     int64_t* sPre = reinterpret_cast<int64_t*>(smem + F::OFF_RING);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < F::NSLOT; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], F::kQ8 ? 33 : 1);
             mbar_init(&empty[i], MW);
+            sTag[i] = -1;
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_empty[i], F::NW);
         }
         *dead = 0;
         mbar_fence_init();
@@ -259,17 +400,17 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
     fence_proxy_async_smem();  // the prefix sums are done with: the ring may be filled
     __syncthreads();
     PlanPos p = *sPos;
+    auto q_buf = [&](int buf, int mt) {
+        return reinterpret_cast<uint2*>(smem + F::OFF_Q + buf * F::QB1) +
+               mt * NT * NP * (HD / 16) * 32;
+    };
 
     if (warp == F::NW) {
         // -------------------------------------------------------- producer
-        if (lane == 0) {
-            prefetch_tensormap(&tk);
-            prefetch_tensormap(&tv);
-        }
         const int box = min(a.b.page_size, KS);  // rows of a box
         const int halves = KS / box;             // boxes over the keys (1 or 2)
-        uint32_t it = 0;
-        for (int left = total; left > 0;) {
+        uint32_t it = 0, seg = 0;
+        for (int left = total; left > 0; ++seg) {
             const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
             const int m = min(tw.count - p.i, left);
             for (int j0 = 0; j0 < m; j0 += 32) {
@@ -279,6 +420,14 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                     id0 = page_of(a.b, p.s, key);
                     if (halves == 2) id1 = page_of(a.b, p.s, key + box);
                 }
+                if (MW == 1 && j0 == 0) {
+                    // the tile's q, while the consumers are on the last one
+                    const int buf = seg & 1;
+                    if (!ring_wait(&q_empty[buf], ((seg >> 1) & 1) ^ 1, dead)) break;
+                    prepare_q<F>(a, p, p.t * TR, q_buf(buf, 0), sC + buf * TR);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&q_full[buf]);
+                }
                 const int jn = min(32, m - j0);
                 for (int j = 0; j < jn; ++j, ++it) {
                     const int k0 = __shfl_sync(0xffffffffu, key, j);
@@ -286,29 +435,35 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                     const int ib = __shfl_sync(0xffffffffu, id1, j);
                     const int s = it % F::NSLOT;
                     if (!ring_wait(&empty[s], ((it / F::NSLOT) & 1) ^ 1, dead)) break;
-                    const int mapped = (ia >= 0 ? 1 : 0) + (ib >= 0 ? 1 : 0);
                     if (lane == 0) {
                         sFlag[s] = halves == 2 ? (ia >= 0 ? 1 : 0) | (ib >= 0 ? 2 : 0)
                                                : (ia >= 0 ? 3 : 0);
-                        mbar_arrive_expect_tx(&full[s],
-                                              F::SLOT + (F::kQ8 ? mapped * 2 * box * 4 : 0));
+                        sTag[s] = (int)it;
+                        mbar_arrive_expect_tx(&full[s], F::SLOT);
                     }
                     __syncwarp();
-                    // lane l: tensor (K, V), 128-byte column, page half
-                    const int kv = lane & 1, col = (lane >> 1) % F::NBOX;
-                    const int half = (lane >> 1) / F::NBOX;
-                    const int id = half ? ib : ia;
                     const int y = p.kvh * a.b.page_size + (k0 & (a.b.page_size - 1));
-                    if (half < halves) {
-                        uint8_t* dst = smem + F::OFF_RING + s * F::SLOT + kv * (KS * F::ROWB) +
-                                       col * (KS * F::BOXB) + half * box * F::BOXB;
-                        // past the last page: zeros
-                        tma_box(dst, kv ? &tv : &tk, col * (F::BOXB / (int)sizeof(C)), y,
-                                id < 0 ? a.b.n_pages : id, &full[s]);
-                        if (F::kQ8 && col == 0 && id >= 0)
-                            bulk_copy(sScale + (s * 2 + kv) * KS + half * box,
-                                      (kv ? a.vs : a.ks) + (int64_t)id * a.b.scale_stride + y,
-                                      box * 4, &full[s]);
+                    {
+                        // lane l: tensor (K, V), 128-byte column, page half
+                        const int kv = lane & 1, col = (lane >> 1) % F::NBOX;
+                        const int half = (lane >> 1) / F::NBOX;
+                        const int id = half ? ib : ia;
+                        if (half < halves)  // past the last page: zeros
+                            tma_box(smem + F::OFF_RING + s * F::SLOT + kv * (KS * F::ROWB) +
+                                        col * (KS * F::BOXB) + half * box * F::BOXB,
+                                    kv ? &tv : &tk, col * (F::BOXB / (int)sizeof(C)), y,
+                                    id < 0 ? a.b.n_pages : id, &full[s]);
+                    }
+                    if constexpr (F::kQ8) {
+                        // four scales a lane (a copy of its own per page would
+                        // cost the TMA unit as much as a box)
+                        const int kv = lane / (KS / 4), q4 = lane % (KS / 4) * 4;
+                        const int id = q4 >= box ? ib : ia;
+                        if (kv < 2 && id >= 0)
+                            cp_async16(sScale + (s * 2 + kv) * KS + q4,
+                                       (kv ? a.vs : a.ks) + (int64_t)id * a.b.scale_stride + y +
+                                           (q4 >= box ? q4 - box : q4));
+                        cp_async_arrive(&full[s]);
                     }
                     __syncwarp();
                 }
@@ -329,108 +484,55 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
     const int grp = warp / MW, mt = warp % MW;
     const int g = lane >> 2, t4 = lane & 3;
     const Vis vis = {a.window, a.n_sink};
-    uint32_t it = 0;
+    uint32_t it = 0, seg = 0;
     bool owner = false;
-    for (int left = total; left > 0;) {
+    for (int left = total; left > 0; ++seg) {
         const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
         const int m = min(tw.count - p.i, left);
         const bool cut_l = p.i > 0, cut_r = p.i + m < tw.count;
         const int rows = p.n * a.gqa;
-        const int pr = p.t * TR + mt * 16;  // the warp's first packed row
-        const int wrows = min(rows - pr, 16);  // <= 0: none
-        const bool two = wrows > 8;
-
-        // q: operand pieces to shared memory, row scales kept
-        float c0 = a.c, c1 = a.c;
-        int pos0 = -1, pos1 = -1;
-        int64_t off0 = 0, off1 = 0;  // of the rows in out
-        {
-            const int ra = pr + g, rb = ra + 8;
-            const bool va = ra < rows, vb = rb < rows;
-            const int ta = ra / a.gqa, tb = rb / a.gqa;
-            const int ha = p.kvh * a.gqa + ra - ta * a.gqa, hb = p.kvh * a.gqa + rb - tb * a.gqa;
-            if (va) pos0 = p.len - p.n + ta;
-            if (vb) pos1 = p.len - p.n + tb;
-            off0 = (int64_t)(p.row + ta) * a.out_stride + (int64_t)ha * HD;
-            off1 = (int64_t)(p.row + tb) * a.out_stride + (int64_t)hb * HD;
-            const X* qa = static_cast<const X*>(a.q) + (int64_t)(p.row + ta) * a.q_stride +
-                          (int64_t)ha * HD;
-            const X* qb = static_cast<const X*>(a.q) + (int64_t)(p.row + tb) * a.q_stride +
-                          (int64_t)hb * HD;
-            // the order of the 16 k of an instruction is free: with 8-bit
-            // codes a lane's four are neighbours (one word of the cache row)
-            const int kl = F::kQ8 ? 4 * t4 : 2 * t4, kh = F::kQ8 ? 4 * t4 + 2 : 2 * t4 + 8;
-            int e0 = 0, e1 = 0;
-            float fa0 = 1.f, fb0 = 1.f, fa1 = 1.f, fb1 = 1.f;
-            if constexpr (F::kRowScale) {
-                uint32_t m0 = 0, m1 = 0;
-#pragma unroll
-                for (int i = 0; i < HD / 16; ++i) {
-                    if (va) {
-                        const float2 x = load2(qa + 16 * i + kl), y = load2(qa + 16 * i + kh);
-                        m0 = max(max(m0, __float_as_uint(fabsf(x.x))),
-                                 max(__float_as_uint(fabsf(x.y)),
-                                     max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y)))));
-                    }
-                    if (vb) {
-                        const float2 x = load2(qb + 16 * i + kl), y = load2(qb + 16 * i + kh);
-                        m1 = max(max(m1, __float_as_uint(fabsf(x.x))),
-                                 max(__float_as_uint(fabsf(x.y)),
-                                     max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y)))));
-                    }
-                }
-#pragma unroll
-                for (int o = 1; o <= 2; o <<= 1) {
-                    m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-                    m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-                }
-                // the row's largest value lands in [2^14, 2^15)
-                if (m0 > 0 && m0 < 0x7F800000u) e0 = (int)(m0 >> 23) - 141;
-                if (m1 > 0 && m1 < 0x7F800000u) e1 = (int)(m1 >> 23) - 141;
-                fa0 = pow2(-e0 / 2), fb0 = pow2(-e0 - -e0 / 2);
-                fa1 = pow2(-e1 / 2), fb1 = pow2(-e1 - -e1 / 2);
-                c0 = fmaxf(a.c * pow2(e0 / 2) * pow2(e0 - e0 / 2), 1e-38f);
-                c1 = fmaxf(a.c * pow2(e1 / 2) * pow2(e1 - e1 / 2), 1e-38f);
-            }
-            if (grp == 0) {
-#pragma unroll
-                for (int i = 0; i < HD / 16; ++i) {
-                    float2 x0 = make_float2(0.f, 0.f), y0 = x0, x1 = x0, y1 = x0;
-                    if (va) x0 = load2(qa + 16 * i + kl), y0 = load2(qa + 16 * i + kh);
-                    if (vb) x1 = load2(qb + 16 * i + kl), y1 = load2(qb + 16 * i + kh);
-                    if constexpr (F::kRowScale) {  // 2^-e as two factors in range
-                        x0.x = x0.x * fa0 * fb0, x0.y = x0.y * fa0 * fb0;
-                        y0.x = y0.x * fa0 * fb0, y0.y = y0.y * fa0 * fb0;
-                        x1.x = x1.x * fa1 * fb1, x1.y = x1.y * fa1 * fb1;
-                        y1.x = y1.x * fa1 * fb1, y1.y = y1.y * fa1 * fb1;
-                    }
-                    uint32_t r0[NP], r1[NP], r2[NP], r3[NP];
-                    split<OT, NP>(x0.x, x0.y, r0);
-                    split<OT, NP>(x1.x, x1.y, r1);
-                    split<OT, NP>(y0.x, y0.y, r2);
-                    split<OT, NP>(y1.x, y1.y, r3);
-#pragma unroll
-                    for (int n = 0; n < NP; ++n)
-                        sQ[((mt * NP + n) * (HD / 16) + i) * 32 + lane] =
-                            make_uint4(r0[n], r1[n], r2[n], r3[n]);
-                }
-            }
+        const int pr = p.t * TR + mt * F::WR;         // the warp's first packed row
+        const int wrows = min(rows - pr, F::WR);      // <= 0: none
+        const int buf = F::NQB == 2 ? seg & 1 : 0;
+        const uint2* sQ = q_buf(buf, mt);
+        const float* cq = sC + buf * TR + mt * F::WR;
+        if constexpr (MW == 1) {
+            ring_wait(&q_full[buf], (seg >> 1) & 1, dead);
+        } else {
+            __syncwarp();
+            prepare_q<F>(a, p, pr, q_buf(0, mt), sC + mt * F::WR);
+            __syncwarp();
         }
-        if constexpr (NG > 1) named_barrier(1, F::NW * 32);
-        else __syncwarp();
+        // this lane's rows: 2 t4 and 2 t4 + 1 of each 8
+        float c[NT][2];
+        int pos[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * n + 2 * t4 + e;
+                c[n][e] = cq[r];
+                pos[n][e] = r < wrows ? p.len - p.n + (pr + r) / a.gqa : -1;
+            }
         // rows of this warp for the mask tests
         const int p_lo = p.len - p.n + pr / a.gqa;
         const int p_hi = wrows > 0 ? p.len - p.n + (pr + wrows - 1) / a.gqa : -1;
 
-        float O[NT][4];
+        float O[DT][NT][4];  // dimensions g, g + 8 of a tile by rows 2 t4, 2 t4 + 1
+        float M[NT][2], l[NT][2];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.f;
-        float M0 = -INFINITY, M1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        for (int n = 0; n < NT; ++n) {
+            M[n][0] = M[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) O[d][n][0] = O[d][n][1] = O[d][n][2] = O[d][n][3] = 0.f;
+        }
         int E = -126;  // 8-bit V: the accumulator's unit is 2^E
 
         for (int j = grp; j < m; j += NG) {
             const uint32_t k = it + j;
             const int s = k % F::NSLOT;
+            if (!tag_wait(&sTag[s], (int)k, dead)) continue;
             if (!ring_wait(&full[s], (k / F::NSLOT) & 1, dead)) continue;
             const int key0 = tw.key0(p.i + j);
             const int flag = sFlag[s];
@@ -445,172 +547,205 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
             const uint32_t ks_addr = smem_u32(smem + F::OFF_RING + s * F::SLOT);
             const uint32_t vs_addr = ks_addr + KS * F::ROWB;
 
-            // ---- scores: KS / 8 tiles of 8 keys
-            // (k outside, so that a piece of q is read once for all of them)
-            float S[KS / 8][4], lo[F::kF32 ? KS / 8 : 1][4];
+            // ---- scores, keys by rows: K is the A operand, q the B operand
+            float S[KT][NT][4], lo[F::kF32 ? KT : 1][F::kF32 ? NT : 1][4];
 #pragma unroll
-            for (int n = 0; n < KS / 8; ++n) {
-                S[n][0] = S[n][1] = S[n][2] = S[n][3] = 0.f;
-                if constexpr (F::kF32) lo[n][0] = lo[n][1] = lo[n][2] = lo[n][3] = 0.f;
-            }
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int c4 = 0; c4 < F::ROWB / 64; ++c4) {
-                constexpr int STEPS = F::kQ8 ? 4 : 2;  // k-steps in four chunks
-                uint32_t r[KS / 8][4];
+                for (int n = 0; n < NT; ++n) {
+                    S[kt][n][0] = S[kt][n][1] = S[kt][n][2] = S[kt][n][3] = 0.f;
+                    if constexpr (F::kF32)
+                        lo[kt][n][0] = lo[kt][n][1] = lo[kt][n][2] = lo[kt][n][3] = 0.f;
+                }
+            constexpr int CPI = F::kQ8 ? 1 : 2;  // 16-byte chunks per 16 k
 #pragma unroll
-                for (int n = 0; n < KS / 8; ++n)
-                    ldsm4(r[n], ks_addr + chunk_off<F>(8 * n + (lane & 7), 4 * c4 + (lane >> 3)));
+            for (int i2 = 0; i2 < HD / 16; i2 += 2 / CPI) {
+                // two chunks of 16 keys: 8-bit, two steps of 16 k; 16-bit, one
+                uint32_t r[KT][4];
 #pragma unroll
-                for (int st = 0; st < STEPS; ++st) {
-                    const uint4* qf = sQ + (mt * NP * (HD / 16) + c4 * STEPS + st) * 32 + lane;
-                    uint4 qv[NP];
+                for (int kt = 0; kt < KT; ++kt)
+                    ldsm4(r[kt], ks_addr + chunk_off<F>(16 * kt + (lane & 15),
+                                                        i2 * CPI + (lane >> 4)));
 #pragma unroll
-                    for (int q = 0; q < NP; ++q) qv[q] = qf[q * (HD / 16) * 32];
+                for (int st = 0; st < 2 / CPI; ++st) {
+                    const int i = i2 + st;
+                    uint2 qv[NT][NP];
 #pragma unroll
-                    for (int n = 0; n < KS / 8; ++n) {
-                        uint32_t b0, b1;
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int q = 0; q < NP; ++q)
+                            qv[n][q] = sQ[((n * NP + q) * (HD / 16) + i) * 32 + lane];
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        uint32_t ka[4];  // keys g, g + 8 of the low k, then of the high
                         if constexpr (F::kQ8) {
-                            const uint32_t u = r[n][st] ^ 0x80808080u;
-                            b0 = codes2<0x4140>(u);
-                            b1 = codes2<0x4342>(u);
+                            const uint32_t u0_ = r[kt][2 * st] ^ 0x80808080u;
+                            const uint32_t u1_ = r[kt][2 * st + 1] ^ 0x80808080u;
+                            ka[0] = codes2<0x4140>(u0_);
+                            ka[1] = codes2<0x4140>(u1_);
+                            ka[2] = codes2<0x4342>(u0_);
+                            ka[3] = codes2<0x4342>(u1_);
                         } else {
-                            b0 = r[n][2 * st];
-                            b1 = r[n][2 * st + 1];
+                            ka[0] = r[kt][0], ka[1] = r[kt][1], ka[2] = r[kt][2], ka[3] = r[kt][3];
                         }
-                        mma16816<F::kHalf>(S[n], qv[0], b0, b1);
 #pragma unroll
-                        for (int q = 1; q < NP; ++q) mma16816<F::kHalf>(lo[n], qv[q], b0, b1);
+                        for (int n = 0; n < NT; ++n) {
+                            mma16816<F::kHalf>(S[kt][n], ka, qv[n][0].x, qv[n][0].y);
+#pragma unroll
+                            for (int q = 1; q < NP; ++q)
+                                mma16816<F::kHalf>(lo[kt][n], ka, qv[n][q].x, qv[n][q].y);
+                        }
                     }
                 }
             }
             if constexpr (F::kF32) {
 #pragma unroll
-                for (int n = 0; n < KS / 8; ++n)
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) S[n][i] += lo[n][i];
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) S[kt][n][i] += lo[kt][n][i];
             }
 
-            // ---- the 8-bit scales of this lane's keys
-            float vsc[KS / 8][2];
+            // ---- the 8-bit scales of this lane's keys, 16 kt + g and + 8
+            float vsc[KT][2];
             float mul = 1.f;  // what E's growth does to the accumulator
             if constexpr (F::kQ8) {
                 const float* ksc = sScale + (s * 2) * KS;
-                float top = 0.f;
+                uint32_t top = 0;
 #pragma unroll
-                for (int n = 0; n < KS / 8; ++n) {
-                    const float2 kk = *reinterpret_cast<const float2*>(ksc + 8 * n + 2 * t4);
-                    const float2 vv = *reinterpret_cast<const float2*>(ksc + KS + 8 * n + 2 * t4);
-                    S[n][0] *= kk.x, S[n][2] *= kk.x;
-                    S[n][1] *= kk.y, S[n][3] *= kk.y;
-                    vsc[n][0] = vv.x, vsc[n][1] = vv.y;
-                    const int key = key0 + 8 * n + 2 * t4;
-                    const bool on = whole || ((flag >> (8 * n / (KS / 2))) & 1);
-                    if (on && key <= p_hi) top = fmaxf(top, fabsf(vv.x));
-                    if (on && key + 1 <= p_hi) top = fmaxf(top, fabsf(vv.y));
-                }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int Ek = min(max((int)(__float_as_uint(top) >> 23) - 126, -126), 126);
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int kk = 16 * kt + 8 * h + g;
+                        const float kf = ksc[kk];
+                        vsc[kt][h] = ksc[KS + kk];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            S[kt][n][2 * h] *= kf;
+                            S[kt][n][2 * h + 1] *= kf;
+                        }
+                        // (hidden slots may hold anything)
+                        uint32_t b = __float_as_uint(fabsf(vsc[kt][h]));
+                        if (!whole && !(((flag >> (kk / (KS / 2))) & 1) && key0 + kk <= p_hi &&
+                                        b < 0x7F800000u))
+                            b = 0;
+                        top = max(top, b);
+                    }
+                top = __reduce_max_sync(0xffffffffu, top);
+                const int Ek = min(max((int)(top >> 23) - 126, -126), 126);
                 if (Ek > E) {
                     mul = E - Ek < -126 ? 0.f : pow2(E - Ek);
                     E = Ek;
                 }
                 const float f = pow2(-E);
 #pragma unroll
-                for (int n = 0; n < KS / 8; ++n) vsc[n][0] *= f, vsc[n][1] *= f;
+                for (int kt = 0; kt < KT; ++kt) vsc[kt][0] *= f, vsc[kt][1] *= f;
             }
 
             // ---- softmax: new maxima, weights (2^14 up in f16), sums
             if (!whole) {
 #pragma unroll
-                for (int n = 0; n < KS / 8; ++n) {
-                    const bool on = (flag >> (8 * n / (KS / 2))) & 1;
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int key = key0 + 8 * n + 2 * t4 + i;
-                        // a hidden score is marked by a NaN with this sign and payload
-                        if (!(on && vis(key, pos0))) S[n][i] = __uint_as_float(0xFFFFDEADu);
-                        if (!(on && vis(key, pos1))) S[n][2 + i] = __uint_as_float(0xFFFFDEADu);
+                    for (int h = 0; h < 2; ++h) {
+                        const int kk = 16 * kt + 8 * h + g;
+                        const bool on = (flag >> (kk / (KS / 2))) & 1;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                // a hidden score is marked by a NaN with this payload
+                                if (!(on && vis(key0 + kk, pos[n][e])))
+                                    S[kt][n][2 * h + e] = __uint_as_float(0xFFFFDEADu);
                     }
-                }
             }
-            float m0 = -INFINITY, m1 = -INFINITY;  // fmaxf skips NaN
-#pragma unroll
-            for (int n = 0; n < KS / 8; ++n) {
-                m0 = fmaxf(m0, fmaxf(S[n][0], S[n][1]));
-                m1 = fmaxf(m1, fmaxf(S[n][2], S[n][3]));
-            }
-            m0 *= c0, m1 *= c1;
-#pragma unroll
-            for (int o = 1; o <= 2; o <<= 1) {
-                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-            }
-            const float N0 = fmaxf(M0, m0), N1 = fmaxf(M1, m1);
-            const float R0 = N0 == -INFINITY ? 0.f : N0, R1 = N1 == -INFINITY ? 0.f : N1;
-            float al0 = ex2(M0 - R0), al1 = ex2(M1 - R1);  // 0 while M is -inf
-            M0 = N0, M1 = N1;
+            float al[NT][2], D[NT][2];
             constexpr float kUp = F::kHalf ? 14.f : 0.f;
-            const float D0 = kUp - R0, D1 = kUp - R1;
-            float s0 = 0.f, s1 = 0.f;
-            uint4 pf[KS / 16][NP];
 #pragma unroll
-            for (int n = 0; n < KS / 8; ++n) {
-                float w[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    w[i] = ex2(fmaf(S[n][i], c0, D0));
-                    if (two) w[2 + i] = ex2(fmaf(S[n][2 + i], c1, D1));
+                for (int e = 0; e < 2; ++e) {
+                    float mx = fmaxf(S[0][n][e], S[0][n][2 + e]);  // fmaxf skips NaN
+#pragma unroll
+                    for (int kt = 1; kt < KT; ++kt)
+                        mx = fmaxf(mx, fmaxf(S[kt][n][e], S[kt][n][2 + e]));
+                    mx = fmaxf(mx, -INFINITY);
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float N = fmaxf(M[n][e], mx * c[n][e]);
+                    const float R = N == -INFINITY ? 0.f : N;
+                    al[n][e] = ex2(M[n][e] - R);  // 0 while M is -inf
+                    M[n][e] = N;
+                    D[n][e] = kUp - R;
                 }
-                if (!whole) {
+            uint32_t pb[KT][NT][NP][2];  // weights as B operand: keys by rows
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (__float_as_uint(S[n][i]) == 0xFFFFDEADu) w[i] = 0.f;
-                }
-                s0 += w[0] + w[1];
-                s1 += w[2] + w[3];
-                if constexpr (F::kQ8) {
+            for (int n = 0; n < NT; ++n) {
+                float sum[2] = {0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = w[i] == 0.f ? 0.f : w[i] * vsc[n][i & 1];
-                }
-                uint32_t x[NP], y[NP];
-                split<OT, NP>(w[0], w[1], x);
-                split<OT, NP>(w[2], w[3], y);
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int q = 0; q < NP; ++q) {
-                    if (n & 1) pf[n / 2][q].z = x[q], pf[n / 2][q].w = y[q];
-                    else pf[n / 2][q].x = x[q], pf[n / 2][q].y = y[q];
+                    for (int h = 0; h < 2; ++h) {
+                        float w[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float sv = S[kt][n][2 * h + e];
+                            w[e] = ex2(fmaf(sv, c[n][e], D[n][e]));
+                            if (!whole && __float_as_uint(sv) == 0xFFFFDEADu) w[e] = 0.f;
+                            sum[e] += w[e];
+                            if constexpr (F::kQ8) {
+                                const float v = w[e] * vsc[kt][h];
+                                w[e] = !whole && w[e] == 0.f ? 0.f : v;
+                            }
+                        }
+                        uint32_t x[NP];
+                        split<OT, NP>(w[0], w[1], x);
+#pragma unroll
+                        for (int q = 0; q < NP; ++q) pb[kt][n][q][h] = movm_t(x[q]);
+                    }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    l[n][e] = fmaf(l[n][e], al[n][e], sum[e]);
+                    if constexpr (F::kQ8) al[n][e] *= mul;
                 }
             }
-            l0 = fmaf(l0, al0, s0);
-            l1 = fmaf(l1, al1, s1);
-            if constexpr (F::kQ8) al0 *= mul, al1 *= mul;
 
-            // ---- weighted V: 16-bit results tolerate the matrix unit's own
-            // accumulation over all keys, fp32 ones get fresh sums per chunk
+            // ---- weighted V, dimensions by rows: V is the A operand.  16-bit
+            // results tolerate the matrix unit's own accumulation over all
+            // keys, fp32 ones get fresh sums per chunk
             bool odd = false;
             if constexpr (!F::kF32) {
-                if (__any_sync(0xffffffffu, al0 != 1.f || al1 != 1.f)) {
+                bool grow = false;
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        O[i][0] *= al0, O[i][1] *= al0;
-                        O[i][2] *= al1, O[i][3] *= al1;
-                    }
+                for (int n = 0; n < NT; ++n) grow |= al[n][0] != 1.f || al[n][1] != 1.f;
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            O[d][n][0] *= al[n][0], O[d][n][1] *= al[n][1];
+                            O[d][n][2] *= al[n][0], O[d][n][3] *= al[n][1];
+                        }
                 }
             }
+            constexpr int DPI = F::kQ8 ? 2 : 1;  // 16-dimension tiles in two chunks
 #pragma unroll
-            for (int c2 = 0; c2 < F::ROWB / 32; ++c2) {
-                constexpr int TPC = F::kQ8 ? 2 : 1;  // output tiles in a 16-byte chunk
-                float acc[2 * TPC][4];
+            for (int d2 = 0; d2 < DT; d2 += DPI) {
+                float acc[F::kF32 ? DPI : 1][F::kF32 ? NT : 1][4];
                 if constexpr (F::kF32) {
 #pragma unroll
-                    for (int i = 0; i < 2 * TPC; ++i)
-                        acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+                    for (int i = 0; i < DPI; ++i)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
                 }
 #pragma unroll
-                for (int st = 0; st < KS / 16; ++st) {
-                    uint32_t r[4];
-                    ldsm4_t(r, vs_addr + chunk_off<F>(16 * st + (lane & 15), 2 * c2 + (lane >> 4)));
+                for (int kt = 0; kt < KT; ++kt) {
+                    uint32_t r[4];  // keys 0-7 and 8-15 of one chunk, then of the next
+                    ldsm4_t(r, vs_addr + chunk_off<F>(16 * kt + (lane & 15),
+                                                      d2 * (F::kQ8 ? 1 : 2) + (lane >> 4)));
                     if constexpr (!F::kQ8) {
                         // V that is not finite may be hidden from some rows,
                         // and pieces of a weight may be 0 or of either sign:
@@ -634,35 +769,44 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 2 * TPC; ++i) {
-                        uint32_t b0, b1;
+                    for (int i = 0; i < DPI; ++i) {
+                        uint32_t va[4];
                         if constexpr (F::kQ8) {
-                            const uint32_t ua = r[i & 2] ^ 0x80808080u;
-                            const uint32_t ub = r[(i & 2) + 1] ^ 0x80808080u;
-                            b0 = (i & 1) ? codes2<0x4341>(ua) : codes2<0x4240>(ua);
-                            b1 = (i & 1) ? codes2<0x4341>(ub) : codes2<0x4240>(ub);
+                            // rows of the tile: even dimensions, then odd ones
+                            const uint32_t ua = r[2 * i] ^ 0x80808080u;
+                            const uint32_t ub = r[2 * i + 1] ^ 0x80808080u;
+                            va[0] = codes2<0x4240>(ua);
+                            va[1] = codes2<0x4341>(ua);
+                            va[2] = codes2<0x4240>(ub);
+                            va[3] = codes2<0x4341>(ub);
                         } else {
-                            b0 = r[2 * i];
-                            b1 = r[2 * i + 1];
+                            va[0] = r[0], va[1] = r[2], va[2] = r[1], va[3] = r[3];
                         }
-                        if constexpr (F::kF32) {
 #pragma unroll
-                            for (int q = 0; q < NP; ++q)
-                                mma16816<F::kHalf>(acc[i], pf[st][q], b0, b1);
-                        } else {
-                            mma16816<F::kHalf>(O[2 * TPC * c2 + i], pf[st][0], b0, b1);
+                        for (int n = 0; n < NT; ++n) {
+                            if constexpr (F::kF32) {
+#pragma unroll
+                                for (int q = 0; q < NP; ++q)
+                                    mma16816<F::kHalf>(acc[i][n], va, pb[kt][n][q][0],
+                                                       pb[kt][n][q][1]);
+                            } else {
+                                mma16816<F::kHalf>(O[d2 + i][n], va, pb[kt][n][0][0],
+                                                   pb[kt][n][0][1]);
+                            }
                         }
                     }
                 }
                 if constexpr (F::kF32) {
 #pragma unroll
-                    for (int i = 0; i < 2 * TPC; ++i) {
-                        float(&o)[4] = O[2 * TPC * c2 + i];
-                        o[0] = fmaf(o[0], al0, acc[i][0]);
-                        o[1] = fmaf(o[1], al0, acc[i][1]);
-                        o[2] = fmaf(o[2], al1, acc[i][2]);
-                        o[3] = fmaf(o[3], al1, acc[i][3]);
-                    }
+                    for (int i = 0; i < DPI; ++i)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float(&o)[4] = O[d2 + i][n];
+                            o[0] = fmaf(o[0], al[n][0], acc[i][n][0]);
+                            o[1] = fmaf(o[1], al[n][1], acc[i][n][1]);
+                            o[2] = fmaf(o[2], al[n][0], acc[i][n][2]);
+                            o[3] = fmaf(o[3], al[n][1], acc[i][n][3]);
+                        }
                 }
             }
             if constexpr (!F::kQ8) {
@@ -670,19 +814,20 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                     const uint8_t* vt = smem + F::OFF_RING + s * F::SLOT + KS * F::ROWB;
                     for (int kk = 0; kk < KS; ++kk) {
                         const bool on = (flag >> (kk / (KS / 2))) & 1;
-                        const bool see0 = on && vis(key0 + kk, pos0);
-                        const bool see1 = on && vis(key0 + kk, pos1);
-                        if (!__any_sync(0xffffffffu, see0 || see1)) continue;
 #pragma unroll
-                        for (int i = 0; i < NT; ++i) {
-                            const float2 x = unpack<OT>(*reinterpret_cast<const uint32_t*>(
-                                vt + chunk_off<F>(kk, i) + 4 * t4));
-                            const bool bx = !(fabsf(x.x) < INFINITY), by = !(fabsf(x.y) < INFINITY);
-                            if (bx && see0) O[i][0] += x.x;
-                            if (by && see0) O[i][1] += x.y;
-                            if (bx && see1) O[i][2] += x.x;
-                            if (by && see1) O[i][3] += x.y;
-                        }
+                        for (int d = 0; d < DT; ++d)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float x = load1(reinterpret_cast<const OT*>(
+                                                          vt + chunk_off<F>(kk, 2 * d + h)) + g);
+                                if (fabsf(x) < INFINITY) continue;
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e)
+                                        if (on && vis(key0 + kk, pos[n][e]))
+                                            O[d][n][2 * h + e] += x;
+                            }
                     }
                 }
             }
@@ -690,48 +835,63 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
             if (lane == 0) mbar_arrive(&empty[s]);
         }
         it += m;
+        __syncwarp();
+        if (MW == 1 && lane == 0) mbar_arrive(&q_empty[buf]);
 
         // ---- join the groups, halving their number per round
         if constexpr (F::kQ8) {
             const float f = pow2(E);
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
+            for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) O[i][e] *= f;
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) O[d][n][i] *= f;
         }
         if constexpr (NG > 1) {
-            constexpr int PER = HD / 2 + 4;  // floats per lane
+            constexpr int PER = F::PER;
+            named_barrier(1, F::NW * 32);  // the last tile's join has been read
             for (int h = NG / 2; h >= 1; h >>= 1) {
+                // rounds after the first write where this warp has read
                 if (grp >= h && grp < 2 * h) {
-                    // rounds after the first write where this warp has read
                     float* x = sX + (((h == NG / 2 ? grp - h : grp) * MW + mt) * PER) * 32 + lane;
 #pragma unroll
-                    for (int i = 0; i < NT; ++i)
+                    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[(4 * i + e) * 32] = O[i][e];
-                    x[(PER - 4) * 32] = M0;
-                    x[(PER - 3) * 32] = M1;
-                    x[(PER - 2) * 32] = l0;
-                    x[(PER - 1) * 32] = l1;
+                        for (int d = 0; d < DT; ++d)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                x[((n * DT + d) * 4 + i) * 32] = O[d][n][i];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            x[(4 * NT * DT + 4 * n + e) * 32] = M[n][e];
+                            x[(4 * NT * DT + 4 * n + 2 + e) * 32] = l[n][e];
+                        }
+                    }
                 }
                 named_barrier(1, F::NW * 32);
                 if (grp < h) {
                     const float* x =
                         sX + (((h == NG / 2 ? grp : grp + h) * MW + mt) * PER) * 32 + lane;
-                    const float B0 = x[(PER - 4) * 32], B1 = x[(PER - 3) * 32];
-                    const float N0 = fmaxf(M0, B0), N1 = fmaxf(M1, B1);
-                    const float R0 = N0 == -INFINITY ? 0.f : N0, R1 = N1 == -INFINITY ? 0.f : N1;
-                    const float a0 = ex2(M0 - R0), a1 = ex2(M1 - R1);
-                    const float b0 = ex2(B0 - R0), b1 = ex2(B1 - R1);
-                    M0 = N0, M1 = N1;
-                    l0 = l0 * a0 + x[(PER - 2) * 32] * b0;
-                    l1 = l1 * a1 + x[(PER - 1) * 32] * b1;
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        O[i][0] = O[i][0] * a0 + x[(4 * i + 0) * 32] * b0;
-                        O[i][1] = O[i][1] * a0 + x[(4 * i + 1) * 32] * b0;
-                        O[i][2] = O[i][2] * a1 + x[(4 * i + 2) * 32] * b1;
-                        O[i][3] = O[i][3] * a1 + x[(4 * i + 3) * 32] * b1;
+                    for (int n = 0; n < NT; ++n) {
+                        float fa[2], fb[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float B = x[(4 * NT * DT + 4 * n + e) * 32];
+                            const float N = fmaxf(M[n][e], B), R = N == -INFINITY ? 0.f : N;
+                            fa[e] = ex2(M[n][e] - R);
+                            fb[e] = ex2(B - R);
+                            M[n][e] = N;
+                            l[n][e] = l[n][e] * fa[e] +
+                                      x[(4 * NT * DT + 4 * n + 2 + e) * 32] * fb[e];
+                        }
+#pragma unroll
+                        for (int d = 0; d < DT; ++d)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                O[d][n][i] = O[d][n][i] * fa[i & 1] +
+                                             x[((n * DT + d) * 4 + i) * 32] * fb[i & 1];
                     }
                 }
             }
@@ -739,61 +899,50 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
 
         // ---- store: the finished rows, or this piece of them
         if (grp == 0 && wrows > 0) {
-#pragma unroll
-            for (int o = 1; o <= 2; o <<= 1) {
-                l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-                l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-            }
             const bool piece = cut_l || cut_r;
             const int64_t pslot = 2 * (int64_t)blockIdx.x + (cut_l ? 0 : 1);
-            float* part = a.part + (pslot * TR + mt * 16) * HD;
-            float2* stat = a.stat + pslot * TR + mt * 16;
-            const float i0 = piece ? 1.f : l0 == 0.f ? 0.f : 1.f / l0;
-            const float i1 = piece ? 1.f : l1 == 0.f ? 0.f : 1.f / l1;
-            if (piece && t4 == 0) {
-                stat[g] = make_float2(M0, l0);
-                stat[g + 8] = make_float2(M1, l1);
-            }
-            // a row that sees nothing has no sum: zeros, whatever O holds
-            auto put = [&](int row, int64_t off, bool on, int d, float4 v) {
-                if (piece) *reinterpret_cast<float4*>(part + row * HD + d) = v;
-                else if (on) store4<X, F>(a, v, off + d);
-            };
-            const bool on0 = g < wrows, on1 = g + 8 < wrows;
-            if constexpr (F::kQ8) {
 #pragma unroll
-                for (int c = 0; c < HD / 16; ++c) {
-                    const float(&x)[4] = O[2 * c];
-                    const float(&y)[4] = O[2 * c + 1];
-                    put(g, off0, on0, 16 * c + 4 * t4,
-                        make_float4(x[0] * i0, y[0] * i0, x[1] * i0, y[1] * i0));
-                    if (two)
-                        put(g + 8, off1, on1, 16 * c + 4 * t4,
-                            make_float4(x[2] * i1, y[2] * i1, x[3] * i1, y[3] * i1));
-                }
-            } else {
-                // two lanes exchange halves so that each stores 16 bytes of fp32
-                const bool up = t4 & 1;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int c = 0; c < NT / 2; ++c) {
-                    const float(&x)[4] = O[2 * c];
-                    const float(&y)[4] = O[2 * c + 1];
-                    // even lanes take tile 2c, odd lanes tile 2c + 1
-                    const float sa = up ? x[0] : y[0], sb = up ? x[1] : y[1];
-                    const float ra = __shfl_xor_sync(0xffffffffu, sa, 1);
-                    const float rb = __shfl_xor_sync(0xffffffffu, sb, 1);
-                    const float4 v = up ? make_float4(ra * i0, rb * i0, y[0] * i0, y[1] * i0)
-                                        : make_float4(x[0] * i0, x[1] * i0, ra * i0, rb * i0);
-                    const int d = 16 * c + (up ? 8 : 0) + 4 * (t4 >> 1);
-                    put(g, off0, on0, d, v);
-                    const float sc = up ? x[2] : y[2], sd = up ? x[3] : y[3];
-                    const float rc = __shfl_xor_sync(0xffffffffu, sc, 1);
-                    const float rd = __shfl_xor_sync(0xffffffffu, sd, 1);
-                    const float4 w = up ? make_float4(rc * i1, rd * i1, y[2] * i1, y[3] * i1)
-                                        : make_float4(x[2] * i1, x[3] * i1, rc * i1, rd * i1);
-                    if (two) put(g + 8, off1, on1, d, w);
+                for (int e = 0; e < 2; ++e) {
+                    float sum = l[n][e];
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                    const int r = 8 * n + 2 * t4 + e;
+                    if (r >= wrows) continue;
+                    if (piece) {
+                        const int64_t row = pslot * TR + mt * F::WR + r;
+                        if (g == 0) a.stat[row] = make_float2(M[n][e], sum);
+                        float* o = a.part + row * HD;
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) {
+                            if constexpr (F::kQ8) {
+                                *reinterpret_cast<float2*>(o + 16 * d + 2 * g) =
+                                    make_float2(O[d][n][e], O[d][n][2 + e]);
+                            } else {
+                                o[16 * d + g] = O[d][n][e];
+                                o[16 * d + 8 + g] = O[d][n][2 + e];
+                            }
+                        }
+                    } else {
+                        // a row that sees nothing has no sum: zeros
+                        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                        const RowRef rr(a, p, pr + r);
+                        X* o = static_cast<X*>(a.out) + (int64_t)(p.row + rr.tok) * a.out_stride +
+                               (int64_t)rr.head * HD;
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) {
+                            if constexpr (F::kQ8) {
+                                store1<X, F>(o + 16 * d + 2 * g, O[d][n][e] * inv);
+                                store1<X, F>(o + 16 * d + 2 * g + 1, O[d][n][2 + e] * inv);
+                            } else {
+                                store1<X, F>(o + 16 * d + g, O[d][n][e] * inv);
+                                store1<X, F>(o + 16 * d + 8 + g, O[d][n][2 + e] * inv);
+                            }
+                        }
+                    }
                 }
-            }
         }
         if (cut_r && !cut_l) {
             owner = true;
@@ -828,7 +977,7 @@ struct PagedJob {
     PagedArgs a;
     const ftc_kv_pages* c;
     PagedSet set;
-    int cls;  // 0: 16 rows a tile, 1: 64, 2: as many as fit
+    int cls;  // 0: 8 rows a tile, 1: 16, 2: 64, 3: as many as fit
     cudaStream_t st;
 };
 
@@ -837,10 +986,9 @@ int page_map(CUtensorMap* m, const void* base, const ftc_kv_pages* c, int key_st
 // Shortest range of chunks worth a CTA of its own, in rounds of its groups.
 constexpr int kLeastRounds = 2;
 
-template <typename X, typename C, int HD, int MW, int NW>
+template <class F>
 int launch_cfg(const PagedJob& j) {
-    using F = Cfg<X, C, HD, MW, NW>;
-    auto fn = paged_mma<X, C, F>;
+    auto fn = paged_mma<F>;
     int rc = opt_in_smem(reinterpret_cast<const void*>(fn), F::SMEM,
                          "cudaFuncSetAttribute(paged_mma)");
     if (rc) return rc;
@@ -863,9 +1011,8 @@ int launch_cfg(const PagedJob& j) {
     return FTC_OK;
 }
 
-template <typename X, typename C, int HD, int MW, int NW>
+template <class F>
 PagedSet geom_cfg() {
-    using F = Cfg<X, C, HD, MW, NW>;
     return {F::OCC * device_sms(), F::TR};
 }
 

@@ -259,10 +259,6 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
 
     if (warp == 0) {
         // -------------------------------------------------------- producer
-        if (lane == 0) {
-            prefetch_tensormap(&tk);
-            prefetch_tensormap(&tv);
-        }
         const int box = min(a.b.page_size, KS), boxes = KS / box;
         constexpr int NBOX = F::kQ8 ? 1 : HD / 64;  // 128-byte columns
         uint32_t it = 0;

@@ -6,40 +6,40 @@
 namespace ftc {
 namespace paged {
 
-// Class 2 runs on tcgen05 with 16-bit queries: fp32 ones need their sums kept
+// Class 3 runs on tcgen05 with 16-bit queries: fp32 ones need their sums kept
 // out of the matrix unit's accumulator, and head_dim 256 its tensor memory.
 template <typename X, int HD>
 constexpr bool kTc = sizeof(X) == 2 && HD < 256;
 
-// The class's shape elsewhere: 4 warps on 16 rows, 4 warps of 16 rows, and 8
-// warps of 16 rows (head_dim 256: 4, nine warps leave a thread too few
-// registers).
+// The class's shape elsewhere: 4 warps in turn on 8 rows and on 16, 4 warps
+// of 16 rows, and 8 warps of 16 rows (head_dim 256: 4, nine warps leave a
+// thread too few registers).
 template <typename X, typename C, int HD, class Fn>
 auto with_class(int cls, Fn fn) {
-    using std::integral_constant;
-    constexpr int big = HD < 256 ? 8 : 4;
-    return cls == 0   ? fn(integral_constant<int, 1>(), integral_constant<int, 4>())
-           : cls == 1 ? fn(integral_constant<int, 4>(), integral_constant<int, 4>())
-                      : fn(integral_constant<int, big>(), integral_constant<int, big>());
+    if (cls == 0) return fn((Cfg<X, C, HD, 1, 1, 4>*)nullptr);
+    if (cls == 1) return fn((Cfg<X, C, HD, 2, 1, 4>*)nullptr);
+    if (cls == 2 || HD == 256) return fn((Cfg<X, C, HD, 2, 4, 4>*)nullptr);
+    constexpr int big = HD == 256 || kTc<X, HD> ? 4 : 8;
+    return fn((Cfg<X, C, HD, 2, big, big>*)nullptr);
 }
 
 template <typename X, typename C, int HD>
 int launch_class(const PagedJob& j) {
     if constexpr (kTc<X, HD>) {
-        if (j.cls == 2) return launch_tc<X, C, HD>(j);
+        if (j.cls == 3) return launch_tc<X, C, HD>(j);
     }
-    return with_class<X, C, HD>(j.cls, [&](auto mw, auto nw) {
-        return launch_cfg<X, C, HD, decltype(mw)::value, decltype(nw)::value>(j);
+    return with_class<X, C, HD>(j.cls, [&](auto* f) {
+        return launch_cfg<typename std::remove_pointer<decltype(f)>::type>(j);
     });
 }
 
 template <typename X, typename C, int HD>
 PagedSet geom_class(int cls) {
     if constexpr (kTc<X, HD>) {
-        if (cls == 2) return {device_sms(), TcCfg<X, C, HD>::TR};
+        if (cls == 3) return {device_sms(), TcCfg<X, C, HD>::TR};
     }
-    return with_class<X, C, HD>(cls, [&](auto mw, auto nw) {
-        return geom_cfg<X, C, HD, decltype(mw)::value, decltype(nw)::value>();
+    return with_class<X, C, HD>(cls, [&](auto* f) {
+        return geom_cfg<typename std::remove_pointer<decltype(f)>::type>();
     });
 }
 
