@@ -15,7 +15,8 @@
 //
 // Warps: 0 brings K and V by TMA, one box per page (V as it lies in the cache:
 // positions by head_dim, the MN-major B operand of PV); 1 issues MMAs; 4-7 and
-// 8-11 are the softmax of the two stages, a thread per row; 12-15 turn 8-bit
+// 8-11 are the softmax of the two stages, a thread per row, its 128 scores in
+// registers (of which these warps get 216 and the others 72); 2-3 turn 8-bit
 // codes into f16 tiles, and in tiles where some row's mask hides something they
 // take V elements that are not finite out (0 x inf would reach every row),
 // which the rows that see them get back at the end.  8-bit scales stay in fp32:
@@ -55,7 +56,9 @@ struct TcCfg {
     static constexpr int OFF_SC = OFF_RAW + (kQ8 ? NR * RAW : 0);
     static constexpr int OFF_BAR = OFF_SC + NSC * (kQ8 ? 2 * KS * 4 : 0);
     static constexpr int SMEM = OFF_BAR + 1024 + 1024;
-    static constexpr int THREADS = 512;
+    static constexpr int THREADS = 384, NPREP = 2;
+    // registers a thread: 384 x 168 at launch, then 128 x 72 + 256 x 216
+    static constexpr int kRegsFew = 72, kRegsMany = 216;
     static_assert(SMEM <= 227 * 1024, "shared memory");
     static_assert(NSL * TILE >= Plan<TR, KS>::kSmem, "the plan's prefix sums fit in the ring");
 };
@@ -79,6 +82,16 @@ __device__ __forceinline__ uint64_t f2fma(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
+}
+
+__device__ __forceinline__ uint64_t f2u(uint32_t a, uint32_t b) {
+    return (uint64_t)a | ((uint64_t)b << 32);
+}
+// (a, b) *= k
+__device__ __forceinline__ void scale2(uint32_t& a, uint32_t& b, uint64_t k) {
+    const uint64_t v = f2mul(f2u(a, b), k);
+    a = (uint32_t)v;
+    b = (uint32_t)(v >> 32);
 }
 
 // Loads done: ties the registers to the wait, so that no use moves above it.
@@ -166,6 +179,15 @@ __device__ __noinline__ void add_odd(const PagedArgs& a, const PlanPos& p,
     }
 }
 
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 template <class F>
 __global__ void __launch_bounds__(F::THREADS, 1)
 paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -206,16 +228,16 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
     if (threadIdx.x == 0) {
         for (int i = 0; i < F::NSL; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&ready[i], 4);
+            mbar_init(&ready[i], F::NPREP);
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < F::NR; ++i) {
             mbar_init(&raw_full[i], 1);
-            mbar_init(&raw_empty[i], 4);
+            mbar_init(&raw_empty[i], F::NPREP);
         }
         for (int i = 0; i < F::NSC; ++i) {
             mbar_init(&sc_full[i], 1);
-            mbar_init(&sc_empty[i], 12);
+            mbar_init(&sc_empty[i], 8 + F::NPREP);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 4);
@@ -257,6 +279,8 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
     const uint32_t tmem = *tmem_slot;
     PlanPos p = *sPos;
 
+    if (warp < 4) {
+        regs_dec<F::kRegsFew>();
     if (warp == 0) {
         // -------------------------------------------------------- producer
         const int box = min(a.b.page_size, KS), boxes = KS / box;
@@ -405,9 +429,10 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             }
         }
         __syncwarp();
-    } else if (warp >= 12) {
+    } else {
         // --------------------------------------------- operand preparation
-        const int w = warp - 12;
+        const int w = warp - 2;
+        constexpr int ROWS = KS / F::NPREP;
         uint32_t it = 0;
         for (int left = total; left > 0;) {
             const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
@@ -432,7 +457,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                         const int c = lane % LPR;           // 16 codes of a row
                         const bool swap = (c >> 2) & 1;     // other bank half first
 #pragma unroll 4
-                        for (int r = w * 32 + lane / LPR; r < w * 32 + 32; r += RPI) {
+                        for (int r = w * ROWS + lane / LPR; r < (w + 1) * ROWS; r += RPI) {
                             const uint4 u = *reinterpret_cast<const uint4*>(src + r * HD + 16 * c);
                             const uint32_t x0 = u.x ^ 0x80808080u, x1 = u.y ^ 0x80808080u;
                             const uint32_t x2 = u.z ^ 0x80808080u, x3 = u.w ^ 0x80808080u;
@@ -467,7 +492,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                         constexpr uint32_t kOne = F::kHalf ? 0x04000400u : 0x00800080u;
                         uint4* v = reinterpret_cast<uint4*>(sRing + s * F::TILE);
 #pragma unroll 4
-                        for (int q = w * 32 + lane; q < F::TILE / 16; q += 128) {
+                        for (int q = w * 32 + lane; q < F::TILE / 16; q += 32 * F::NPREP) {
                             uint4 u = v[q];
                             uint32_t* x = reinterpret_cast<uint32_t*>(&u);
                             uint32_t z = 0;
@@ -493,8 +518,10 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             left -= m;
             if (left > 0) P::next_tile(a, p);
         }
-    } else if (warp >= 4) {
+    }
+    } else {
         // --------------------------------------------------------- softmax
+        regs_inc<F::kRegsMany>();
         const int st = warp >= 8 ? 1 : 0;
         const int r = (warp & 3) * 32 + lane;  // row of the stage, TMEM lane
         const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + st * 128;
@@ -577,68 +604,62 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                     const bool whole = flag == 0xFF && key0 + KS - 1 <= p_lo &&
                                        (a.window == 0 || p_hi - key0 < a.window ||
                                         key0 + KS - 1 < a.n_sink);
-                    // ---- the row's maximum (masked scores go back as -inf)
-                    float mx = -INFINITY;
-                    uint32_t s[32];
+                    // ---- the row's scores and their maximum
+                    uint32_t s[4][32];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        tmem_ld_32x32b_x32(tS + 32 * q, s);
-                        tmem_ld_done(s);
-                        if (!whole) {
-                            const int hi = pos - key0 - 32 * q;
-                            const int lo = a.window > 0 ? hi - a.window + 1 : INT_MIN;
-                            const int sk = a.n_sink - key0 - 32 * q;
+                    for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x32(tS + 32 * q, s[q]);
+                    tmem_ld_done(s[0]);
+                    tmem_ld_done(s[1]);
+                    tmem_ld_done(s[2]);
+                    tmem_ld_done(s[3]);
+                    if constexpr (F::kQ8) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const bool on = (flag >> (2 * q + i / 16)) & 1;
-                                if (!(on && i <= hi && (i >= lo || i < sk)))
-                                    s[i] = 0xFF800000u;
+                        for (int q = 0; q < 4; ++q) {
+                            float4 k4[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) k4[i] = ksc[8 * q + i];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                scale2(s[q][4 * i], s[q][4 * i + 1], f2(k4[i].x, k4[i].y));
+                                scale2(s[q][4 * i + 2], s[q][4 * i + 3], f2(k4[i].z, k4[i].w));
                             }
-                            tmem_st_x32(tS + 32 * q, s);
                         }
-                        float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const uint32_t* u = s + i;
-                            float v0 = __uint_as_float(s[i]), v1 = __uint_as_float(s[i + 1]);
-                            float v2 = __uint_as_float(s[i + 2]), v3 = __uint_as_float(s[i + 3]);
-                            if constexpr (F::kQ8) {
-                                const float4 k4 = ksc[8 * q + i / 4];
-                                const uint64_t a2 = f2mul(f2(v0, v1), f2(k4.x, k4.y));
-                                const uint64_t b2 = f2mul(f2(v2, v3), f2(k4.z, k4.w));
-                                v0 = f2lo(a2), v1 = f2hi(a2), v2 = f2lo(b2), v3 = f2hi(b2);
-                                if (!whole) {  // hidden, whatever the scale there
-                                    if (u[0] == 0xFF800000u) v0 = -INFINITY;
-                                    if (u[1] == 0xFF800000u) v1 = -INFINITY;
-                                    if (u[2] == 0xFF800000u) v2 = -INFINITY;
-                                    if (u[3] == 0xFF800000u) v3 = -INFINITY;
-                                }
-                            }
-                            m0 = fmaxf(m0, fmaxf(v0, v1));
-                            m1 = fmaxf(m1, fmaxf(v2, v3));
-                        }
-                        mx = fmaxf(mx, fmaxf(m0, m1));
                     }
-                    if (!whole) tmem_st_wait();
-                    mx *= c;
+                    if (!whole) {
+                        const int hi = pos - key0;
+                        const int lo = a.window > 0 ? hi - a.window + 1 : INT_MIN;
+                        const int sk = a.n_sink - key0;
+#pragma unroll
+                        for (int i = 0; i < 128; ++i) {
+                            const bool on = (flag >> (i / 16)) & 1;
+                            if (!(on && i <= hi && (i >= lo || i < sk)))
+                                s[i / 32][i % 32] = 0xFF800000u;
+                        }
+                    }
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                m4[k] = fmaxf(m4[k], fmaxf(__uint_as_float(s[q][i + 2 * k]),
+                                                           __uint_as_float(s[q][i + 2 * k + 1])));
+                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
                     int Et = E;
                     if constexpr (F::kQ8) {
                         // V's largest scale in this tile, of positions some row may see
-                        float top = 0.f;
                         const float4 v4 = vsc[lane];
-                        if ((flag >> (lane / 4)) & 1) {
-                            const int k = key0 + 4 * lane;
-                            if (k <= tw.p_last) top = fabsf(v4.x);
-                            if (k + 1 <= tw.p_last) top = fmaxf(top, fabsf(v4.y));
-                            if (k + 2 <= tw.p_last) top = fmaxf(top, fabsf(v4.z));
-                            if (k + 3 <= tw.p_last) top = fmaxf(top, fabsf(v4.w));
-                        }
-                        uint32_t tb = __float_as_uint(top);
-                        if (tb > 0x7F800000u) tb = 0;  // a NaN scale says nothing
-#pragma unroll
-                        for (int o = 16; o > 0; o >>= 1)
-                            tb = max(tb, __shfl_xor_sync(0xffffffffu, tb, o));
-                        Et = max(E, min((int)(tb >> 23) - 126, 126));
+                        const int k = key0 + 4 * lane;
+                        const int n = ((flag >> (lane / 4)) & 1) ? tw.p_last - k : -1;
+                        auto bits = [&](float v, int at) {
+                            const uint32_t b = __float_as_uint(fabsf(v));
+                            return at <= n && b < 0x7F800000u ? b : 0u;
+                        };
+                        const uint32_t top = __reduce_max_sync(
+                            0xffffffffu, max(max(bits(v4.x, 0), bits(v4.y, 1)),
+                                             max(bits(v4.z, 2), bits(v4.w, 3))));
+                        Et = max(E, min((int)(top >> 23) - 126, 126));
                     }
                     if (__any_sync(0xffffffffu, mx > M + 8.f || Et > E)) {
                         const float N = fmaxf(M, mx);
@@ -648,55 +669,48 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                         E = Et;
                         l2 = f2mul(l2, f2(f, f));
                         if (j > 0) {
-#pragma unroll
+#pragma unroll 1
                             for (int q = 0; q < HD / 32; ++q) {
-                                tmem_ld_32x32b_x32(tO + 32 * q, s);
-                                tmem_ld_done(s);
+                                uint32_t o[32];
+                                tmem_ld_32x32b_x32(tO + 32 * q, o);
+                                tmem_ld_done(o);
 #pragma unroll
                                 for (int i = 0; i < 32; ++i)
-                                    s[i] = __float_as_uint(__uint_as_float(s[i]) * f);
-                                tmem_st_x32(tO + 32 * q, s);
+                                    o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tmem_st_x32(tO + 32 * q, o);
                             }
                         }
                     }
                     // ---- weights 2^(z - D), packed over the scores
                     const float D = kUp - (M == -INFINITY ? 0.f : M) - (float)(F::kQ8 ? E : 0);
                     const uint64_t c2 = f2(c, c), d2 = f2(D, D);
+                    uint64_t lb = 0;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        tmem_ld_32x32b_x32(tS + 32 * q, s);
-                        tmem_ld_done(s);
                         uint32_t w[16];
+                        float4 v4[F::kQ8 ? 8 : 1];
+                        if constexpr (F::kQ8) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) v4[i] = vsc[8 * q + i];
+                        }
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            uint64_t z0 = f2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                            uint64_t z1 = f2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
-                            if constexpr (F::kQ8) {
-                                const float4 k4 = ksc[8 * q + i / 4];
-                                z0 = f2mul(z0, f2(k4.x, k4.y));
-                                z1 = f2mul(z1, f2(k4.z, k4.w));
-                                if (!whole) {  // -inf times a scale of a hidden position
-                                    z0 = f2(s[i] == 0xFF800000u ? -INFINITY : f2lo(z0),
-                                            s[i + 1] == 0xFF800000u ? -INFINITY : f2hi(z0));
-                                    z1 = f2(s[i + 2] == 0xFF800000u ? -INFINITY : f2lo(z1),
-                                            s[i + 3] == 0xFF800000u ? -INFINITY : f2hi(z1));
-                                }
-                            }
-                            z0 = f2fma(z0, c2, d2);
-                            z1 = f2fma(z1, c2, d2);
+                            const uint64_t z0 = f2fma(f2u(s[q][i], s[q][i + 1]), c2, d2);
+                            const uint64_t z1 = f2fma(f2u(s[q][i + 2], s[q][i + 3]), c2, d2);
                             float w0 = ex2(f2lo(z0)), w1 = ex2(f2hi(z0));
                             float w2 = ex2(f2lo(z1)), w3 = ex2(f2hi(z1));
-                            l2 = f2add(l2, f2add(f2(w0, w1), f2(w2, w3)));
+                            l2 = f2add(l2, f2(w0, w1));
+                            lb = f2add(lb, f2(w2, w3));
                             if constexpr (F::kQ8) {
-                                const float4 v4 = vsc[8 * q + i / 4];
-                                if (!whole) {
-                                    w0 = w0 == 0.f ? 0.f : w0 * v4.x;
-                                    w1 = w1 == 0.f ? 0.f : w1 * v4.y;
-                                    w2 = w2 == 0.f ? 0.f : w2 * v4.z;
-                                    w3 = w3 == 0.f ? 0.f : w3 * v4.w;
+                                const float4 v = v4[i / 4];
+                                if (!whole) {  // a hidden position's scale may be anything
+                                    w0 = w0 == 0.f ? 0.f : w0 * v.x;
+                                    w1 = w1 == 0.f ? 0.f : w1 * v.y;
+                                    w2 = w2 == 0.f ? 0.f : w2 * v.z;
+                                    w3 = w3 == 0.f ? 0.f : w3 * v.w;
                                 } else {
-                                    const uint64_t y0 = f2mul(f2(w0, w1), f2(v4.x, v4.y));
-                                    const uint64_t y1 = f2mul(f2(w2, w3), f2(v4.z, v4.w));
+                                    const uint64_t y0 = f2mul(f2(w0, w1), f2(v.x, v.y));
+                                    const uint64_t y1 = f2mul(f2(w2, w3), f2(v.z, v.w));
                                     w0 = f2lo(y0), w1 = f2hi(y0), w2 = f2lo(y1), w3 = f2hi(y1);
                                 }
                             }
@@ -705,6 +719,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                         }
                         tmem_st_x16(tS + 16 * q, w);
                     }
+                    l2 = f2add(l2, lb);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
