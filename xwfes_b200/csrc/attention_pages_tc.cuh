@@ -50,6 +50,7 @@ struct TcCfg {
     static constexpr int RAW = kQ8 ? KS * HD : 0;
     static constexpr int NR = kQ8 ? 3 : 1;
     static constexpr int NSC = 3;
+    static constexpr bool kPoly = false;
     static constexpr int OFF_RING = 0;
     static constexpr int OFF_Q = OFF_RING + NSL * TILE;
     static constexpr int OFF_RAW = OFF_Q + QB;
@@ -87,11 +88,52 @@ __device__ __forceinline__ uint64_t f2fma(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t f2u(uint32_t a, uint32_t b) {
     return (uint64_t)a | ((uint64_t)b << 32);
 }
+__device__ __forceinline__ void scale2f(float& a, float& b, uint64_t k) {
+    const uint64_t v = f2mul(f2(a, b), k);
+    a = f2lo(v);
+    b = f2hi(v);
+}
 // (a, b) *= k
 __device__ __forceinline__ void scale2(uint32_t& a, uint32_t& b, uint64_t k) {
     const uint64_t v = f2mul(f2u(a, b), k);
     a = (uint32_t)v;
     b = (uint32_t)(v >> 32);
+}
+
+// max of three, NaN if one of them is (an fmaxf chain would lose it).
+__device__ __forceinline__ float max3n(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 2^z of a pair on the FMA pipe: z = n + f, |f| <= 1/2 (adding 1.5 * 2^23
+// rounds), a minimax polynomial for 2^f (relative error 2^-13.7 with degree 3,
+// below a bf16 weight's rounding; 2^-18.5 with 4, for f16), n added to the
+// exponent.  z below -126 counts as that.
+template <bool kFine>
+__device__ __forceinline__ void ex2_pair(uint64_t z, float& a, float& b) {
+    z = f2(fmaxf(f2lo(z), -126.f), fmaxf(f2hi(z), -126.f));
+    const uint64_t r = f2add(z, f2(12582912.f, 12582912.f));
+    const uint64_t f = f2fma(f2add(r, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), z);
+    uint64_t p;
+    if constexpr (kFine) {
+        p = f2fma(f, f2(0.009570102f, 0.009570102f), f2(0.05591786f, 0.05591786f));
+        p = f2fma(f, p, f2(0.24024744f, 0.24024744f));
+        p = f2fma(f, p, f2(0.6931218f, 0.6931218f));
+        p = f2fma(f, p, f2(0.9999993f, 0.9999993f));
+    } else {
+        p = f2fma(f, f2(0.05517167f, 0.05517167f), f2(0.24261113f, 0.24261113f));
+        p = f2fma(f, p, f2(0.693261f, 0.693261f));
+        p = f2fma(f, p, f2(0.99992806f, 0.99992806f));
+    }
+    a = __uint_as_float((uint32_t)p + ((uint32_t)r << 23));
+    b = __uint_as_float((uint32_t)(p >> 32) + ((uint32_t)(r >> 32) << 23));
+}
+
+// Bits below n, of 32.
+__device__ __forceinline__ uint32_t low_bits(int n) {
+    return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
 }
 
 // Loads done: ties the registers to the wait, so that no use moves above it.
@@ -145,11 +187,53 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(const void* tile, uint32_
     return d;
 }
 
-__device__ __forceinline__ bool one_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-    if (*dead) return false;
-    if (mbar_wait(bar, parity)) return true;
-    *dead = 1;
-    return false;
+// 1 in one lane of the warp, the same one every time.
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t e;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(e));
+    return e;
+}
+
+__device__ __forceinline__ uint64_t uniform(uint64_t v) {
+    const uint32_t lo = __shfl_sync(0xffffffffu, (uint32_t)v, 0);
+    const uint32_t hi = __shfl_sync(0xffffffffu, (uint32_t)(v >> 32), 0);
+    return (uint64_t)lo | ((uint64_t)hi << 32);
+}
+
+// The MMAs and the commit of sm100.cuh, by the lane whose `lead` is 1.
+__device__ __forceinline__ void umma_ss_lead(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t acc, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_ts_lead(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t acc, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+        : "memory");
+}
+
+__device__ __forceinline__ void commit_lead(uint64_t* bar, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+            smem_u32(bar)), "r"(lead)
+        : "memory");
 }
 
 // V elements that are not finite, of the positions that a row sees, added to
@@ -214,7 +298,8 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
     uint64_t* q_full = sc_empty + F::NSC;  // [2]
     uint64_t* s_full = q_full + 2;
     uint64_t* p_full = s_full + 2;
-    uint64_t* o_full = p_full + 2;
+    uint64_t* p_half = p_full + 2;   // keys 0-63 of p_full
+    uint64_t* o_full = p_half + 2;
     uint64_t* o_empty = o_full + 2;
     uint64_t* drain = o_empty + 2;
     volatile int* dead = reinterpret_cast<volatile int*>(drain + 1);
@@ -243,6 +328,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             mbar_init(&q_full[i], 4);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
+            mbar_init(&p_half[i], 4);
             mbar_init(&o_full[i], 1);
             mbar_init(&o_empty[i], 4);
         }
@@ -281,244 +367,263 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
 
     if (warp < 4) {
         regs_dec<F::kRegsFew>();
-    if (warp == 0) {
-        // -------------------------------------------------------- producer
-        const int box = min(a.b.page_size, KS), boxes = KS / box;
-        constexpr int NBOX = F::kQ8 ? 1 : HD / 64;  // 128-byte columns
-        uint32_t it = 0;
-        for (int left = total; left > 0 && !*dead;) {
-            const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
-            const int m = min(tw.count - p.i, left);
-            for (int j = 0; j < m; ++j, ++it) {
-                const int key0 = tw.key0(p.i + j);
-                const int id = lane < boxes ? page_of(a.b, p.s, key0 + lane * box) : -1;
-                const unsigned on = __ballot_sync(0xffffffffu, id >= 0);
-                const int y = p.kvh * a.b.page_size + (key0 & (a.b.page_size - 1));
-                const int ss = it % F::NSC;
-                if (!ring_wait(&sc_empty[ss], ((it / F::NSC) & 1) ^ 1, dead)) break;
-                if (lane == 0) {
-                    int flag = 0;  // a bit per 16 positions
-                    for (int b = 0; b < boxes; ++b)
-                        if ((on >> b) & 1) flag |= ((1 << (box / 16)) - 1) << (b * box / 16);
-                    sFlag[ss] = flag;
-                    if constexpr (F::kQ8)
-                        mbar_arrive_expect_tx(&sc_full[ss], __popc(on) * 2 * box * 4);
-                    else mbar_arrive(&sc_full[ss]);
-                }
-                __syncwarp();
-                if constexpr (F::kQ8) {
-                    if (id >= 0) {
-                        const int64_t src = (int64_t)id * a.b.scale_stride + y;
-                        bulk_copy(sScale + (ss * 2 + 0) * KS + lane * box, a.ks + src, box * 4,
-                                  &sc_full[ss]);
-                        bulk_copy(sScale + (ss * 2 + 1) * KS + lane * box, a.vs + src, box * 4,
-                                  &sc_full[ss]);
-                    }
-                }
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    const uint32_t t = 2 * it + kv;
-                    uint64_t* bar;
-                    uint8_t* dst;
-                    if constexpr (F::kQ8) {
-                        const int s = t % F::NR;
-                        if (!ring_wait(&raw_empty[s], ((t / F::NR) & 1) ^ 1, dead)) break;
-                        bar = &raw_full[s];
-                        dst = sRaw + s * F::RAW;
-                        if (lane == 0) mbar_arrive_expect_tx(bar, F::RAW);
-                    } else {
-                        const int s = t % F::NSL;
-                        if (!ring_wait(&empty[s], ((t / F::NSL) & 1) ^ 1, dead)) break;
-                        bar = &full[s];
-                        dst = sRing + s * F::TILE;
-                        if (lane == 0) mbar_arrive_expect_tx(bar, F::TILE);
-                    }
-                    __syncwarp();
-                    const int b = lane / NBOX, col = lane % NBOX;
-                    const int pg = __shfl_sync(0xffffffffu, id, b);
-                    if (b < boxes)  // past the last page: zeros
-                        tma_box(dst + col * F::SUB + b * box * (F::kQ8 ? HD : 128),
-                                kv ? &tv : &tk, col * 64, y, pg < 0 ? a.b.n_pages : pg, bar);
-                    __syncwarp();
-                }
-                if (*dead) break;
-            }
-            left -= m;
-            if (left > 0) P::next_tile(a, p);
-        }
-        if (*dead && lane == 0) {  // let issued copies land before the CTA leaves
-            for (int i = 0; i < F::NSC; ++i) {
-                mbar_wait(&sc_full[i], 0);
-                mbar_wait(&sc_full[i], 1);
-            }
-            for (int i = 0; i < (F::kQ8 ? F::NR : F::NSL); ++i) {
-                uint64_t* b = F::kQ8 ? &raw_full[i] : &full[i];
-                mbar_wait(b, 0);
-                mbar_wait(b, 1);
-            }
-        }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------- MMA
-        if (lane == 0) {
-            constexpr uint32_t fmt = F::kHalf ? 0u : 1u;
-            constexpr uint32_t id_s = idesc_f16(fmt, 128, KS);
-            constexpr uint32_t id_o = idesc_f16(fmt, 128, HD) | (1u << 16);  // B is MN-major
-            uint32_t it = 0, np[2] = {0, 0}, no[2] = {0, 0};  // no: segments of a stage
-            auto operand = [&](uint32_t t) -> uint8_t* {
-                const int s = t % F::NSL;
-                uint64_t* b = F::kQ8 || (t & 1) ? &ready[s] : &full[s];
-                // ready of a 16-bit ring only counts V tiles (odd t, even NSL)
-                if (!one_wait(b, (t / F::NSL) & 1, dead)) return nullptr;
-                tc_fence_after();
-                return sRing + s * F::TILE;
-            };
-            auto scores = [&](int i, const uint8_t* kt) {
-#pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const uint64_t dq = smem_desc_k_sw128(sQ + i * F::TILE + (k / 4) * F::SUB);
-                    const uint64_t dk = smem_desc_k_sw128(kt + (k / 4) * F::SUB);
-                    umma_f16_ss(tmem + i * 128, dq + 2 * (k % 4), dk + 2 * (k % 4), id_s, k != 0);
-                }
-                umma_commit(&s_full[i]);
-            };
+        if (warp == 0) {
+            // -------------------------------------------------------- producer
+            const int box = min(a.b.page_size, KS), boxes = KS / box;
+            constexpr int NBOX = F::kQ8 ? 1 : HD / 64;  // 128-byte columns
+            uint32_t it = 0;
             for (int left = total; left > 0 && !*dead;) {
                 const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
                 const int m = min(tw.count - p.i, left);
-                const int stages = p.n * a.gqa - p.t * TR > 128 ? 2 : 1;
-                const uint8_t* kt = operand(2 * it);
-                if (!kt) break;
-                for (int i = 0; i < stages; ++i) {
-                    if (!one_wait(&q_full[i], no[i] & 1, dead)) break;
-                    tc_fence_after();
-                    scores(i, kt);
+                for (int j = 0; j < m; ++j, ++it) {
+                    const int key0 = tw.key0(p.i + j);
+                    const int id = lane < boxes ? page_of(a.b, p.s, key0 + lane * box) : -1;
+                    const unsigned on = __ballot_sync(0xffffffffu, id >= 0);
+                    const int y = p.kvh * a.b.page_size + (key0 & (a.b.page_size - 1));
+                    const int ss = it % F::NSC;
+                    if (!ring_wait(&sc_empty[ss], ((it / F::NSC) & 1) ^ 1, dead)) break;
+                    if (lane == 0) {
+                        int flag = 0;  // a bit per 16 positions
+                        for (int b = 0; b < boxes; ++b)
+                            if ((on >> b) & 1) flag |= ((1 << (box / 16)) - 1) << (b * box / 16);
+                        sFlag[ss] = flag;
+                        if constexpr (F::kQ8)
+                            mbar_arrive_expect_tx(&sc_full[ss], __popc(on) * 2 * box * 4);
+                        else mbar_arrive(&sc_full[ss]);
+                    }
+                    __syncwarp();
+                    if constexpr (F::kQ8) {
+                        if (id >= 0) {
+                            const int64_t src = (int64_t)id * a.b.scale_stride + y;
+                            bulk_copy(sScale + (ss * 2 + 0) * KS + lane * box, a.ks + src, box * 4,
+                                      &sc_full[ss]);
+                            bulk_copy(sScale + (ss * 2 + 1) * KS + lane * box, a.vs + src, box * 4,
+                                      &sc_full[ss]);
+                        }
+                    }
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const uint32_t t = 2 * it + kv;
+                        uint64_t* bar;
+                        uint8_t* dst;
+                        if constexpr (F::kQ8) {
+                            const int s = t % F::NR;
+                            if (!ring_wait(&raw_empty[s], ((t / F::NR) & 1) ^ 1, dead)) break;
+                            bar = &raw_full[s];
+                            dst = sRaw + s * F::RAW;
+                            if (lane == 0) mbar_arrive_expect_tx(bar, F::RAW);
+                        } else {
+                            const int s = t % F::NSL;
+                            if (!ring_wait(&empty[s], ((t / F::NSL) & 1) ^ 1, dead)) break;
+                            bar = &full[s];
+                            dst = sRing + s * F::TILE;
+                            if (lane == 0) mbar_arrive_expect_tx(bar, F::TILE);
+                        }
+                        __syncwarp();
+                        const int b = lane / NBOX, col = lane % NBOX;
+                        const int pg = __shfl_sync(0xffffffffu, id, b);
+                        if (b < boxes)  // past the last page: zeros
+                            tma_box(dst + col * F::SUB + b * box * (F::kQ8 ? HD : 128),
+                                    kv ? &tv : &tk, col * 64, y, pg < 0 ? a.b.n_pages : pg, bar);
+                        __syncwarp();
+                    }
+                    if (*dead) break;
                 }
-                umma_commit(&empty[2 * it % F::NSL]);
+                left -= m;
+                if (left > 0) P::next_tile(a, p);
+            }
+            if (*dead && lane == 0) {  // let issued copies land before the CTA leaves
+                for (int i = 0; i < F::NSC; ++i) {
+                    mbar_wait(&sc_full[i], 0);
+                    mbar_wait(&sc_full[i], 1);
+                }
+                for (int i = 0; i < (F::kQ8 ? F::NR : F::NSL); ++i) {
+                    uint64_t* b = F::kQ8 ? &raw_full[i] : &full[i];
+                    mbar_wait(b, 0);
+                    mbar_wait(b, 1);
+                }
+            }
+        } else if (warp == 1) {
+            // ------------------------------------------------------------- MMA
+            // The whole warp runs this, one elected lane issues: an MMA of 128
+            // x 128 x 16 takes 64 clocks, and operands in uniform registers are
+            // what lets one be issued in less.
+            constexpr uint32_t fmt = F::kHalf ? 0u : 1u;
+            constexpr uint32_t id_s = idesc_f16(fmt, 128, KS);
+            constexpr uint32_t id_o = idesc_f16(fmt, 128, HD) | (1u << 16);  // B is MN-major
+            const uint32_t lead = elect_lane();
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint64_t dq0 = uniform(smem_desc_k_sw128(sQ));
+            const uint64_t dk0 = uniform(smem_desc_k_sw128(sRing));
+            const uint64_t dv0 = uniform(smem_desc_mn_sw128(sRing, F::SUB));
+            uint32_t it = 0, np[2] = {0, 0}, no[2] = {0, 0};  // no: segments of a stage
+            // slot of operand tile t once it is there, as descriptor offset
+            auto operand = [&](uint32_t t, uint32_t& off) -> bool {
+                const int s = t % F::NSL;
+                // ready of a 16-bit ring only counts V tiles (odd t, even NSL)
+                uint64_t* b = F::kQ8 || (t & 1) ? &ready[s] : &full[s];
+                if (!ring_wait(b, (t / F::NSL) & 1, dead)) return false;
+                tc_fence_after();
+                off = __shfl_sync(0xffffffffu, (uint32_t)s * (F::TILE >> 4), 0);
+                return true;
+            };
+            auto scores = [&](int i, uint32_t koff) {
+                const uint64_t dq = dq0 + i * (F::TILE >> 4), dk = dk0 + koff;
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const int o = (k / 4) * (F::SUB >> 4) + 2 * (k % 4);
+                    umma_ss_lead(tm + i * 128, dq + o, dk + o, id_s, k != 0, lead);
+                }
+                commit_lead(&s_full[i], lead);
+            };
+            for (int left = total; left > 0;) {
+                const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
+                const int m = min(tw.count - p.i, left);
+                const int stages = p.n * a.gqa - p.t * TR > 128 ? 2 : 1;
+                uint32_t koff, voff = 0;
+                bool on = operand(2 * it, koff);
+                for (int i = 0; on && i < stages; ++i) {
+                    on = ring_wait(&q_full[i], no[i] & 1, dead);
+                    if (!on) break;
+                    tc_fence_after();
+                    scores(i, koff);
+                }
+                if (!on) break;
+                commit_lead(&empty[2 * it % F::NSL], lead);
                 for (int j = 0; j < m; ++j) {
-                    const uint8_t* vt = nullptr;
-                    kt = nullptr;
-                    for (int i = 0; i < stages; ++i) {
-                        if (!one_wait(&p_full[i], np[i]++ & 1, dead)) break;
-                        if (i == 0 && !(vt = operand(2 * (it + j) + 1))) break;
-                        if (j == 0 && !one_wait(&o_empty[i], (no[i] & 1) ^ 1, dead)) break;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (i >= stages) break;
+                        on = ring_wait(&p_half[i], np[i] & 1, dead) &&
+                             (i != 0 || operand(2 * (it + j) + 1, voff)) &&
+                             (j != 0 || ring_wait(&o_empty[i], (no[i] & 1) ^ 1, dead));
+                        if (!on) break;
+                        tc_fence_after();
+                        const uint64_t dv = dv0 + voff;
+#pragma unroll
+                        for (int k = 0; k < KS / 32; ++k)
+                            umma_ts_lead(tm + 256 + i * 128, tm + i * 128 + 8 * k, dv + k * 128,
+                                         id_o, j != 0 || k != 0, lead);
+                        on = ring_wait(&p_full[i], np[i]++ & 1, dead);
+                        if (!on) break;
                         tc_fence_after();
 #pragma unroll
-                        for (int k = 0; k < KS / 16; ++k)
-                            umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k,
-                                        smem_desc_mn_sw128(vt + k * 2048, F::SUB), id_o,
-                                        j != 0 || k != 0);
+                        for (int k = KS / 32; k < KS / 16; ++k)
+                            umma_ts_lead(tm + 256 + i * 128, tm + i * 128 + 8 * k, dv + k * 128,
+                                         id_o, 1, lead);
                         if (j + 1 < m) {
-                            if (i == 0 && !(kt = operand(2 * (it + j + 1)))) break;
-                            scores(i, kt);
+                            on = i != 0 || operand(2 * (it + j + 1), koff);
+                            if (!on) break;
+                            scores(i, koff);
                         } else {
-                            umma_commit(&o_full[i]);
+                            commit_lead(&o_full[i], lead);
                             ++no[i];
                         }
                     }
-                    if (*dead) break;
-                    umma_commit(&empty[(2 * (it + j) + 1) % F::NSL]);
-                    if (j + 1 < m) umma_commit(&empty[2 * (it + j + 1) % F::NSL]);
+                    if (!on) break;
+                    commit_lead(&empty[(2 * (it + j) + 1) % F::NSL], lead);
+                    if (j + 1 < m) commit_lead(&empty[2 * (it + j + 1) % F::NSL], lead);
                 }
-                if (*dead) break;
+                if (!on) break;
                 it += m;
                 left -= m;
                 if (left > 0) P::next_tile(a, p);
             }
             if (*dead) {  // nothing of this CTA may be in flight when it leaves
-                umma_commit(drain);
-                mbar_wait(drain, 0);
+                commit_lead(drain, lead);
+                mbar_wait_warp(drain, 0);
             }
-        }
-        __syncwarp();
-    } else {
-        // --------------------------------------------- operand preparation
-        const int w = warp - 2;
-        constexpr int ROWS = KS / F::NPREP;
-        uint32_t it = 0;
-        for (int left = total; left > 0;) {
-            const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
-            const int m = min(tw.count - p.i, left);
-            for (int j = 0; j < m; ++j, ++it) {
-                const int ss = it % F::NSC;
-                ring_wait(&sc_full[ss], (it / F::NSC) & 1, dead);
-                const int flag = sFlag[ss];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sc_empty[ss]);
-                if constexpr (F::kQ8) {
+            __syncwarp();
+        } else {
+            // --------------------------------------------- operand preparation
+            const int w = warp - 2;
+            constexpr int ROWS = KS / F::NPREP;
+            uint32_t it = 0;
+            for (int left = total; left > 0;) {
+                const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
+                const int m = min(tw.count - p.i, left);
+                for (int j = 0; j < m; ++j, ++it) {
+                    const int ss = it % F::NSC;
+                    ring_wait(&sc_full[ss], (it / F::NSC) & 1, dead);
+                    const int flag = sFlag[ss];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_empty[ss]);
+                    if constexpr (F::kQ8) {
 #pragma unroll
-                    for (int kv = 0; kv < 2; ++kv) {
-                        const uint32_t t = 2 * it + kv;
-                        const int rs = t % F::NR, s = t % F::NSL;
-                        if (!ring_wait(&raw_full[rs], (t / F::NR) & 1, dead)) continue;
-                        if (!ring_wait(&empty[s], ((t / F::NSL) & 1) ^ 1, dead)) continue;
-                        const uint8_t* src = sRaw + rs * F::RAW;
-                        uint8_t* dst = sRing + s * F::TILE;
-                        constexpr int LPR = HD / 16;        // lanes per row
-                        constexpr int RPI = 32 / LPR;       // rows per step
-                        const int c = lane % LPR;           // 16 codes of a row
-                        const bool swap = (c >> 2) & 1;     // other bank half first
+                        for (int kv = 0; kv < 2; ++kv) {
+                            const uint32_t t = 2 * it + kv;
+                            const int rs = t % F::NR, s = t % F::NSL;
+                            if (!ring_wait(&raw_full[rs], (t / F::NR) & 1, dead)) continue;
+                            if (!ring_wait(&empty[s], ((t / F::NSL) & 1) ^ 1, dead)) continue;
+                            const uint8_t* src = sRaw + rs * F::RAW;
+                            uint8_t* dst = sRing + s * F::TILE;
+                            constexpr int LPR = HD / 16;        // lanes per row
+                            constexpr int RPI = 32 / LPR;       // rows per step
+                            const int c = lane % LPR;           // 16 codes of a row
+                            const bool swap = (c >> 2) & 1;     // other bank half first
 #pragma unroll 4
-                        for (int r = w * ROWS + lane / LPR; r < (w + 1) * ROWS; r += RPI) {
-                            const uint4 u = *reinterpret_cast<const uint4*>(src + r * HD + 16 * c);
-                            const uint32_t x0 = u.x ^ 0x80808080u, x1 = u.y ^ 0x80808080u;
-                            const uint32_t x2 = u.z ^ 0x80808080u, x3 = u.w ^ 0x80808080u;
-                            const uint4 lo = make_uint4(codes2<0x4140>(x0), codes2<0x4342>(x0),
-                                                        codes2<0x4140>(x1), codes2<0x4342>(x1));
-                            const uint4 hi = make_uint4(codes2<0x4140>(x2), codes2<0x4342>(x2),
-                                                        codes2<0x4140>(x3), codes2<0x4342>(x3));
-                            uint8_t* row = dst + (c >> 2) * F::SUB + r * 128;
-                            const int ch = 2 * (c & 3);
-                            *reinterpret_cast<uint4*>(row + (((ch + swap) ^ (r & 7)) << 4)) =
-                                swap ? hi : lo;
-                            *reinterpret_cast<uint4*>(row + (((ch + !swap) ^ (r & 7)) << 4)) =
-                                swap ? lo : hi;
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) {
-                            mbar_arrive(&ready[s]);
-                            mbar_arrive(&raw_empty[rs]);
-                        }
-                    }
-                } else {
-                    const uint32_t t = 2 * it + 1;
-                    const int s = t % F::NSL;
-                    if (!ring_wait(&full[s], (t / F::NSL) & 1, dead)) continue;
-                    const int key0 = tw.key0(p.i + j);
-                    const bool whole = flag == 0xFF && key0 + KS - 1 <= tw.p_first &&
-                                       (a.window == 0 || tw.p_last - key0 < a.window ||
-                                        key0 + KS - 1 < a.n_sink);
-                    if (!whole) {
-                        constexpr uint32_t kInf = F::kHalf ? 0x7C007C00u : 0x7F807F80u;
-                        constexpr uint32_t kOne = F::kHalf ? 0x04000400u : 0x00800080u;
-                        uint4* v = reinterpret_cast<uint4*>(sRing + s * F::TILE);
-#pragma unroll 4
-                        for (int q = w * 32 + lane; q < F::TILE / 16; q += 32 * F::NPREP) {
-                            uint4 u = v[q];
-                            uint32_t* x = reinterpret_cast<uint32_t*>(&u);
-                            uint32_t z = 0;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) z |= (x[i] & kInf) + kOne;
-                            if (z & 0x80008000u) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const uint32_t b = ((x[i] & kInf) + kOne) & 0x80008000u;
-                                    x[i] &= ~((b & 0x8000u ? 0xFFFFu : 0u) |
-                                              (b & 0x80000000u ? 0xFFFF0000u : 0u));
-                                }
-                                v[q] = u;
-                                *odd = 1;
+                            for (int r = w * ROWS + lane / LPR; r < (w + 1) * ROWS; r += RPI) {
+                                const uint4 u = *reinterpret_cast<const uint4*>(src + r * HD + 16 * c);
+                                const uint32_t x0 = u.x ^ 0x80808080u, x1 = u.y ^ 0x80808080u;
+                                const uint32_t x2 = u.z ^ 0x80808080u, x3 = u.w ^ 0x80808080u;
+                                const uint4 lo = make_uint4(codes2<0x4140>(x0), codes2<0x4342>(x0),
+                                                            codes2<0x4140>(x1), codes2<0x4342>(x1));
+                                const uint4 hi = make_uint4(codes2<0x4140>(x2), codes2<0x4342>(x2),
+                                                            codes2<0x4140>(x3), codes2<0x4342>(x3));
+                                uint8_t* row = dst + (c >> 2) * F::SUB + r * 128;
+                                const int ch = 2 * (c & 3);
+                                *reinterpret_cast<uint4*>(row + (((ch + swap) ^ (r & 7)) << 4)) =
+                                    swap ? hi : lo;
+                                *reinterpret_cast<uint4*>(row + (((ch + !swap) ^ (r & 7)) << 4)) =
+                                    swap ? lo : hi;
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                mbar_arrive(&ready[s]);
+                                mbar_arrive(&raw_empty[rs]);
                             }
                         }
-                        fence_proxy_async_smem();
-                        __syncwarp();
+                    } else {
+                        const uint32_t t = 2 * it + 1;
+                        const int s = t % F::NSL;
+                        if (!ring_wait(&full[s], (t / F::NSL) & 1, dead)) continue;
+                        const int key0 = tw.key0(p.i + j);
+                        const bool whole = flag == 0xFF && key0 + KS - 1 <= tw.p_first &&
+                                           (a.window == 0 || tw.p_last - key0 < a.window ||
+                                            key0 + KS - 1 < a.n_sink);
+                        if (!whole) {
+                            constexpr uint32_t kInf = F::kHalf ? 0x7C007C00u : 0x7F807F80u;
+                            constexpr uint32_t kOne = F::kHalf ? 0x04000400u : 0x00800080u;
+                            uint4* v = reinterpret_cast<uint4*>(sRing + s * F::TILE);
+#pragma unroll 4
+                            for (int q = w * 32 + lane; q < F::TILE / 16; q += 32 * F::NPREP) {
+                                uint4 u = v[q];
+                                uint32_t* x = reinterpret_cast<uint32_t*>(&u);
+                                uint32_t z = 0;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) z |= (x[i] & kInf) + kOne;
+                                if (z & 0x80008000u) {
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        const uint32_t b = ((x[i] & kInf) + kOne) & 0x80008000u;
+                                        x[i] &= ~((b & 0x8000u ? 0xFFFFu : 0u) |
+                                                  (b & 0x80000000u ? 0xFFFF0000u : 0u));
+                                    }
+                                    v[q] = u;
+                                    *odd = 1;
+                                }
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                        }
+                        if (lane == 0) mbar_arrive(&ready[s]);
                     }
-                    if (lane == 0) mbar_arrive(&ready[s]);
                 }
+                left -= m;
+                if (left > 0) P::next_tile(a, p);
             }
-            left -= m;
-            if (left > 0) P::next_tile(a, p);
         }
-    }
     } else {
         // --------------------------------------------------------- softmax
         regs_inc<F::kRegsMany>();
@@ -625,27 +730,30 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                             }
                         }
                     }
+                    uint32_t seen[4];  // of the row, when a mask hides something
                     if (!whole) {
-                        const int hi = pos - key0;
-                        const int lo = a.window > 0 ? hi - a.window + 1 : INT_MIN;
-                        const int sk = a.n_sink - key0;
+                        const int hi = pos - key0 + 1;
+                        const int lo = a.window > 0 ? max(hi - a.window, 0) : 0;
+                        const int sk = a.window > 0 ? a.n_sink - key0 : 0;
 #pragma unroll
-                        for (int i = 0; i < 128; ++i) {
-                            const bool on = (flag >> (i / 16)) & 1;
-                            if (!(on && i <= hi && (i >= lo || i < sk)))
-                                s[i / 32][i % 32] = 0xFF800000u;
+                        for (int q = 0; q < 4; ++q) {
+                            seen[q] = low_bits(hi - 32 * q) &
+                                      (~low_bits(lo - 32 * q) | low_bits(sk - 32 * q)) &
+                                      (((flag >> (2 * q)) & 1 ? 0xFFFFu : 0u) |
+                                       ((flag >> (2 * q)) & 2 ? 0xFFFF0000u : 0u));
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (!((seen[q] >> i) & 1)) s[q][i] = 0xFF800000u;
                         }
                     }
                     float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                m4[k] = fmaxf(m4[k], fmaxf(__uint_as_float(s[q][i + 2 * k]),
-                                                           __uint_as_float(s[q][i + 2 * k + 1])));
-                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
+                        for (int i = 0; i < 32; i += 2)
+                            m4[q] = max3n(m4[q], __uint_as_float(s[q][i]),
+                                          __uint_as_float(s[q][i + 1]));
+                    const float mx = max3n(max3n(m4[0], m4[1], m4[2]), m4[3], m4[3]) * c;
                     int Et = E;
                     if constexpr (F::kQ8) {
                         // V's largest scale in this tile, of positions some row may see
@@ -681,8 +789,11 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                             }
                         }
                     }
-                    // ---- weights 2^(z - D), packed over the scores
-                    const float D = kUp - (M == -INFINITY ? 0.f : M) - (float)(F::kQ8 ? E : 0);
+                    // ---- weights 2^(z - D), packed over the scores; a visible NaN
+                    // makes all of them NaN
+                    const float D = mx != mx ? mx
+                                             : kUp - (M == -INFINITY ? 0.f : M) -
+                                                   (float)(F::kQ8 ? E : 0);
                     const uint64_t c2 = f2(c, c), d2 = f2(D, D);
                     uint64_t lb = 0;
 #pragma unroll
@@ -697,33 +808,39 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                         for (int i = 0; i < 32; i += 4) {
                             const uint64_t z0 = f2fma(f2u(s[q][i], s[q][i + 1]), c2, d2);
                             const uint64_t z1 = f2fma(f2u(s[q][i + 2], s[q][i + 3]), c2, d2);
-                            float w0 = ex2(f2lo(z0)), w1 = ex2(f2hi(z0));
-                            float w2 = ex2(f2lo(z1)), w3 = ex2(f2hi(z1));
+                            float w0 = ex2(f2lo(z0)), w1 = ex2(f2hi(z0)), w2, w3;
+                            // three pairs of eight on the FMA pipe
+                            if (F::kPoly && i % 16 != 4) {
+                                ex2_pair<F::kHalf>(z1, w2, w3);
+                            } else {
+                                w2 = ex2(f2lo(z1));
+                                w3 = ex2(f2hi(z1));
+                            }
                             l2 = f2add(l2, f2(w0, w1));
                             lb = f2add(lb, f2(w2, w3));
                             if constexpr (F::kQ8) {
                                 const float4 v = v4[i / 4];
+                                scale2f(w0, w1, f2(v.x, v.y));
+                                scale2f(w2, w3, f2(v.z, v.w));
                                 if (!whole) {  // a hidden position's scale may be anything
-                                    w0 = w0 == 0.f ? 0.f : w0 * v.x;
-                                    w1 = w1 == 0.f ? 0.f : w1 * v.y;
-                                    w2 = w2 == 0.f ? 0.f : w2 * v.z;
-                                    w3 = w3 == 0.f ? 0.f : w3 * v.w;
-                                } else {
-                                    const uint64_t y0 = f2mul(f2(w0, w1), f2(v.x, v.y));
-                                    const uint64_t y1 = f2mul(f2(w2, w3), f2(v.z, v.w));
-                                    w0 = f2lo(y0), w1 = f2hi(y0), w2 = f2lo(y1), w3 = f2hi(y1);
+                                    if (!((seen[q] >> i) & 1)) w0 = 0.f;
+                                    if (!((seen[q] >> (i + 1)) & 1)) w1 = 0.f;
+                                    if (!((seen[q] >> (i + 2)) & 1)) w2 = 0.f;
+                                    if (!((seen[q] >> (i + 3)) & 1)) w3 = 0.f;
                                 }
                             }
                             w[i / 2] = pack<OT>(w0, w1);
                             w[i / 2 + 1] = pack<OT>(w2, w3);
                         }
                         tmem_st_x16(tS + 16 * q, w);
+                        if (q & 1) {  // half of the keys: its products may begin
+                            tmem_st_wait();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(q == 1 ? &p_half[st] : &p_full[st]);
+                        }
                     }
                     l2 = f2add(l2, lb);
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[st]);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sc_empty[ss]);
@@ -734,7 +851,8 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                 tc_fence_after();
                 const bool piece = cut_l || cut_r;
                 const float l = f2lo(l2) + f2hi(l2);
-                const float inv = piece ? 1.f : l == 0.f ? 0.f : 1.f / l;
+                // no finite score seen: zeros, unless it was a NaN
+                const float inv = piece ? 1.f : M == -INFINITY && l == l ? 0.f : 1.f / l;
                 const int64_t pslot = 2 * (int64_t)blockIdx.x + (cut_l ? 0 : 1);
                 float* part = a.part + (pslot * TR + st * 128 + r) * HD;
                 if (piece)
