@@ -220,6 +220,7 @@ __device__ __forceinline__ uint32_t chunk_off(int r, int c) {
 }
 
 __device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     if (__any_sync(0xffffffffu, *dead != 0)) return false;
     if (mbar_wait_warp(bar, parity)) return true;
     *dead = 1;

@@ -1,29 +1,35 @@
 // attention_pages_tc.cuh -- the paged attention of long chunks with 16-bit
 // queries on the tcgen05 tensor cores.
 //
-// A tile is 256 packed rows, two stages of 128; its keys come 128 at a time.
-// Per stage and key tile, S = Q K^T (128 x 128) and O += P V (128 x head_dim)
-// accumulate in tensor memory: S 128 columns, the weights P written over it as
-// 16-bit A operand, O head_dim columns.  One thread issues all MMAs,
-//   S0(0) S1(0) | PV0(j) S0(j+1) PV1(j) S1(j+1) | ...
-// so that the tensor cores work on one stage while the other's softmax runs.
-// The MMAs of one thread run in order, which is what makes S(j+1) after PV(j)
-// safe on the same columns, and what lets the softmax warps rescale O: when
-// S(j) has arrived, PV(j-1) is done and PV(j) waits for this stage's P.
-// Rescaling is lazy: the reference maximum only moves when a score passes it by
-// 2^8, which f16 weights leave room for (they sit 2^7 up).
+// A tile is 256 packed rows, two stages of 128; its keys come 64 at a time.
+// Per stage and key chunk, S = Q K^T (128 x 64) and O += P V (128 x head_dim)
+// accumulate in tensor memory: two S buffers of 64 columns, the weights P
+// written over their S as 16-bit A operand, O head_dim columns.  One warp
+// issues all MMAs, per chunk u and stage
+//   PV(u), then S(u + 2) into the buffer that P(u) has left,
+// so a stage's next scores are there before its weights are done and the
+// softmax warps never wait for the tensor cores: an MMA takes its 64 clocks,
+// but a batch of 8 comes back only ~500 clocks after its last issue, and with
+// one S buffer of 128 keys that latency stood in every step (5000 clocks per
+// 128 keys, 2048 of them MMAs).  MMAs of one warp run in order, which makes
+// S(u + 2) after PV(u) safe on the same columns.
+// Rescaling O is lazy: the reference maximum only moves when a score passes it
+// by 2^8, which f16 weights leave room for (they sit 2^7 up); then the softmax
+// warp waits for PV(u - 1) and multiplies O in tensor memory itself.
 //
 // Warps: 0 brings K and V by TMA, one box per page (V as it lies in the cache:
-// positions by head_dim, the MN-major B operand of PV); 1 issues MMAs; 4-7 and
-// 8-11 are the softmax of the two stages, a thread per row, its 128 scores in
-// registers (of which these warps get 216 and the others 72); 2-3 turn 8-bit
-// codes into f16 tiles, and in tiles where some row's mask hides something they
-// take V elements that are not finite out (0 x inf would reach every row),
-// which the rows that see them get back at the end.  8-bit scales stay in fp32:
-// K's multiplies S, V's multiplies P, relative to its running maximum 2^E.
+// positions by head_dim, the MN-major B operand of PV); 1 issues MMAs; 2 and 3
+// fetch a stage's q rows of the next tile as soon as this tile's last scores
+// are issued; 8-11 and 12-15 are the softmax of the two stages, a thread per
+// row; 4-7 turn 8-bit codes into f16 tiles, and in chunks where some row's mask
+// hides something they take V elements that are not finite out (0 x inf would
+// reach every row), which the rows that see them get back at the end.  8-bit
+// scales stay in fp32: K's multiplies S, V's multiplies P, relative to its
+// running maximum 2^E.
 //
-// What bounds it: per key tile and stage pair the tensor cores need 4 x 512
-// clocks at head_dim 128, and the exponentials, 16 a clock, as many.
+// What bounds it: per 128 keys and stage pair the tensor cores need 2048
+// clocks at head_dim 128 (2560 with the narrow S, whose operands are what
+// shared memory can feed), and the exponentials, 16 a clock, 2048.
 #pragma once
 
 #include <climits>
@@ -37,31 +43,32 @@ template <typename X_, typename C_, int HD_>
 struct TcCfg {
     using X = X_;
     using C = C_;
-    static constexpr int HD = HD_, TR = 256, KS = 128;
+    static constexpr int HD = HD_, TR = 256, KS = 64;
     static constexpr bool kQ8 = sizeof(C) == 1;
     using OT = typename std::conditional<std::is_same<C, __nv_bfloat16>::value, __nv_bfloat16,
                                          __half>::type;
     static constexpr bool kHalf = std::is_same<OT, __half>::value;
     static constexpr bool kRowScale = kHalf && !std::is_same<X, __half>::value;
-    static constexpr int SUB = KS * 128;           // 64 dimensions of 128 rows
-    static constexpr int TILE = SUB * (HD / 64);   // K or V tile, 16-bit
-    static constexpr int QB = 2 * TILE;
-    static constexpr int NSL = kQ8 ? (HD == 128 ? 3 : 4) : (HD == 128 ? 4 : 6);
+    static constexpr int SUB = KS * 128;           // 64 dimensions of a chunk's rows
+    static constexpr int TILE = SUB * (HD / 64);   // K or V chunk, 16-bit
+    static constexpr int QSUB = 128 * 128;         // 64 dimensions of a stage's rows
+    static constexpr int QTILE = QSUB * (HD / 64);
+    static constexpr int NS = kQ8 && HD == 128 ? 3 : 4;  // slots of the K and of the V ring
     static constexpr int RAW = kQ8 ? KS * HD : 0;
-    static constexpr int NR = kQ8 ? 3 : 1;
-    static constexpr int NSC = 3;
-    static constexpr bool kPoly = false;
-    static constexpr int OFF_RING = 0;
-    static constexpr int OFF_Q = OFF_RING + NSL * TILE;
-    static constexpr int OFF_RAW = OFF_Q + QB;
+    static constexpr int NR = 4;                   // raw slots, K and V as they come
+    static constexpr int NSC = 4;
+    static constexpr int NPREP = 4;
+    static constexpr int OFF_K = 0;
+    static constexpr int OFF_V = OFF_K + NS * TILE;
+    static constexpr int OFF_Q = OFF_V + NS * TILE;
+    static constexpr int OFF_RAW = OFF_Q + 2 * QTILE;
     static constexpr int OFF_SC = OFF_RAW + (kQ8 ? NR * RAW : 0);
-    static constexpr int OFF_BAR = OFF_SC + NSC * (kQ8 ? 2 * KS * 4 : 0);
+    static constexpr int OFF_C = OFF_SC + NSC * (kQ8 ? 2 * KS * 4 : 0);
+    static constexpr int OFF_BAR = OFF_C + (kRowScale ? 4 * TR * 4 : 0);
     static constexpr int SMEM = OFF_BAR + 1024 + 1024;
-    static constexpr int THREADS = 384, NPREP = 2;
-    // registers a thread: 384 x 168 at launch, then 128 x 72 + 256 x 216
-    static constexpr int kRegsFew = 72, kRegsMany = 216;
+    static constexpr int THREADS = 512;
     static_assert(SMEM <= 227 * 1024, "shared memory");
-    static_assert(NSL * TILE >= Plan<TR, KS>::kSmem, "the plan's prefix sums fit in the ring");
+    static_assert(2 * NS * TILE >= Plan<TR, KS>::kSmem, "the plan's prefix sums fit in the rings");
 };
 
 __device__ __forceinline__ uint64_t f2(float a, float b) {
@@ -107,33 +114,19 @@ __device__ __forceinline__ float max3n(float a, float b, float c) {
     return d;
 }
 
-// 2^z of a pair on the FMA pipe: z = n + f, |f| <= 1/2 (adding 1.5 * 2^23
-// rounds), a minimax polynomial for 2^f (relative error 2^-13.7 with degree 3,
-// below a bf16 weight's rounding; 2^-18.5 with 4, for f16), n added to the
-// exponent.  z below -126 counts as that.
-template <bool kFine>
-__device__ __forceinline__ void ex2_pair(uint64_t z, float& a, float& b) {
-    z = f2(fmaxf(f2lo(z), -126.f), fmaxf(f2hi(z), -126.f));
-    const uint64_t r = f2add(z, f2(12582912.f, 12582912.f));
-    const uint64_t f = f2fma(f2add(r, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), z);
-    uint64_t p;
-    if constexpr (kFine) {
-        p = f2fma(f, f2(0.009570102f, 0.009570102f), f2(0.05591786f, 0.05591786f));
-        p = f2fma(f, p, f2(0.24024744f, 0.24024744f));
-        p = f2fma(f, p, f2(0.6931218f, 0.6931218f));
-        p = f2fma(f, p, f2(0.9999993f, 0.9999993f));
-    } else {
-        p = f2fma(f, f2(0.05517167f, 0.05517167f), f2(0.24261113f, 0.24261113f));
-        p = f2fma(f, p, f2(0.693261f, 0.693261f));
-        p = f2fma(f, p, f2(0.99992806f, 0.99992806f));
-    }
-    a = __uint_as_float((uint32_t)p + ((uint32_t)r << 23));
-    b = __uint_as_float((uint32_t)(p >> 32) + ((uint32_t)(r >> 32) << 23));
-}
-
 // Bits below n, of 32.
 __device__ __forceinline__ uint32_t low_bits(int n) {
     return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
+}
+
+// The positions of 32 from key0 + 32 q that a row at `pos` sees, as bits.
+__device__ __forceinline__ uint32_t seen_bits(const PagedArgs& a, int pos, int key0, int flag,
+                                              int q) {
+    const int hi = pos - key0 + 1 - 32 * q;
+    const uint32_t near = a.window > 0 ? ~low_bits(hi - a.window) | low_bits(a.n_sink - key0 - 32 * q)
+                                       : 0xFFFFFFFFu;
+    return low_bits(hi) & near &
+           (((flag >> (2 * q)) & 1 ? 0xFFFFu : 0u) | ((flag >> (2 * q)) & 2 ? 0xFFFF0000u : 0u));
 }
 
 // Loads done: ties the registers to the wait, so that no use moves above it.
@@ -263,58 +256,162 @@ __device__ __noinline__ void add_odd(const PagedArgs& a, const PlanPos& p,
     }
 }
 
-template <int N>
-__device__ __forceinline__ void regs_dec() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+// 32 words a lane as 8 chunks of 4: lane i of each 8 comes to hold chunk i of
+// the 8 lanes' rows (word 4 k + j: row k), so that 8 lanes store 128
+// neighbouring bytes (a thread storing its own row touches 32 lines an
+// instruction).
+__device__ __forceinline__ void turn8(uint32_t (&v)[32]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int b = 1; b < 8; b <<= 1) {
+        const bool up = lane & b;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (c & b) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t& lo = v[4 * c + j];
+                uint32_t& hi = v[4 * (c | b) + j];
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, b);
+                if (up) lo = got;
+                else hi = got;
+            }
+        }
+    }
 }
-template <int N>
-__device__ __forceinline__ void regs_inc() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+
+// One stage's q rows into the K-major operand tile by a warp, all of them in
+// flight at once; where they become f16, a power of two per row brings the
+// largest value to [2^14, 2^15) and goes to the score factor.
+template <class F>
+__device__ __forceinline__ void load_q(const PagedArgs& a, const PlanPos& p, int pr0, int rows,
+                                       uint8_t* tile, float* sC) {
+    using X = typename F::X;
+    using OT = typename F::OT;
+    constexpr int LPR = F::HD / 8;   // lanes to a row
+    constexpr int RPI = 32 / LPR;    // rows a step
+    const int lane = threadIdx.x & 31, c = lane % LPR;
+    auto at = [&](int r) {
+        return tile + (c / 8) * F::QSUB + r * 128 + (((c % 8) ^ (r & 7)) << 4);
+    };
+#pragma unroll 2
+    for (int r = lane / LPR; r < 128; r += RPI) {
+        const int pr = pr0 + r;
+        if (pr < rows) {
+            const RowRef rr(a, p, pr);
+            cp_async16(at(r), static_cast<const X*>(a.q) + (int64_t)(p.row + rr.tok) * a.q_stride +
+                                  (int64_t)rr.head * F::HD + 8 * c);
+        } else {
+            *reinterpret_cast<uint4*>(at(r)) = make_uint4(0, 0, 0, 0);
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if constexpr (F::kRowScale) {
+        // (a lane converts the chunks that it brought)
+#pragma unroll 4
+        for (int r = lane / LPR; r < 128; r += RPI) {
+            uint4 u = *reinterpret_cast<const uint4*>(at(r));
+            uint32_t* x = reinterpret_cast<uint32_t*>(&u);
+            uint32_t top = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                top = max(top, max((x[k] << 16) & 0x7FFF0000u, x[k] & 0x7FFF0000u));
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1)
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int e = top > 0 && top < 0x7F800000u ? (int)(top >> 23) - 141 : 0;
+            const float fa = pow2(-e / 2), fb = pow2(-e - -e / 2);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 v = unpack<X>(x[k]);
+                x[k] = pack<OT>(v.x * fa * fb, v.y * fa * fb);
+            }
+            if (c == 0) sC[r] = fmaxf(a.c * pow2(e / 2) * pow2(e - e / 2), 1e-38f);
+            *reinterpret_cast<uint4*>(at(r)) = u;
+        }
+    }
 }
+
+// The chunks of a CTA's share, one after another.
+template <class F>
+struct Walk {
+    PlanPos p;
+    int left, m, j;  // chunks to go, of this segment, done of it
+    TileWork<F::TR, F::KS> tw;
+
+    __device__ __forceinline__ Walk(const PagedArgs& a, const PlanPos& p0, int total)
+        : p(p0), left(total), j(0), tw(a, p0.n, p0.len, p0.t) {
+        m = min(tw.count - p.i, left);
+    }
+    __device__ __forceinline__ int key0() const { return tw.key0(p.i + j); }
+    __device__ __forceinline__ int stages(const PagedArgs& a) const {
+        return p.n * a.gqa - p.t * F::TR > 128 ? 2 : 1;
+    }
+    __device__ __forceinline__ bool first() const { return j == 0; }
+    __device__ __forceinline__ bool last() const { return j + 1 == m; }
+    __device__ __forceinline__ void next(const PagedArgs& a) {
+        --left;
+        if (++j < m || left == 0) return;
+        Plan<F::TR, F::KS>::next_tile(a, p);
+        tw = TileWork<F::TR, F::KS>(a, p.n, p.len, p.t);
+        m = min(tw.count, left);
+        j = 0;
+    }
+};
 
 template <class F>
 __global__ void __launch_bounds__(F::THREADS, 1)
 paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
          const __grid_constant__ PagedArgs a, int least) {
     using X = typename F::X;
-    using C = typename F::C;
     using OT = typename F::OT;
-    constexpr int HD = F::HD, TR = F::TR, KS = F::KS;
+    constexpr int HD = F::HD, TR = F::TR, KS = F::KS, NS = F::NS;
     using P = Plan<TR, KS>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sRing = smem + F::OFF_RING;
+    uint8_t* sK = smem + F::OFF_K;
+    uint8_t* sV = smem + F::OFF_V;
     uint8_t* sQ = smem + F::OFF_Q;
     uint8_t* sRaw = smem + F::OFF_RAW;
-    float* sScale = reinterpret_cast<float*>(smem + F::OFF_SC);  // [NSC][K, V][128]
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + F::OFF_BAR);  // 16-bit tiles landed
-    uint64_t* ready = full + F::NSL;     // tile is an operand (converted, cleaned)
-    uint64_t* empty = ready + F::NSL;    // its MMAs are done
-    uint64_t* raw_full = empty + F::NSL;
+    float* sScale = reinterpret_cast<float*>(smem + F::OFF_SC);  // [NSC][K, V][KS]
+    float* sC = reinterpret_cast<float*>(smem + F::OFF_C);       // [4][2][128] score factors
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + F::OFF_BAR);  // 16-bit chunks landed
+    uint64_t* v_full = k_full + NS;
+    uint64_t* k_ready = v_full + NS;     // converted; 16-bit: not used
+    uint64_t* v_ready = k_ready + NS;    // converted, or cleaned
+    uint64_t* k_empty = v_ready + NS;    // its MMAs are done
+    uint64_t* v_empty = k_empty + NS;
+    uint64_t* raw_full = v_empty + NS;
     uint64_t* raw_empty = raw_full + F::NR;
-    uint64_t* sc_full = raw_empty + F::NR;  // flags and scales of a key tile
+    uint64_t* sc_full = raw_empty + F::NR;  // flags and scales of a chunk
     uint64_t* sc_empty = sc_full + F::NSC;
-    uint64_t* q_full = sc_empty + F::NSC;  // [2]
-    uint64_t* s_full = q_full + 2;
-    uint64_t* p_full = s_full + 2;
-    uint64_t* p_half = p_full + 2;   // keys 0-63 of p_full
-    uint64_t* o_full = p_half + 2;
+    uint64_t* q_full = sc_empty + F::NSC;   // [stage]
+    uint64_t* q_empty = q_full + 2;
+    uint64_t* s_full = q_empty + 2;         // [stage][buffer]
+    uint64_t* p_full = s_full + 4;
+    uint64_t* pv_done = p_full + 4;         // [stage][in turn]
+    uint64_t* o_full = pv_done + 4;
     uint64_t* o_empty = o_full + 2;
     uint64_t* drain = o_empty + 2;
     volatile int* dead = reinterpret_cast<volatile int*>(drain + 1);
     volatile int* odd = dead + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(dead) + 2);
     int* sFlag = const_cast<int*>(dead) + 4;  // [NSC]
-    PlanPos* sPos = reinterpret_cast<PlanPos*>(sFlag + 4);
-    int64_t* sPre = reinterpret_cast<int64_t*>(sRing);
+    PlanPos* sPos = reinterpret_cast<PlanPos*>(sFlag + F::NSC);
+    static_assert((6 * NS + 2 * F::NR + 2 * F::NSC + 21) * 8 + 16 + 4 * F::NSC +
+                          (int)sizeof(PlanPos) <= 1024, "control block");
+    int64_t* sPre = reinterpret_cast<int64_t*>(sK);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < F::NSL; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&ready[i], F::NPREP);
-            mbar_init(&empty[i], 1);
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&v_full[i], 1);
+            mbar_init(&k_ready[i], F::NPREP);
+            mbar_init(&v_ready[i], F::NPREP);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_empty[i], 1);
         }
         for (int i = 0; i < F::NR; ++i) {
             mbar_init(&raw_full[i], 1);
@@ -325,12 +422,15 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             mbar_init(&sc_empty[i], 8 + F::NPREP);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&q_full[i], 4);
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
-            mbar_init(&p_half[i], 4);
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_empty[i], 1);
             mbar_init(&o_full[i], 1);
             mbar_init(&o_empty[i], 4);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&pv_done[i], 1);
         }
         mbar_init(drain, 1);
         *dead = 0;
@@ -358,282 +458,322 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
-    fence_proxy_async_smem();  // the prefix sums are done with: the ring may be filled
+    fence_proxy_async_smem();  // the prefix sums are done with: the rings may be filled
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    PlanPos p = *sPos;
+    // columns: stage i's S buffer b at 128 i + 64 b, its O at 256 + 128 i
+    Walk<F> wk(a, *sPos, total);
 
-    if (warp < 4) {
-        regs_dec<F::kRegsFew>();
-        if (warp == 0) {
-            // -------------------------------------------------------- producer
-            const int box = min(a.b.page_size, KS), boxes = KS / box;
-            constexpr int NBOX = F::kQ8 ? 1 : HD / 64;  // 128-byte columns
-            uint32_t it = 0;
-            for (int left = total; left > 0 && !*dead;) {
-                const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
-                const int m = min(tw.count - p.i, left);
-                for (int j = 0; j < m; ++j, ++it) {
-                    const int key0 = tw.key0(p.i + j);
-                    const int id = lane < boxes ? page_of(a.b, p.s, key0 + lane * box) : -1;
-                    const unsigned on = __ballot_sync(0xffffffffu, id >= 0);
-                    const int y = p.kvh * a.b.page_size + (key0 & (a.b.page_size - 1));
-                    const int ss = it % F::NSC;
-                    if (!ring_wait(&sc_empty[ss], ((it / F::NSC) & 1) ^ 1, dead)) break;
-                    if (lane == 0) {
-                        int flag = 0;  // a bit per 16 positions
-                        for (int b = 0; b < boxes; ++b)
-                            if ((on >> b) & 1) flag |= ((1 << (box / 16)) - 1) << (b * box / 16);
-                        sFlag[ss] = flag;
-                        if constexpr (F::kQ8)
-                            mbar_arrive_expect_tx(&sc_full[ss], __popc(on) * 2 * box * 4);
-                        else mbar_arrive(&sc_full[ss]);
-                    }
-                    __syncwarp();
-                    if constexpr (F::kQ8) {
-                        if (id >= 0) {
-                            const int64_t src = (int64_t)id * a.b.scale_stride + y;
-                            bulk_copy(sScale + (ss * 2 + 0) * KS + lane * box, a.ks + src, box * 4,
-                                      &sc_full[ss]);
-                            bulk_copy(sScale + (ss * 2 + 1) * KS + lane * box, a.vs + src, box * 4,
-                                      &sc_full[ss]);
-                        }
-                    }
-#pragma unroll
-                    for (int kv = 0; kv < 2; ++kv) {
-                        const uint32_t t = 2 * it + kv;
-                        uint64_t* bar;
-                        uint8_t* dst;
-                        if constexpr (F::kQ8) {
-                            const int s = t % F::NR;
-                            if (!ring_wait(&raw_empty[s], ((t / F::NR) & 1) ^ 1, dead)) break;
-                            bar = &raw_full[s];
-                            dst = sRaw + s * F::RAW;
-                            if (lane == 0) mbar_arrive_expect_tx(bar, F::RAW);
-                        } else {
-                            const int s = t % F::NSL;
-                            if (!ring_wait(&empty[s], ((t / F::NSL) & 1) ^ 1, dead)) break;
-                            bar = &full[s];
-                            dst = sRing + s * F::TILE;
-                            if (lane == 0) mbar_arrive_expect_tx(bar, F::TILE);
-                        }
-                        __syncwarp();
-                        const int b = lane / NBOX, col = lane % NBOX;
-                        const int pg = __shfl_sync(0xffffffffu, id, b);
-                        if (b < boxes)  // past the last page: zeros
-                            tma_box(dst + col * F::SUB + b * box * (F::kQ8 ? HD : 128),
-                                    kv ? &tv : &tk, col * 64, y, pg < 0 ? a.b.n_pages : pg, bar);
-                        __syncwarp();
-                    }
-                    if (*dead) break;
-                }
-                left -= m;
-                if (left > 0) P::next_tile(a, p);
-            }
-            if (*dead && lane == 0) {  // let issued copies land before the CTA leaves
-                for (int i = 0; i < F::NSC; ++i) {
-                    mbar_wait(&sc_full[i], 0);
-                    mbar_wait(&sc_full[i], 1);
-                }
-                for (int i = 0; i < (F::kQ8 ? F::NR : F::NSL); ++i) {
-                    uint64_t* b = F::kQ8 ? &raw_full[i] : &full[i];
-                    mbar_wait(b, 0);
-                    mbar_wait(b, 1);
-                }
-            }
-        } else if (warp == 1) {
-            // ------------------------------------------------------------- MMA
-            // The whole warp runs this, one elected lane issues: an MMA of 128
-            // x 128 x 16 takes 64 clocks, and operands in uniform registers are
-            // what lets one be issued in less.
-            constexpr uint32_t fmt = F::kHalf ? 0u : 1u;
-            constexpr uint32_t id_s = idesc_f16(fmt, 128, KS);
-            constexpr uint32_t id_o = idesc_f16(fmt, 128, HD) | (1u << 16);  // B is MN-major
-            const uint32_t lead = elect_lane();
-            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-            const uint64_t dq0 = uniform(smem_desc_k_sw128(sQ));
-            const uint64_t dk0 = uniform(smem_desc_k_sw128(sRing));
-            const uint64_t dv0 = uniform(smem_desc_mn_sw128(sRing, F::SUB));
-            uint32_t it = 0, np[2] = {0, 0}, no[2] = {0, 0};  // no: segments of a stage
-            // slot of operand tile t once it is there, as descriptor offset
-            auto operand = [&](uint32_t t, uint32_t& off) -> bool {
-                const int s = t % F::NSL;
-                // ready of a 16-bit ring only counts V tiles (odd t, even NSL)
-                uint64_t* b = F::kQ8 || (t & 1) ? &ready[s] : &full[s];
-                if (!ring_wait(b, (t / F::NSL) & 1, dead)) return false;
-                tc_fence_after();
-                off = __shfl_sync(0xffffffffu, (uint32_t)s * (F::TILE >> 4), 0);
-                return true;
-            };
-            auto scores = [&](int i, uint32_t koff) {
-                const uint64_t dq = dq0 + i * (F::TILE >> 4), dk = dk0 + koff;
-#pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const int o = (k / 4) * (F::SUB >> 4) + 2 * (k % 4);
-                    umma_ss_lead(tm + i * 128, dq + o, dk + o, id_s, k != 0, lead);
-                }
-                commit_lead(&s_full[i], lead);
-            };
-            for (int left = total; left > 0;) {
-                const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
-                const int m = min(tw.count - p.i, left);
-                const int stages = p.n * a.gqa - p.t * TR > 128 ? 2 : 1;
-                uint32_t koff, voff = 0;
-                bool on = operand(2 * it, koff);
-                for (int i = 0; on && i < stages; ++i) {
-                    on = ring_wait(&q_full[i], no[i] & 1, dead);
-                    if (!on) break;
-                    tc_fence_after();
-                    scores(i, koff);
-                }
-                if (!on) break;
-                commit_lead(&empty[2 * it % F::NSL], lead);
-                for (int j = 0; j < m; ++j) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (i >= stages) break;
-                        on = ring_wait(&p_half[i], np[i] & 1, dead) &&
-                             (i != 0 || operand(2 * (it + j) + 1, voff)) &&
-                             (j != 0 || ring_wait(&o_empty[i], (no[i] & 1) ^ 1, dead));
-                        if (!on) break;
-                        tc_fence_after();
-                        const uint64_t dv = dv0 + voff;
-#pragma unroll
-                        for (int k = 0; k < KS / 32; ++k)
-                            umma_ts_lead(tm + 256 + i * 128, tm + i * 128 + 8 * k, dv + k * 128,
-                                         id_o, j != 0 || k != 0, lead);
-                        on = ring_wait(&p_full[i], np[i]++ & 1, dead);
-                        if (!on) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int k = KS / 32; k < KS / 16; ++k)
-                            umma_ts_lead(tm + 256 + i * 128, tm + i * 128 + 8 * k, dv + k * 128,
-                                         id_o, 1, lead);
-                        if (j + 1 < m) {
-                            on = i != 0 || operand(2 * (it + j + 1), koff);
-                            if (!on) break;
-                            scores(i, koff);
-                        } else {
-                            commit_lead(&o_full[i], lead);
-                            ++no[i];
-                        }
-                    }
-                    if (!on) break;
-                    commit_lead(&empty[(2 * (it + j) + 1) % F::NSL], lead);
-                    if (j + 1 < m) commit_lead(&empty[2 * (it + j + 1) % F::NSL], lead);
-                }
-                if (!on) break;
-                it += m;
-                left -= m;
-                if (left > 0) P::next_tile(a, p);
-            }
-            if (*dead) {  // nothing of this CTA may be in flight when it leaves
-                commit_lead(drain, lead);
-                mbar_wait_warp(drain, 0);
+    if (warp == 0) {
+        // -------------------------------------------------------- producer
+        // K(0), K(1), V(0), K(2), V(1), ...: the order in which the MMAs need them
+        const int box = min(a.b.page_size, KS), boxes = KS / box;
+        constexpr int NBOX = F::kQ8 ? 1 : HD / 64;  // 128-byte columns
+        uint32_t raw = 0;
+        int id = -1, y = 0, id_last = -1, y_last = 0;
+        auto load = [&](bool v, uint32_t u, int ids, int row) -> bool {
+            uint64_t* bar;
+            uint8_t* dst;
+            if constexpr (F::kQ8) {
+                const int s = raw % F::NR;
+                if (!ring_wait(&raw_empty[s], ((raw / F::NR) & 1) ^ 1, dead)) return false;
+                bar = &raw_full[s];
+                dst = sRaw + s * F::RAW;
+                if (lane == 0) mbar_arrive_expect_tx(bar, F::RAW);
+                ++raw;
+            } else {
+                const int s = u % NS;
+                if (!ring_wait(v ? &v_empty[s] : &k_empty[s], ((u / NS) & 1) ^ 1, dead))
+                    return false;
+                bar = v ? &v_full[s] : &k_full[s];
+                dst = (v ? sV : sK) + s * F::TILE;
+                if (lane == 0) mbar_arrive_expect_tx(bar, F::TILE);
             }
             __syncwarp();
-        } else {
-            // --------------------------------------------- operand preparation
-            const int w = warp - 2;
-            constexpr int ROWS = KS / F::NPREP;
-            uint32_t it = 0;
-            for (int left = total; left > 0;) {
-                const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
-                const int m = min(tw.count - p.i, left);
-                for (int j = 0; j < m; ++j, ++it) {
-                    const int ss = it % F::NSC;
-                    ring_wait(&sc_full[ss], (it / F::NSC) & 1, dead);
-                    const int flag = sFlag[ss];
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sc_empty[ss]);
-                    if constexpr (F::kQ8) {
-#pragma unroll
-                        for (int kv = 0; kv < 2; ++kv) {
-                            const uint32_t t = 2 * it + kv;
-                            const int rs = t % F::NR, s = t % F::NSL;
-                            if (!ring_wait(&raw_full[rs], (t / F::NR) & 1, dead)) continue;
-                            if (!ring_wait(&empty[s], ((t / F::NSL) & 1) ^ 1, dead)) continue;
-                            const uint8_t* src = sRaw + rs * F::RAW;
-                            uint8_t* dst = sRing + s * F::TILE;
-                            constexpr int LPR = HD / 16;        // lanes per row
-                            constexpr int RPI = 32 / LPR;       // rows per step
-                            const int c = lane % LPR;           // 16 codes of a row
-                            const bool swap = (c >> 2) & 1;     // other bank half first
-#pragma unroll 4
-                            for (int r = w * ROWS + lane / LPR; r < (w + 1) * ROWS; r += RPI) {
-                                const uint4 u = *reinterpret_cast<const uint4*>(src + r * HD + 16 * c);
-                                const uint32_t x0 = u.x ^ 0x80808080u, x1 = u.y ^ 0x80808080u;
-                                const uint32_t x2 = u.z ^ 0x80808080u, x3 = u.w ^ 0x80808080u;
-                                const uint4 lo = make_uint4(codes2<0x4140>(x0), codes2<0x4342>(x0),
-                                                            codes2<0x4140>(x1), codes2<0x4342>(x1));
-                                const uint4 hi = make_uint4(codes2<0x4140>(x2), codes2<0x4342>(x2),
-                                                            codes2<0x4140>(x3), codes2<0x4342>(x3));
-                                uint8_t* row = dst + (c >> 2) * F::SUB + r * 128;
-                                const int ch = 2 * (c & 3);
-                                *reinterpret_cast<uint4*>(row + (((ch + swap) ^ (r & 7)) << 4)) =
-                                    swap ? hi : lo;
-                                *reinterpret_cast<uint4*>(row + (((ch + !swap) ^ (r & 7)) << 4)) =
-                                    swap ? lo : hi;
-                            }
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                            if (lane == 0) {
-                                mbar_arrive(&ready[s]);
-                                mbar_arrive(&raw_empty[rs]);
-                            }
-                        }
-                    } else {
-                        const uint32_t t = 2 * it + 1;
-                        const int s = t % F::NSL;
-                        if (!ring_wait(&full[s], (t / F::NSL) & 1, dead)) continue;
-                        const int key0 = tw.key0(p.i + j);
-                        const bool whole = flag == 0xFF && key0 + KS - 1 <= tw.p_first &&
-                                           (a.window == 0 || tw.p_last - key0 < a.window ||
-                                            key0 + KS - 1 < a.n_sink);
-                        if (!whole) {
-                            constexpr uint32_t kInf = F::kHalf ? 0x7C007C00u : 0x7F807F80u;
-                            constexpr uint32_t kOne = F::kHalf ? 0x04000400u : 0x00800080u;
-                            uint4* v = reinterpret_cast<uint4*>(sRing + s * F::TILE);
-#pragma unroll 4
-                            for (int q = w * 32 + lane; q < F::TILE / 16; q += 32 * F::NPREP) {
-                                uint4 u = v[q];
-                                uint32_t* x = reinterpret_cast<uint32_t*>(&u);
-                                uint32_t z = 0;
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) z |= (x[i] & kInf) + kOne;
-                                if (z & 0x80008000u) {
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        const uint32_t b = ((x[i] & kInf) + kOne) & 0x80008000u;
-                                        x[i] &= ~((b & 0x8000u ? 0xFFFFu : 0u) |
-                                                  (b & 0x80000000u ? 0xFFFF0000u : 0u));
-                                    }
-                                    v[q] = u;
-                                    *odd = 1;
-                                }
-                            }
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                        }
-                        if (lane == 0) mbar_arrive(&ready[s]);
+            const int b = lane / NBOX, col = lane % NBOX;
+            const int pg = __shfl_sync(0xffffffffu, ids, b);
+            if (b < boxes)  // past the last page: zeros
+                tma_box(dst + col * F::SUB + b * box * (F::kQ8 ? HD : 128), v ? &tv : &tk, col * 64,
+                        row, pg < 0 ? a.b.n_pages : pg, bar);
+            __syncwarp();
+            return true;
+        };
+        for (uint32_t u = 0; u <= (uint32_t)total; ++u) {
+            if (u < (uint32_t)total) {
+                const int key0 = wk.key0();
+                id = lane < boxes ? page_of(a.b, wk.p.s, key0 + lane * box) : -1;
+                y = wk.p.kvh * a.b.page_size + (key0 & (a.b.page_size - 1));
+                const unsigned on = __ballot_sync(0xffffffffu, id >= 0);
+                const int ss = u % F::NSC;
+                if (!ring_wait(&sc_empty[ss], ((u / F::NSC) & 1) ^ 1, dead)) break;
+                if (lane == 0) {
+                    int flag = 0;  // a bit per 16 positions
+                    for (int b = 0; b < boxes; ++b)
+                        if ((on >> b) & 1) flag |= ((1 << (box / 16)) - 1) << (b * box / 16);
+                    sFlag[ss] = flag;
+                    if constexpr (F::kQ8)
+                        mbar_arrive_expect_tx(&sc_full[ss], __popc(on) * 2 * box * 4);
+                    else mbar_arrive(&sc_full[ss]);
+                }
+                __syncwarp();
+                if constexpr (F::kQ8) {
+                    if (id >= 0) {
+                        const int64_t src = (int64_t)id * a.b.scale_stride + y;
+                        bulk_copy(sScale + (ss * 2 + 0) * KS + lane * box, a.ks + src, box * 4,
+                                  &sc_full[ss]);
+                        bulk_copy(sScale + (ss * 2 + 1) * KS + lane * box, a.vs + src, box * 4,
+                                  &sc_full[ss]);
                     }
                 }
-                left -= m;
-                if (left > 0) P::next_tile(a, p);
+            }
+            bool on = true;
+#pragma unroll 1
+            for (int v = 0; on && v < 2; ++v)
+                if (v ? u > 0 : u < (uint32_t)total)
+                    on = load(v != 0, v ? u - 1 : u, v ? id_last : id, v ? y_last : y);
+            if (!on) break;
+            id_last = id;
+            y_last = y;
+            if (u < (uint32_t)total) wk.next(a);
+        }
+        if (*dead && lane == 0) {  // let issued copies land before the CTA leaves
+            for (int par = 0; par < 2; ++par) {
+                for (int i = 0; i < F::NSC; ++i) mbar_wait(&sc_full[i], par);
+                if constexpr (F::kQ8) {
+                    for (int i = 0; i < F::NR; ++i) mbar_wait(&raw_full[i], par);
+                } else {
+                    for (int i = 0; i < NS; ++i) {
+                        mbar_wait(&k_full[i], par);
+                        mbar_wait(&v_full[i], par);
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------- MMA
+        // The whole warp runs this, one elected lane issues.
+        constexpr uint32_t fmt = F::kHalf ? 0u : 1u;
+        constexpr uint32_t id_s = idesc_f16(fmt, 128, KS);
+        constexpr uint32_t id_o = idesc_f16(fmt, 128, HD) | (1u << 16);  // B is MN-major
+        const uint32_t lead = elect_lane();
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t dq0 = uniform(smem_desc_k_sw128(sQ));
+        const uint64_t dk0 = uniform(smem_desc_k_sw128(sK));
+        const uint64_t dv0 = uniform(smem_desc_mn_sw128(sV, F::SUB));
+        // per stage, a byte each: S and PV issued so far, segments whose q is
+        // used and whose O is begun, PVs that answered on pv_done
+        uint32_t ns = 0, np = 0, sq = 0, so = 0, nd = 0;
+        auto count = [](uint32_t x, int i) { return x >> (8 * i); };
+        auto bump = [](uint32_t& x, int i) { x = (x + (1u << (8 * i))) & 0x0F0Fu; };
+        Walk<F> ws = wk;   // of the S that are issued, two chunks ahead of wk
+        uint32_t us = 0;
+        bool on = true;
+        for (int u = -2; on && u < total; ++u) {
+            // A stage's S(u + 2) takes the buffer of its own last P but one:
+            // with both chunks in play on the same stages that is P(u).  A
+            // stage that rests in between has nothing in flight there.
+            const bool pv = u >= 0, sc = us < (uint32_t)total;
+            const int st_v = pv ? wk.stages(a) : 0, st_s = sc ? ws.stages(a) : 0;
+            const uint32_t vs = (uint32_t)u % NS, vph = ((uint32_t)u / NS) & 1;
+            const uint32_t ks = us % NS, kph = (us / NS) & 1;
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+                if (i < st_v) {
+                    const uint32_t n = count(np, i);
+                    on = ring_wait(&p_full[2 * i + (n & 1)], (n >> 1) & 1, dead) &&
+                         (i != 0 || ring_wait(&v_ready[vs], vph, dead));
+                    if (on && wk.first()) {
+                        on = ring_wait(&o_empty[i], (count(so, i) & 1) ^ 1, dead);
+                        bump(so, i);
+                    }
+                    if (!on) break;
+                    tc_fence_after();
+                    const uint32_t off = __shfl_sync(0xffffffffu, vs * (F::TILE >> 4), 0);
+                    const uint32_t col = __shfl_sync(0xffffffffu, i * 128 + (n & 1) * 64, 0);
+                    const uint32_t dcol = __shfl_sync(0xffffffffu, 256 + i * 128, 0);
+                    const uint32_t acc = !wk.first();
+#pragma unroll
+                    for (int k = 0; k < KS / 16; ++k)
+                        umma_ts_lead(tm + dcol, tm + col + 8 * k, dv0 + off + k * 128, id_o,
+                                     k != 0 ? 1u : acc, lead);
+                    if (wk.last()) {
+                        commit_lead(&o_full[i], lead);
+                    } else {
+                        commit_lead(&pv_done[2 * i + (count(nd, i) & 1)], lead);
+                        bump(nd, i);
+                    }
+                    bump(np, i);
+                }
+                if (i < st_s) {
+                    if (i == 0)
+                        on = ring_wait(F::kQ8 ? &k_ready[ks] : &k_full[ks], kph, dead);
+                    if (on && ws.first()) {
+                        on = ring_wait(&q_full[i], count(sq, i) & 1, dead);
+                        bump(sq, i);
+                    }
+                    if (!on) break;
+                    tc_fence_after();
+                    const uint32_t n = count(ns, i);
+                    const uint32_t off = __shfl_sync(0xffffffffu, ks * (F::TILE >> 4), 0);
+                    const uint32_t qoff = __shfl_sync(0xffffffffu, i * (F::QTILE >> 4), 0);
+                    const uint32_t col = __shfl_sync(0xffffffffu, i * 128 + (n & 1) * 64, 0);
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k)
+                        umma_ss_lead(tm + col, dq0 + qoff + (k / 4) * (F::QSUB >> 4) + 2 * (k % 4),
+                                     dk0 + off + (k / 4) * (F::SUB >> 4) + 2 * (k % 4), id_s,
+                                     k != 0, lead);
+                    commit_lead(&s_full[2 * i + (n & 1)], lead);
+                    if (ws.last()) commit_lead(&q_empty[i], lead);
+                    bump(ns, i);
+                }
+            }
+            if (!on) break;
+            if (pv) {
+                commit_lead(&v_empty[vs], lead);
+                wk.next(a);
+            }
+            if (sc) {
+                commit_lead(&k_empty[ks], lead);
+                ws.next(a);
+                ++us;
+            }
+        }
+        if (*dead) {  // nothing of this CTA may be in flight when it leaves
+            commit_lead(drain, lead);
+            mbar_wait_warp(drain, 0);
+        }
+        __syncwarp();
+    } else if (warp < 4) {
+        // ---------------------------------------------------------- q rows
+        const int st = warp - 2;
+        uint32_t seg = 0, n = 0;  // segments, and those with rows here
+        for (int left = total; left > 0; ++seg) {
+            const TileWork<TR, KS> tw(a, wk.p.n, wk.p.len, wk.p.t);
+            const int m = min(tw.count - wk.p.i, left);
+            const int pr0 = wk.p.t * TR + st * 128, rows = wk.p.n * a.gqa;
+            if (pr0 < rows) {
+                if (!ring_wait(&q_empty[st], (n & 1) ^ 1, dead)) break;
+                ++n;
+                load_q<F>(a, wk.p, pr0, rows, sQ + st * F::QTILE, sC + ((seg & 3) * 2 + st) * 128);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[st]);
+            }
+            left -= m;
+            if (left > 0) P::next_tile(a, wk.p);
+        }
+    } else if (warp < 8) {
+        // ----------------------------------------------- operand preparation
+        const int w = warp - 4;
+        if constexpr (F::kQ8) {
+            // raw chunks in the order in which they come
+            auto convert = [&](uint32_t t, uint64_t* empty, uint64_t* ready, uint8_t* ring,
+                               uint32_t u) {
+                const int rs = t % F::NR, s = u % NS;
+                if (!ring_wait(&raw_full[rs], (t / F::NR) & 1, dead)) return;
+                if (!ring_wait(&empty[s], ((u / NS) & 1) ^ 1, dead)) return;
+                const uint8_t* src = sRaw + rs * F::RAW;
+                uint8_t* dst = ring + s * F::TILE;
+                constexpr int LPR = HD / 16;              // lanes per row
+                constexpr int RPI = 32 / LPR;             // rows per step
+                constexpr int STEPS = KS / F::NPREP / RPI;
+                const int c = lane % LPR;                 // 16 codes of a row
+                const bool swap = (c >> 2) & 1;           // other bank half first
+                const int r0 = w * (KS / F::NPREP) + lane / LPR;
+                uint4 x[STEPS];
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i)
+                    x[i] = *reinterpret_cast<const uint4*>(src + (r0 + i * RPI) * HD + 16 * c);
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const int r = r0 + i * RPI;
+                    const uint32_t x0 = x[i].x ^ 0x80808080u, x1 = x[i].y ^ 0x80808080u;
+                    const uint32_t x2 = x[i].z ^ 0x80808080u, x3 = x[i].w ^ 0x80808080u;
+                    const uint4 lo = make_uint4(codes2<0x4140>(x0), codes2<0x4342>(x0),
+                                                codes2<0x4140>(x1), codes2<0x4342>(x1));
+                    const uint4 hi = make_uint4(codes2<0x4140>(x2), codes2<0x4342>(x2),
+                                                codes2<0x4140>(x3), codes2<0x4342>(x3));
+                    uint8_t* row = dst + (c >> 2) * F::SUB + r * 128;
+                    const int ch = 2 * (c & 3);
+                    *reinterpret_cast<uint4*>(row + (((ch + swap) ^ (r & 7)) << 4)) =
+                        swap ? hi : lo;
+                    *reinterpret_cast<uint4*>(row + (((ch + !swap) ^ (r & 7)) << 4)) =
+                        swap ? lo : hi;
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&ready[s]);
+                    mbar_arrive(&raw_empty[rs]);
+                }
+            };
+            uint32_t t = 0;
+            for (uint32_t u = 0; u <= (uint32_t)total; ++u) {
+                if (u < (uint32_t)total) {
+                    const int ss = u % F::NSC;
+                    ring_wait(&sc_full[ss], (u / F::NSC) & 1, dead);
+                    if (lane == 0) mbar_arrive(&sc_empty[ss]);
+                }
+#pragma unroll 1
+                for (int v = 0; v < 2; ++v)
+                    if (v ? u > 0 : u < (uint32_t)total)
+                        convert(t++, v ? v_empty : k_empty, v ? v_ready : k_ready, v ? sV : sK,
+                                u - v);
+            }
+        } else {
+            for (uint32_t u = 0; u < (uint32_t)total; ++u) {
+                const int ss = u % F::NSC, s = u % NS;
+                ring_wait(&sc_full[ss], (u / F::NSC) & 1, dead);
+                const int flag = sFlag[ss];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sc_empty[ss]);
+                const int key0 = wk.key0();
+                const bool whole = flag == 15 && key0 + KS - 1 <= wk.tw.p_first &&
+                                   (a.window == 0 || wk.tw.p_last - key0 < a.window ||
+                                    key0 + KS - 1 < a.n_sink);
+                if (ring_wait(&v_full[s], (u / NS) & 1, dead)) {
+                    if (!whole) {
+                        constexpr uint32_t kInf = F::kHalf ? 0x7C007C00u : 0x7F807F80u;
+                        constexpr uint32_t kOne = F::kHalf ? 0x04000400u : 0x00800080u;
+                        uint4* v = reinterpret_cast<uint4*>(sV + s * F::TILE);
+#pragma unroll 4
+                        for (int q = w * 32 + lane; q < F::TILE / 16; q += 32 * F::NPREP) {
+                            uint4 x4 = v[q];
+                            uint32_t* x = reinterpret_cast<uint32_t*>(&x4);
+                            uint32_t z = 0;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) z |= (x[i] & kInf) + kOne;
+                            if (z & 0x80008000u) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const uint32_t b = ((x[i] & kInf) + kOne) & 0x80008000u;
+                                    x[i] &= ~((b & 0x8000u ? 0xFFFFu : 0u) |
+                                              (b & 0x80000000u ? 0xFFFF0000u : 0u));
+                                }
+                                v[q] = x4;
+                                *odd = 1;
+                            }
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive(&v_ready[s]);
+                }
+                wk.next(a);
             }
         }
     } else {
         // --------------------------------------------------------- softmax
-        regs_inc<F::kRegsMany>();
-        const int st = warp >= 8 ? 1 : 0;
+        const int st = warp >= 12 ? 1 : 0;
         const int r = (warp & 3) * 32 + lane;  // row of the stage, TMEM lane
-        const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + st * 128;
-        const uint32_t tO = tS - st * 128 + 256 + st * 128;
-        uint32_t it = 0, ns = 0, no = 0;
+        const uint32_t tS0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + st * 128;
+        const uint32_t tO = tS0 + 256;
+        uint32_t u = 0, ns = 0, nd = 0, no = 0, seg = 0;
         bool owner = false;
-        for (int left = total; left > 0;) {
+        PlanPos& p = wk.p;
+        for (int left = total; left > 0; ++seg) {
             const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
             const int m = min(tw.count - p.i, left);
             const bool cut_l = p.i > 0, cut_r = p.i + m < tw.count;
@@ -644,51 +784,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             const int tok = live ? pr / a.gqa : 0;
             const int h = p.kvh * a.gqa + pr - tok * a.gqa;
             const int pos = live ? p.len - p.n + tok : -1;
-            const int64_t off = (int64_t)(p.row + tok) * a.out_stride + (int64_t)h * HD;
             float c = a.c;
-
-            // q row into the K-major operand tile
-            if (active) {
-                const X* q = static_cast<const X*>(a.q) + (int64_t)(p.row + tok) * a.q_stride +
-                             (int64_t)h * HD;
-                uint8_t* dst = sQ + st * F::TILE + r * 128;
-                int e = 0;
-                if constexpr (F::kRowScale) {
-                    uint32_t top = 0;
-                    if (live) {
-#pragma unroll
-                        for (int k = 0; k < HD / 8; ++k) {
-                            const uint4 u = reinterpret_cast<const uint4*>(q)[k];
-                            top = max(top, max(max((u.x << 16) & 0x7FFF0000u, u.x & 0x7FFF0000u),
-                                               max((u.y << 16) & 0x7FFF0000u, u.y & 0x7FFF0000u)));
-                            top = max(top, max(max((u.z << 16) & 0x7FFF0000u, u.z & 0x7FFF0000u),
-                                               max((u.w << 16) & 0x7FFF0000u, u.w & 0x7FFF0000u)));
-                        }
-                    }
-                    // the row's largest value lands in [2^14, 2^15)
-                    if (top > 0 && top < 0x7F800000u) e = (int)(top >> 23) - 141;
-                    c = fmaxf(a.c * pow2(e / 2) * pow2(e - e / 2), 1e-38f);
-                }
-                const float fa = pow2(-e / 2), fb = pow2(-e - -e / 2);
-#pragma unroll
-                for (int k = 0; k < HD / 8; ++k) {
-                    uint4 u = live ? reinterpret_cast<const uint4*>(q)[k] : make_uint4(0, 0, 0, 0);
-                    if constexpr (F::kRowScale) {
-                        uint32_t* x = reinterpret_cast<uint32_t*>(&u);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 v = unpack<X>(x[i]);
-                            x[i] = pack<OT>(v.x * fa * fb, v.y * fa * fb);
-                        }
-                    }
-                    *reinterpret_cast<uint4*>(dst + (k / 8) * F::SUB + (((k % 8) ^ (r & 7)) << 4)) =
-                        u;
-                }
-                fence_proxy_async_smem();
-            }
-            __syncwarp();
-            if (active && lane == 0) mbar_arrive(&q_full[st]);
-
             // positions of this warp's rows, for the mask tests
             const int wr = p.t * TR + st * 128 + (warp & 3) * 32;
             const int p_lo = p.len - p.n + min(wr, rows - 1) / a.gqa;
@@ -697,76 +793,73 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             float M = -INFINITY;  // reference maximum (log2)
             int E = F::kQ8 ? -90 : 0;
             uint64_t l2 = 0;      // two partial sums of weights
-            for (int j = 0; j < m; ++j, ++it) {
-                const int ss = it % F::NSC;
-                ring_wait(&sc_full[ss], (it / F::NSC) & 1, dead);
-                if (active && ring_wait(&s_full[st], ns++ & 1, dead)) {
+            for (int j = 0; j < m; ++j, ++u) {
+                const int ss = u % F::NSC;
+                ring_wait(&sc_full[ss], (u / F::NSC) & 1, dead);
+                if (active) {
+                    const int buf = ns & 1;
+                    const bool on = ring_wait(&s_full[2 * st + buf], (ns >> 1) & 1, dead);
+                    ++ns;
+                    if (!on) continue;
+                    const uint32_t tS = tS0 + 64 * buf;
                     tc_fence_after();
+                    // (there are scores, so q and its factors were there; they
+                    // stay for four segments, scores come two chunks early)
+                    if (F::kRowScale && j == 0) c = sC[((seg & 3) * 2 + st) * 128 + r];
                     const int key0 = tw.key0(p.i + j);
                     const int flag = sFlag[ss];
                     const float4* ksc = reinterpret_cast<const float4*>(sScale + ss * 2 * KS);
                     const float4* vsc = ksc + KS / 4;
-                    const bool whole = flag == 0xFF && key0 + KS - 1 <= p_lo &&
+                    const bool whole = flag == 15 && key0 + KS - 1 <= p_lo &&
                                        (a.window == 0 || p_hi - key0 < a.window ||
                                         key0 + KS - 1 < a.n_sink);
-                    // ---- the row's scores and their maximum
-                    uint32_t s[4][32];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x32(tS + 32 * q, s[q]);
-                    tmem_ld_done(s[0]);
-                    tmem_ld_done(s[1]);
-                    tmem_ld_done(s[2]);
-                    tmem_ld_done(s[3]);
-                    if constexpr (F::kQ8) {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
+                    // Both passes are loops over 32 columns, read from tensor
+                    // memory twice: unrolled, with the scores in registers, the
+                    // roles' code no longer fits the SM's instruction cache
+                    // (77 % hits, the next level 74 % busy, twice the time).
+                    // ---- pass 1: the row's maximum; scaled and masked scores go back
+                    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll 1
+                    for (int q = 0; q < KS / 32; ++q) {
+                        uint32_t s[32];
+                        tmem_ld_32x32b_x32(tS + 32 * q, s);
+                        tmem_ld_done(s);
+                        if constexpr (F::kQ8) {
                             float4 k4[8];
 #pragma unroll
                             for (int i = 0; i < 8; ++i) k4[i] = ksc[8 * q + i];
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                scale2(s[q][4 * i], s[q][4 * i + 1], f2(k4[i].x, k4[i].y));
-                                scale2(s[q][4 * i + 2], s[q][4 * i + 3], f2(k4[i].z, k4[i].w));
+                                scale2(s[4 * i], s[4 * i + 1], f2(k4[i].x, k4[i].y));
+                                scale2(s[4 * i + 2], s[4 * i + 3], f2(k4[i].z, k4[i].w));
                             }
                         }
-                    }
-                    uint32_t seen[4];  // of the row, when a mask hides something
-                    if (!whole) {
-                        const int hi = pos - key0 + 1;
-                        const int lo = a.window > 0 ? max(hi - a.window, 0) : 0;
-                        const int sk = a.window > 0 ? a.n_sink - key0 : 0;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            seen[q] = low_bits(hi - 32 * q) &
-                                      (~low_bits(lo - 32 * q) | low_bits(sk - 32 * q)) &
-                                      (((flag >> (2 * q)) & 1 ? 0xFFFFu : 0u) |
-                                       ((flag >> (2 * q)) & 2 ? 0xFFFF0000u : 0u));
+                        if (!whole) {
+                            const uint32_t seen = seen_bits(a, pos, key0, flag, q);
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                if (!((seen[q] >> i) & 1)) s[q][i] = 0xFF800000u;
+                                if (!((seen >> i) & 1)) s[i] = 0xFF800000u;
+                        }
+                        if (F::kQ8 || !whole) tmem_st_x32(tS + 32 * q, s);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            m0 = max3n(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                            m1 = max3n(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
                         }
                     }
-                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2)
-                            m4[q] = max3n(m4[q], __uint_as_float(s[q][i]),
-                                          __uint_as_float(s[q][i + 1]));
-                    const float mx = max3n(max3n(m4[0], m4[1], m4[2]), m4[3], m4[3]) * c;
+                    if (F::kQ8 || !whole) tmem_st_wait();
+                    const float mx = max3n(m0, m1, m1) * c;
                     int Et = E;
                     if constexpr (F::kQ8) {
-                        // V's largest scale in this tile, of positions some row may see
-                        const float4 v4 = vsc[lane];
-                        const int k = key0 + 4 * lane;
-                        const int n = ((flag >> (lane / 4)) & 1) ? tw.p_last - k : -1;
+                        // V's largest scale in this chunk, of positions some row may see
+                        const float2 v2 = reinterpret_cast<const float2*>(vsc)[lane];
+                        const int n = ((flag >> (lane / 8)) & 1) ? tw.p_last - key0 - 2 * lane : -1;
                         auto bits = [&](float v, int at) {
                             const uint32_t b = __float_as_uint(fabsf(v));
                             return at <= n && b < 0x7F800000u ? b : 0u;
                         };
-                        const uint32_t top = __reduce_max_sync(
-                            0xffffffffu, max(max(bits(v4.x, 0), bits(v4.y, 1)),
-                                             max(bits(v4.z, 2), bits(v4.w, 3))));
+                        const uint32_t top =
+                            __reduce_max_sync(0xffffffffu, max(bits(v2.x, 0), bits(v2.y, 1)));
                         Et = max(E, min((int)(top >> 23) - 126, 126));
                     }
                     if (__any_sync(0xffffffffu, mx > M + 8.f || Et > E)) {
@@ -776,7 +869,12 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                         M = N;
                         E = Et;
                         l2 = f2mul(l2, f2(f, f));
-                        if (j > 0) {
+                        // PV of the last chunk (not every PV is waited for; the
+                        // two barriers in turn are at most one phase behind,
+                        // since S of the last chunk came after the PV before it)
+                        const uint32_t g = nd + j - 1;
+                        if (j > 0 && ring_wait(&pv_done[2 * st + (g & 1)], (g >> 1) & 1, dead)) {
+                            tc_fence_after();
 #pragma unroll 1
                             for (int q = 0; q < HD / 32; ++q) {
                                 uint32_t o[32];
@@ -789,62 +887,57 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                             }
                         }
                     }
-                    // ---- weights 2^(z - D), packed over the scores; a visible NaN
-                    // makes all of them NaN
+                    // ---- pass 2: weights 2^(z - D), packed over the scores; a
+                    // visible NaN makes all of them NaN
                     const float D = mx != mx ? mx
                                              : kUp - (M == -INFINITY ? 0.f : M) -
                                                    (float)(F::kQ8 ? E : 0);
                     const uint64_t c2 = f2(c, c), d2 = f2(D, D);
-                    uint64_t lb = 0;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t w[16];
+#pragma unroll 1
+                    for (int q = 0; q < KS / 32; ++q) {
+                        uint32_t s[32], w[16];
+                        tmem_ld_32x32b_x32(tS + 32 * q, s);
                         float4 v4[F::kQ8 ? 8 : 1];
                         if constexpr (F::kQ8) {
 #pragma unroll
                             for (int i = 0; i < 8; ++i) v4[i] = vsc[8 * q + i];
                         }
+                        tmem_ld_done(s);
+                        uint64_t la = 0, lb = 0;
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            const uint64_t z0 = f2fma(f2u(s[q][i], s[q][i + 1]), c2, d2);
-                            const uint64_t z1 = f2fma(f2u(s[q][i + 2], s[q][i + 3]), c2, d2);
-                            float w0 = ex2(f2lo(z0)), w1 = ex2(f2hi(z0)), w2, w3;
-                            // three pairs of eight on the FMA pipe
-                            if (F::kPoly && i % 16 != 4) {
-                                ex2_pair<F::kHalf>(z1, w2, w3);
-                            } else {
-                                w2 = ex2(f2lo(z1));
-                                w3 = ex2(f2hi(z1));
-                            }
-                            l2 = f2add(l2, f2(w0, w1));
+                            const uint64_t z0 = f2fma(f2u(s[i], s[i + 1]), c2, d2);
+                            const uint64_t z1 = f2fma(f2u(s[i + 2], s[i + 3]), c2, d2);
+                            float w0 = ex2(f2lo(z0)), w1 = ex2(f2hi(z0));
+                            float w2 = ex2(f2lo(z1)), w3 = ex2(f2hi(z1));
+                            la = f2add(la, f2(w0, w1));
                             lb = f2add(lb, f2(w2, w3));
                             if constexpr (F::kQ8) {
-                                const float4 v = v4[i / 4];
-                                scale2f(w0, w1, f2(v.x, v.y));
-                                scale2f(w2, w3, f2(v.z, v.w));
-                                if (!whole) {  // a hidden position's scale may be anything
-                                    if (!((seen[q] >> i) & 1)) w0 = 0.f;
-                                    if (!((seen[q] >> (i + 1)) & 1)) w1 = 0.f;
-                                    if (!((seen[q] >> (i + 2)) & 1)) w2 = 0.f;
-                                    if (!((seen[q] >> (i + 3)) & 1)) w3 = 0.f;
-                                }
+                                scale2f(w0, w1, f2(v4[i / 4].x, v4[i / 4].y));
+                                scale2f(w2, w3, f2(v4[i / 4].z, v4[i / 4].w));
                             }
                             w[i / 2] = pack<OT>(w0, w1);
                             w[i / 2 + 1] = pack<OT>(w2, w3);
                         }
-                        tmem_st_x16(tS + 16 * q, w);
-                        if (q & 1) {  // half of the keys: its products may begin
-                            tmem_st_wait();
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(q == 1 ? &p_half[st] : &p_full[st]);
+                        l2 = f2add(l2, f2add(la, lb));
+                        if (F::kQ8 && !whole) {  // a hidden position's scale may be anything
+                            const uint32_t seen = seen_bits(a, pos, key0, flag, q);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                w[i] &= ((seen >> (2 * i)) & 1 ? 0xFFFFu : 0u) |
+                                        ((seen >> (2 * i)) & 2 ? 0xFFFF0000u : 0u);
                         }
+                        tmem_st_x16(tS + 16 * q, w);
                     }
-                    l2 = f2add(l2, lb);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * st + buf]);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sc_empty[ss]);
             }
+            if (active) nd += m - 1;  // the last PV of a segment answers on o_full
 
             // ---- the finished rows, or this piece of them
             if (active && ring_wait(&o_full[st], no++ & 1, dead)) {
@@ -853,34 +946,48 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                 const float l = f2lo(l2) + f2hi(l2);
                 // no finite score seen: zeros, unless it was a NaN
                 const float inv = piece ? 1.f : M == -INFINITY && l == l ? 0.f : 1.f / l;
-                const int64_t pslot = 2 * (int64_t)blockIdx.x + (cut_l ? 0 : 1);
-                float* part = a.part + (pslot * TR + st * 128 + r) * HD;
-                if (piece)
-                    a.stat[pslot * TR + st * 128 + r] =
-                        make_float2(M + (float)(F::kQ8 ? E : 0), l);
-                X* o = static_cast<X*>(a.out) + off;
+                const int64_t row0 =
+                    (2 * (int64_t)blockIdx.x + (cut_l ? 0 : 1)) * TR + st * 128 + (warp & 3) * 32;
+                if (piece) a.stat[row0 + lane] = make_float2(M + (float)(F::kQ8 ? E : 0), l);
+                const unsigned alive = __ballot_sync(0xffffffffu, live);
+                const int64_t off = (int64_t)(p.row + tok) * a.out_stride + (int64_t)h * HD;
+#pragma unroll 1
+                for (int q2 = 0; q2 < HD / 64; ++q2) {
+                    uint32_t y[32];  // 64 dimensions of this row, 16 bits each
+#pragma unroll 1
+                    for (int q = 2 * q2; q < 2 * q2 + 2; ++q) {
+                        uint32_t s[32];
+                        tmem_ld_32x32b_x32(tO + 32 * q, s);
+                        tmem_ld_done(s);
+                        if constexpr (!F::kQ8) {
+                            if (*odd && live) add_odd<F>(a, p, tw, m, pos, 32 * q, s);
+                        }
+                        if (piece) {
+                            turn8(s);
+                            float* o = a.part + (row0 + (lane & ~7)) * HD + 32 * q + 4 * (lane & 7);
 #pragma unroll
-                for (int q = 0; q < HD / 32; ++q) {
-                    uint32_t s[32];
-                    tmem_ld_32x32b_x32(tO + 32 * q, s);
-                    tmem_ld_done(s);
-                    if (!F::kQ8 && *odd && live)
-                        add_odd<F>(a, p, tw, m, pos, 32 * q, s);
-                    if (piece) {
+                            for (int k = 0; k < 8; ++k)
+                                *reinterpret_cast<uint4*>(o + k * HD) =
+                                    make_uint4(s[4 * k], s[4 * k + 1], s[4 * k + 2], s[4 * k + 3]);
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<uint4*>(part + 32 * q + i) =
-                                make_uint4(s[i], s[i + 1], s[i + 2], s[i + 3]);
-                    } else if (live) {
+                            for (int k = 0; k < 16; ++k) {
+                                y[k] = y[16 + k];
+                                y[16 + k] = pack<X>(__uint_as_float(s[2 * k]) * inv,
+                                                    __uint_as_float(s[2 * k + 1]) * inv);
+                            }
+                        }
+                    }
+                    if (!piece) {
+                        turn8(y);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            uint32_t y[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                y[k] = pack<X>(__uint_as_float(s[i + 2 * k]) * inv,
-                                               __uint_as_float(s[i + 2 * k + 1]) * inv);
-                            *reinterpret_cast<uint4*>(o + 32 * q + i) =
-                                make_uint4(y[0], y[1], y[2], y[3]);
+                        for (int k = 0; k < 8; ++k) {
+                            const int from = (lane & ~7) + k;
+                            const int64_t at = __shfl_sync(0xffffffffu, off, from);
+                            X* o = static_cast<X*>(a.out) + at + 64 * q2 + 8 * (lane & 7);
+                            if ((alive >> from) & 1)
+                                *reinterpret_cast<uint4*>(o) =
+                                    make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
                         }
                     }
                 }
@@ -890,7 +997,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             }
             if (cut_r && !cut_l) {
                 owner = true;
-                if (threadIdx.x == 128) {
+                if (threadIdx.x == 256) {
                     const int64_t end = u0 + (total - left) + tw.count;
                     CutTile ct;
                     ct.pieces = (int)((end - 1) / L - blockIdx.x) + 1;
@@ -904,7 +1011,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             left -= m;
             if (left > 0) P::next_tile(a, p);
         }
-        if (!owner && threadIdx.x == 128) a.cut[blockIdx.x].pieces = 0;
+        if (!owner && threadIdx.x == 256) a.cut[blockIdx.x].pieces = 0;
     }
 
     tc_fence_before();
@@ -935,7 +1042,7 @@ int launch_tc(const PagedJob& j) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tk, tv, j.a, 2);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tk, tv, j.a, 4);
     if (e != cudaSuccess) return cuda_error(e, "launch paged_tc");
     return FTC_OK;
 }
