@@ -1,35 +1,40 @@
 // attention_pages_tc.cuh -- the paged attention of long chunks with 16-bit
 // queries on the tcgen05 tensor cores.
 //
-// A tile is 256 packed rows, two stages of 128; its keys come 64 at a time.
-// Per stage and key chunk, S = Q K^T (128 x 64) and O += P V (128 x head_dim)
-// accumulate in tensor memory: two S buffers of 64 columns, the weights P
-// written over their S as 16-bit A operand, O head_dim columns.  One warp
-// issues all MMAs, per chunk u and stage
-//   PV(u), then S(u + 2) into the buffer that P(u) has left,
-// so a stage's next scores are there before its weights are done and the
-// softmax warps never wait for the tensor cores: an MMA takes its 64 clocks,
-// but a batch of 8 comes back only ~500 clocks after its last issue, and with
-// one S buffer of 128 keys that latency stood in every step (5000 clocks per
-// 128 keys, 2048 of them MMAs).  MMAs of one warp run in order, which makes
-// S(u + 2) after PV(u) safe on the same columns.
-// Rescaling O is lazy: the reference maximum only moves when a score passes it
-// by 2^8, which f16 weights leave room for (they sit 2^7 up); then the softmax
-// warp waits for PV(u - 1) and multiplies O in tensor memory itself.
+// A tile is 256 packed rows, two stages of 128; its keys come 128 at a time.
+// Per stage and key chunk, S = Q K^T (128 x 128) and O += P V (128 x head_dim)
+// accumulate in tensor memory: S 128 columns, the weights P written over it as
+// 16-bit A operand, O head_dim columns.  One warp issues all MMAs, per chunk u
+// and stage PV(u), then S(u + 1): the tensor cores work on one stage while the
+// other's softmax runs, and PV(u) begins when half of its weights are there.
+// MMAs of one warp run in order, which makes S(u + 1) after PV(u) safe on the
+// same columns, and lets the softmax warps rescale O without a barrier of its
+// own: S(u) has arrived, so PV(u - 1) is done, and PV(u) waits for this P.
+// Rescaling is lazy: the reference maximum only moves when a score passes it by
+// 2^8, which f16 weights leave room for (they sit 2^7 up).
 //
 // Warps: 0 brings K and V by TMA, one box per page (V as it lies in the cache:
-// positions by head_dim, the MN-major B operand of PV); 1 issues MMAs; 2 and 3
-// fetch a stage's q rows of the next tile as soon as this tile's last scores
-// are issued; 8-11 and 12-15 are the softmax of the two stages, a thread per
-// row; 4-7 turn 8-bit codes into f16 tiles, and in chunks where some row's mask
-// hides something they take V elements that are not finite out (0 x inf would
-// reach every row), which the rows that see them get back at the end.  8-bit
-// scales stay in fp32: K's multiplies S, V's multiplies P, relative to its
-// running maximum 2^E.
+// positions by head_dim, the MN-major B operand of PV); 1 issues MMAs; 4-7 and
+// 8-11 are the softmax of the two stages, a thread per row, its 128 scores in
+// registers (these warps get 216, the others 72); 2 and 3 turn 8-bit codes
+// into f16 tiles, and in chunks where some row's mask hides something they take
+// V elements that are not finite out (0 x inf would reach every row), which the
+// rows that see them get back at the end; between tiles each fetches the q rows
+// of a stage.  8-bit scales stay in fp32: K's multiplies S, V's multiplies P,
+// relative to its running maximum 2^E.
 //
-// What bounds it: per 128 keys and stage pair the tensor cores need 2048
-// clocks at head_dim 128 (2560 with the narrow S, whose operands are what
-// shared memory can feed), and the exponentials, 16 a clock, 2048.
+// What bounds it: per chunk and stage pair the tensor cores need 2048 clocks
+// at head_dim 128 and the exponentials, 16 a clock, as many; a chunk takes 2.4
+// times that (2048 bf16 rows of 32 heads on 16384 positions: 514 us, 1.0
+// PFLOP/s).  A stage's softmax (~2100 clocks) and its MMAs (a batch of 8 comes
+// back ~500 clocks after its last issue) stand one after the other, two stages
+// are what tensor memory holds, and the roles' code passes the SM's
+// instruction cache.  Tried and not kept, with the time of the same call: two S
+// buffers of 64 keys, scores a chunk early (820 us: what is done once per chunk
+// weighs double); 16 warps, q fetched by two of their own (668 us); a part of
+// the exponentials as polynomials on the FMA pipe (720 us: no one waits for the
+// exponential unit); stage loops rolled (634 us); a shuffled, coalesced
+// epilogue (552 us).
 #pragma once
 
 #include <climits>
@@ -43,32 +48,32 @@ template <typename X_, typename C_, int HD_>
 struct TcCfg {
     using X = X_;
     using C = C_;
-    static constexpr int HD = HD_, TR = 256, KS = 64;
+    static constexpr int HD = HD_, TR = 256, KS = 128;
     static constexpr bool kQ8 = sizeof(C) == 1;
     using OT = typename std::conditional<std::is_same<C, __nv_bfloat16>::value, __nv_bfloat16,
                                          __half>::type;
     static constexpr bool kHalf = std::is_same<OT, __half>::value;
     static constexpr bool kRowScale = kHalf && !std::is_same<X, __half>::value;
-    static constexpr int SUB = KS * 128;           // 64 dimensions of a chunk's rows
-    static constexpr int TILE = SUB * (HD / 64);   // K or V chunk, 16-bit
-    static constexpr int QSUB = 128 * 128;         // 64 dimensions of a stage's rows
-    static constexpr int QTILE = QSUB * (HD / 64);
-    static constexpr int NS = kQ8 && HD == 128 ? 3 : 4;  // slots of the K and of the V ring
+    static constexpr int SUB = KS * 128;           // 64 dimensions of 128 rows
+    static constexpr int TILE = SUB * (HD / 64);   // K or V chunk or a stage's q, 16-bit
+    // operand ring, K and V chunks in turn (16-bit: an even number of slots)
+    static constexpr int NS = kQ8 ? (HD == 128 ? 3 : 4) : (HD == 128 ? 4 : 6);
     static constexpr int RAW = kQ8 ? KS * HD : 0;
-    static constexpr int NR = 4;                   // raw slots, K and V as they come
-    static constexpr int NSC = 4;
-    static constexpr int NPREP = 4;
-    static constexpr int OFF_K = 0;
-    static constexpr int OFF_V = OFF_K + NS * TILE;
-    static constexpr int OFF_Q = OFF_V + NS * TILE;
-    static constexpr int OFF_RAW = OFF_Q + 2 * QTILE;
+    static constexpr int NR = 3;                   // slots of raw codes
+    static constexpr int NSC = 3;
+    static constexpr int NPREP = 2;
+    static constexpr int OFF_RING = 0;
+    static constexpr int OFF_Q = OFF_RING + NS * TILE;
+    static constexpr int OFF_RAW = OFF_Q + 2 * TILE;
     static constexpr int OFF_SC = OFF_RAW + (kQ8 ? NR * RAW : 0);
     static constexpr int OFF_C = OFF_SC + NSC * (kQ8 ? 2 * KS * 4 : 0);
     static constexpr int OFF_BAR = OFF_C + (kRowScale ? 4 * TR * 4 : 0);
     static constexpr int SMEM = OFF_BAR + 1024 + 1024;
-    static constexpr int THREADS = 512;
+    static constexpr int THREADS = 384;
+    // registers a thread: 384 x 168 at launch, then 128 x 72 + 256 x 216
+    static constexpr int kRegsFew = 72, kRegsMany = 216;
     static_assert(SMEM <= 227 * 1024, "shared memory");
-    static_assert(2 * NS * TILE >= Plan<TR, KS>::kSmem, "the plan's prefix sums fit in the rings");
+    static_assert(NS * TILE >= Plan<TR, KS>::kSmem, "the plan's prefix sums fit in the ring");
 };
 
 __device__ __forceinline__ uint64_t f2(float a, float b) {
@@ -119,14 +124,14 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
     return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
 }
 
-// The positions of 32 from key0 + 32 q that a row at `pos` sees, as bits.
-__device__ __forceinline__ uint32_t seen_bits(const PagedArgs& a, int pos, int key0, int flag,
-                                              int q) {
-    const int hi = pos - key0 + 1 - 32 * q;
-    const uint32_t near = a.window > 0 ? ~low_bits(hi - a.window) | low_bits(a.n_sink - key0 - 32 * q)
+// The 32 positions from key0 on that a row at `pos` sees, as bits; `mapped`:
+// a bit per 16 of them.
+__device__ __forceinline__ uint32_t seen_bits(const PagedArgs& a, int pos, int key0, int mapped) {
+    const int hi = pos - key0 + 1;
+    const uint32_t near = a.window > 0 ? ~low_bits(hi - a.window) | low_bits(a.n_sink - key0)
                                        : 0xFFFFFFFFu;
     return low_bits(hi) & near &
-           (((flag >> (2 * q)) & 1 ? 0xFFFFu : 0u) | ((flag >> (2 * q)) & 2 ? 0xFFFF0000u : 0u));
+           ((mapped & 1 ? 0xFFFFu : 0u) | (mapped & 2 ? 0xFFFF0000u : 0u));
 }
 
 // Loads done: ties the registers to the wait, so that no use moves above it.
@@ -191,35 +196,14 @@ __device__ __forceinline__ uint32_t elect_lane() {
     return e;
 }
 
+// A value every lane holds, as the compiler can know it.
 __device__ __forceinline__ uint64_t uniform(uint64_t v) {
     const uint32_t lo = __shfl_sync(0xffffffffu, (uint32_t)v, 0);
     const uint32_t hi = __shfl_sync(0xffffffffu, (uint32_t)(v >> 32), 0);
     return (uint64_t)lo | ((uint64_t)hi << 32);
 }
 
-// The MMAs and the commit of sm100.cuh, by the lane whose `lead` is 1.
-__device__ __forceinline__ void umma_ss_lead(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                             uint32_t acc, uint32_t lead) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
-        : "memory");
-}
-
-__device__ __forceinline__ void umma_ts_lead(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                             uint32_t acc, uint32_t lead) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
-        : "memory");
-}
-
+// The commit of sm100.cuh by the lane whose `lead` is 1.
 __device__ __forceinline__ void commit_lead(uint64_t* bar, uint32_t lead) {
     asm volatile(
         "{\n\t.reg .pred q;\n\t"
@@ -256,30 +240,6 @@ __device__ __noinline__ void add_odd(const PagedArgs& a, const PlanPos& p,
     }
 }
 
-// 32 words a lane as 8 chunks of 4: lane i of each 8 comes to hold chunk i of
-// the 8 lanes' rows (word 4 k + j: row k), so that 8 lanes store 128
-// neighbouring bytes (a thread storing its own row touches 32 lines an
-// instruction).
-__device__ __forceinline__ void turn8(uint32_t (&v)[32]) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int b = 1; b < 8; b <<= 1) {
-        const bool up = lane & b;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            if (c & b) continue;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t& lo = v[4 * c + j];
-                uint32_t& hi = v[4 * (c | b) + j];
-                const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, b);
-                if (up) lo = got;
-                else hi = got;
-            }
-        }
-    }
-}
-
 // One stage's q rows into the K-major operand tile by a warp, all of them in
 // flight at once; where they become f16, a power of two per row brings the
 // largest value to [2^14, 2^15) and goes to the score factor.
@@ -292,7 +252,7 @@ __device__ __forceinline__ void load_q(const PagedArgs& a, const PlanPos& p, int
     constexpr int RPI = 32 / LPR;    // rows a step
     const int lane = threadIdx.x & 31, c = lane % LPR;
     auto at = [&](int r) {
-        return tile + (c / 8) * F::QSUB + r * 128 + (((c % 8) ^ (r & 7)) << 4);
+        return tile + (c / 8) * F::SUB + r * 128 + (((c % 8) ^ (r & 7)) << 4);
     };
 #pragma unroll 2
     for (int r = lane / LPR; r < 128; r += RPI) {
@@ -332,6 +292,15 @@ __device__ __forceinline__ void load_q(const PagedArgs& a, const PlanPos& p, int
     }
 }
 
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // The chunks of a CTA's share, one after another.
 template <class F>
 struct Walk {
@@ -344,11 +313,7 @@ struct Walk {
         m = min(tw.count - p.i, left);
     }
     __device__ __forceinline__ int key0() const { return tw.key0(p.i + j); }
-    __device__ __forceinline__ int stages(const PagedArgs& a) const {
-        return p.n * a.gqa - p.t * F::TR > 128 ? 2 : 1;
-    }
     __device__ __forceinline__ bool first() const { return j == 0; }
-    __device__ __forceinline__ bool last() const { return j + 1 == m; }
     __device__ __forceinline__ void next(const PagedArgs& a) {
         --left;
         if (++j < m || left == 0) return;
@@ -370,28 +335,24 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sK = smem + F::OFF_K;
-    uint8_t* sV = smem + F::OFF_V;
+    uint8_t* sRing = smem + F::OFF_RING;
     uint8_t* sQ = smem + F::OFF_Q;
     uint8_t* sRaw = smem + F::OFF_RAW;
     float* sScale = reinterpret_cast<float*>(smem + F::OFF_SC);  // [NSC][K, V][KS]
     float* sC = reinterpret_cast<float*>(smem + F::OFF_C);       // [4][2][128] score factors
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + F::OFF_BAR);  // 16-bit chunks landed
-    uint64_t* v_full = k_full + NS;
-    uint64_t* k_ready = v_full + NS;     // converted; 16-bit: not used
-    uint64_t* v_ready = k_ready + NS;    // converted, or cleaned
-    uint64_t* k_empty = v_ready + NS;    // its MMAs are done
-    uint64_t* v_empty = k_empty + NS;
-    uint64_t* raw_full = v_empty + NS;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + F::OFF_BAR);  // 16-bit chunk landed
+    uint64_t* ready = full + NS;            // converted; 16-bit: V looked over
+    uint64_t* empty = ready + NS;           // its MMAs are done
+    uint64_t* raw_full = empty + NS;
     uint64_t* raw_empty = raw_full + F::NR;
     uint64_t* sc_full = raw_empty + F::NR;  // flags and scales of a chunk
     uint64_t* sc_empty = sc_full + F::NSC;
-    uint64_t* q_full = sc_empty + F::NSC;   // [stage]
+    uint64_t* q_full = sc_empty + F::NSC;   // [stage] from here on
     uint64_t* q_empty = q_full + 2;
-    uint64_t* s_full = q_empty + 2;         // [stage][buffer]
-    uint64_t* p_full = s_full + 4;
-    uint64_t* pv_done = p_full + 4;         // [stage][in turn]
-    uint64_t* o_full = pv_done + 4;
+    uint64_t* s_full = q_empty + 2;
+    uint64_t* p_half = s_full + 2;          // weights of keys 0-63
+    uint64_t* p_full = p_half + 2;
+    uint64_t* o_full = p_full + 2;
     uint64_t* o_empty = o_full + 2;
     uint64_t* drain = o_empty + 2;
     volatile int* dead = reinterpret_cast<volatile int*>(drain + 1);
@@ -399,19 +360,16 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(dead) + 2);
     int* sFlag = const_cast<int*>(dead) + 4;  // [NSC]
     PlanPos* sPos = reinterpret_cast<PlanPos*>(sFlag + F::NSC);
-    static_assert((6 * NS + 2 * F::NR + 2 * F::NSC + 21) * 8 + 16 + 4 * F::NSC +
+    static_assert((3 * NS + 2 * F::NR + 2 * F::NSC + 15) * 8 + 16 + 4 * F::NSC +
                           (int)sizeof(PlanPos) <= 1024, "control block");
-    int64_t* sPre = reinterpret_cast<int64_t*>(sK);
+    int64_t* sPre = reinterpret_cast<int64_t*>(sRing);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) {
-            mbar_init(&k_full[i], 1);
-            mbar_init(&v_full[i], 1);
-            mbar_init(&k_ready[i], F::NPREP);
-            mbar_init(&v_ready[i], F::NPREP);
-            mbar_init(&k_empty[i], 1);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&full[i], 1);
+            mbar_init(&ready[i], F::NPREP);
+            mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < F::NR; ++i) {
             mbar_init(&raw_full[i], 1);
@@ -424,13 +382,11 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 1);
             mbar_init(&q_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_half[i], 4);
+            mbar_init(&p_full[i], 4);
             mbar_init(&o_full[i], 1);
             mbar_init(&o_empty[i], 4);
-        }
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
-            mbar_init(&pv_done[i], 1);
         }
         mbar_init(drain, 1);
         *dead = 0;
@@ -458,63 +414,35 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
-    fence_proxy_async_smem();  // the prefix sums are done with: the rings may be filled
+    fence_proxy_async_smem();  // the prefix sums are done with: the ring may be filled
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    // columns: stage i's S buffer b at 128 i + 64 b, its O at 256 + 128 i
-    Walk<F> wk(a, *sPos, total);
+    // columns: stage i's S (and P over it) at 128 i, its O at 256 + 128 i
 
-    if (warp == 0) {
-        // -------------------------------------------------------- producer
-        // K(0), K(1), V(0), K(2), V(1), ...: the order in which the MMAs need them
-        const int box = min(a.b.page_size, KS), boxes = KS / box;
-        constexpr int NBOX = F::kQ8 ? 1 : HD / 64;  // 128-byte columns
-        uint32_t raw = 0;
-        int id = -1, y = 0, id_last = -1, y_last = 0;
-        auto load = [&](bool v, uint32_t u, int ids, int row) -> bool {
-            uint64_t* bar;
-            uint8_t* dst;
-            if constexpr (F::kQ8) {
-                const int s = raw % F::NR;
-                if (!ring_wait(&raw_empty[s], ((raw / F::NR) & 1) ^ 1, dead)) return false;
-                bar = &raw_full[s];
-                dst = sRaw + s * F::RAW;
-                if (lane == 0) mbar_arrive_expect_tx(bar, F::RAW);
-                ++raw;
-            } else {
-                const int s = u % NS;
-                if (!ring_wait(v ? &v_empty[s] : &k_empty[s], ((u / NS) & 1) ^ 1, dead))
-                    return false;
-                bar = v ? &v_full[s] : &k_full[s];
-                dst = (v ? sV : sK) + s * F::TILE;
-                if (lane == 0) mbar_arrive_expect_tx(bar, F::TILE);
-            }
-            __syncwarp();
-            const int b = lane / NBOX, col = lane % NBOX;
-            const int pg = __shfl_sync(0xffffffffu, ids, b);
-            if (b < boxes)  // past the last page: zeros
-                tma_box(dst + col * F::SUB + b * box * (F::kQ8 ? HD : 128), v ? &tv : &tk, col * 64,
-                        row, pg < 0 ? a.b.n_pages : pg, bar);
-            __syncwarp();
-            return true;
-        };
-        for (uint32_t u = 0; u <= (uint32_t)total; ++u) {
-            if (u < (uint32_t)total) {
+    if (warp < 4) {
+        regs_dec<F::kRegsFew>();
+        Walk<F> wk(a, *sPos, total);
+        if (warp == 0) {
+            // ---------------------------------------------------- producer
+            const int box = min(a.b.page_size, KS), boxes = KS / box;
+            constexpr int NBOX = F::kQ8 ? 1 : HD / 64;  // 128-byte columns
+            bool on = true;
+            for (uint32_t u = 0; on && u < (uint32_t)total; ++u) {
                 const int key0 = wk.key0();
-                id = lane < boxes ? page_of(a.b, wk.p.s, key0 + lane * box) : -1;
-                y = wk.p.kvh * a.b.page_size + (key0 & (a.b.page_size - 1));
-                const unsigned on = __ballot_sync(0xffffffffu, id >= 0);
+                const int id = lane < boxes ? page_of(a.b, wk.p.s, key0 + lane * box) : -1;
+                const int y = wk.p.kvh * a.b.page_size + (key0 & (a.b.page_size - 1));
+                const unsigned mapped = __ballot_sync(0xffffffffu, id >= 0);
                 const int ss = u % F::NSC;
                 if (!ring_wait(&sc_empty[ss], ((u / F::NSC) & 1) ^ 1, dead)) break;
                 if (lane == 0) {
                     int flag = 0;  // a bit per 16 positions
                     for (int b = 0; b < boxes; ++b)
-                        if ((on >> b) & 1) flag |= ((1 << (box / 16)) - 1) << (b * box / 16);
+                        if ((mapped >> b) & 1) flag |= ((1 << (box / 16)) - 1) << (b * box / 16);
                     sFlag[ss] = flag;
                     if constexpr (F::kQ8)
-                        mbar_arrive_expect_tx(&sc_full[ss], __popc(on) * 2 * box * 4);
+                        mbar_arrive_expect_tx(&sc_full[ss], __popc(mapped) * 2 * box * 4);
                     else mbar_arrive(&sc_full[ss]);
                 }
                 __syncwarp();
@@ -527,252 +455,257 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                                   &sc_full[ss]);
                     }
                 }
-            }
-            bool on = true;
 #pragma unroll 1
-            for (int v = 0; on && v < 2; ++v)
-                if (v ? u > 0 : u < (uint32_t)total)
-                    on = load(v != 0, v ? u - 1 : u, v ? id_last : id, v ? y_last : y);
-            if (!on) break;
-            id_last = id;
-            y_last = y;
-            if (u < (uint32_t)total) wk.next(a);
-        }
-        if (*dead && lane == 0) {  // let issued copies land before the CTA leaves
-            for (int par = 0; par < 2; ++par) {
-                for (int i = 0; i < F::NSC; ++i) mbar_wait(&sc_full[i], par);
-                if constexpr (F::kQ8) {
-                    for (int i = 0; i < F::NR; ++i) mbar_wait(&raw_full[i], par);
-                } else {
-                    for (int i = 0; i < NS; ++i) {
-                        mbar_wait(&k_full[i], par);
-                        mbar_wait(&v_full[i], par);
-                    }
-                }
-            }
-        }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------- MMA
-        // The whole warp runs this, one elected lane issues.
-        constexpr uint32_t fmt = F::kHalf ? 0u : 1u;
-        constexpr uint32_t id_s = idesc_f16(fmt, 128, KS);
-        constexpr uint32_t id_o = idesc_f16(fmt, 128, HD) | (1u << 16);  // B is MN-major
-        const uint32_t lead = elect_lane();
-        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        const uint64_t dq0 = uniform(smem_desc_k_sw128(sQ));
-        const uint64_t dk0 = uniform(smem_desc_k_sw128(sK));
-        const uint64_t dv0 = uniform(smem_desc_mn_sw128(sV, F::SUB));
-        // per stage, a byte each: S and PV issued so far, segments whose q is
-        // used and whose O is begun, PVs that answered on pv_done
-        uint32_t ns = 0, np = 0, sq = 0, so = 0, nd = 0;
-        auto count = [](uint32_t x, int i) { return x >> (8 * i); };
-        auto bump = [](uint32_t& x, int i) { x = (x + (1u << (8 * i))) & 0x0F0Fu; };
-        Walk<F> ws = wk;   // of the S that are issued, two chunks ahead of wk
-        uint32_t us = 0;
-        bool on = true;
-        for (int u = -2; on && u < total; ++u) {
-            // A stage's S(u + 2) takes the buffer of its own last P but one:
-            // with both chunks in play on the same stages that is P(u).  A
-            // stage that rests in between has nothing in flight there.
-            const bool pv = u >= 0, sc = us < (uint32_t)total;
-            const int st_v = pv ? wk.stages(a) : 0, st_s = sc ? ws.stages(a) : 0;
-            const uint32_t vs = (uint32_t)u % NS, vph = ((uint32_t)u / NS) & 1;
-            const uint32_t ks = us % NS, kph = (us / NS) & 1;
-#pragma unroll 1
-            for (int i = 0; i < 2; ++i) {
-                if (i < st_v) {
-                    const uint32_t n = count(np, i);
-                    on = ring_wait(&p_full[2 * i + (n & 1)], (n >> 1) & 1, dead) &&
-                         (i != 0 || ring_wait(&v_ready[vs], vph, dead));
-                    if (on && wk.first()) {
-                        on = ring_wait(&o_empty[i], (count(so, i) & 1) ^ 1, dead);
-                        bump(so, i);
-                    }
+                for (int v = 0; on && v < 2; ++v) {
+                    const uint32_t t = 2 * u + v;
+                    constexpr int N = F::kQ8 ? F::NR : NS;
+                    constexpr int BYTES = F::kQ8 ? F::RAW : F::TILE;
+                    const int s = t % N;
+                    uint64_t* bar = F::kQ8 ? &raw_full[s] : &full[s];
+                    on = ring_wait(F::kQ8 ? &raw_empty[s] : &empty[s], ((t / N) & 1) ^ 1, dead);
                     if (!on) break;
-                    tc_fence_after();
-                    const uint32_t off = __shfl_sync(0xffffffffu, vs * (F::TILE >> 4), 0);
-                    const uint32_t col = __shfl_sync(0xffffffffu, i * 128 + (n & 1) * 64, 0);
-                    const uint32_t dcol = __shfl_sync(0xffffffffu, 256 + i * 128, 0);
-                    const uint32_t acc = !wk.first();
-#pragma unroll
-                    for (int k = 0; k < KS / 16; ++k)
-                        umma_ts_lead(tm + dcol, tm + col + 8 * k, dv0 + off + k * 128, id_o,
-                                     k != 0 ? 1u : acc, lead);
-                    if (wk.last()) {
-                        commit_lead(&o_full[i], lead);
-                    } else {
-                        commit_lead(&pv_done[2 * i + (count(nd, i) & 1)], lead);
-                        bump(nd, i);
-                    }
-                    bump(np, i);
+                    if (lane == 0) mbar_arrive_expect_tx(bar, BYTES);
+                    __syncwarp();
+                    const int b = lane / NBOX, col = lane % NBOX;
+                    const int pg = __shfl_sync(0xffffffffu, id, b);
+                    if (b < boxes)  // past the last page: zeros
+                        tma_box((F::kQ8 ? sRaw : sRing) + s * BYTES + col * F::SUB +
+                                    b * box * (F::kQ8 ? HD : 128),
+                                v ? &tv : &tk, col * 64, y, pg < 0 ? a.b.n_pages : pg, bar);
+                    __syncwarp();
                 }
-                if (i < st_s) {
-                    if (i == 0)
-                        on = ring_wait(F::kQ8 ? &k_ready[ks] : &k_full[ks], kph, dead);
-                    if (on && ws.first()) {
-                        on = ring_wait(&q_full[i], count(sq, i) & 1, dead);
-                        bump(sq, i);
-                    }
-                    if (!on) break;
-                    tc_fence_after();
-                    const uint32_t n = count(ns, i);
-                    const uint32_t off = __shfl_sync(0xffffffffu, ks * (F::TILE >> 4), 0);
-                    const uint32_t qoff = __shfl_sync(0xffffffffu, i * (F::QTILE >> 4), 0);
-                    const uint32_t col = __shfl_sync(0xffffffffu, i * 128 + (n & 1) * 64, 0);
-#pragma unroll
-                    for (int k = 0; k < HD / 16; ++k)
-                        umma_ss_lead(tm + col, dq0 + qoff + (k / 4) * (F::QSUB >> 4) + 2 * (k % 4),
-                                     dk0 + off + (k / 4) * (F::SUB >> 4) + 2 * (k % 4), id_s,
-                                     k != 0, lead);
-                    commit_lead(&s_full[2 * i + (n & 1)], lead);
-                    if (ws.last()) commit_lead(&q_empty[i], lead);
-                    bump(ns, i);
-                }
-            }
-            if (!on) break;
-            if (pv) {
-                commit_lead(&v_empty[vs], lead);
                 wk.next(a);
             }
-            if (sc) {
-                commit_lead(&k_empty[ks], lead);
-                ws.next(a);
-                ++us;
-            }
-        }
-        if (*dead) {  // nothing of this CTA may be in flight when it leaves
-            commit_lead(drain, lead);
-            mbar_wait_warp(drain, 0);
-        }
-        __syncwarp();
-    } else if (warp < 4) {
-        // ---------------------------------------------------------- q rows
-        const int st = warp - 2;
-        uint32_t seg = 0, n = 0;  // segments, and those with rows here
-        for (int left = total; left > 0; ++seg) {
-            const TileWork<TR, KS> tw(a, wk.p.n, wk.p.len, wk.p.t);
-            const int m = min(tw.count - wk.p.i, left);
-            const int pr0 = wk.p.t * TR + st * 128, rows = wk.p.n * a.gqa;
-            if (pr0 < rows) {
-                if (!ring_wait(&q_empty[st], (n & 1) ^ 1, dead)) break;
-                ++n;
-                load_q<F>(a, wk.p, pr0, rows, sQ + st * F::QTILE, sC + ((seg & 3) * 2 + st) * 128);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[st]);
-            }
-            left -= m;
-            if (left > 0) P::next_tile(a, wk.p);
-        }
-    } else if (warp < 8) {
-        // ----------------------------------------------- operand preparation
-        const int w = warp - 4;
-        if constexpr (F::kQ8) {
-            // raw chunks in the order in which they come
-            auto convert = [&](uint32_t t, uint64_t* empty, uint64_t* ready, uint8_t* ring,
-                               uint32_t u) {
-                const int rs = t % F::NR, s = u % NS;
-                if (!ring_wait(&raw_full[rs], (t / F::NR) & 1, dead)) return;
-                if (!ring_wait(&empty[s], ((u / NS) & 1) ^ 1, dead)) return;
-                const uint8_t* src = sRaw + rs * F::RAW;
-                uint8_t* dst = ring + s * F::TILE;
-                constexpr int LPR = HD / 16;              // lanes per row
-                constexpr int RPI = 32 / LPR;             // rows per step
-                constexpr int STEPS = KS / F::NPREP / RPI;
-                const int c = lane % LPR;                 // 16 codes of a row
-                const bool swap = (c >> 2) & 1;           // other bank half first
-                const int r0 = w * (KS / F::NPREP) + lane / LPR;
-                uint4 x[STEPS];
-#pragma unroll
-                for (int i = 0; i < STEPS; ++i)
-                    x[i] = *reinterpret_cast<const uint4*>(src + (r0 + i * RPI) * HD + 16 * c);
-#pragma unroll
-                for (int i = 0; i < STEPS; ++i) {
-                    const int r = r0 + i * RPI;
-                    const uint32_t x0 = x[i].x ^ 0x80808080u, x1 = x[i].y ^ 0x80808080u;
-                    const uint32_t x2 = x[i].z ^ 0x80808080u, x3 = x[i].w ^ 0x80808080u;
-                    const uint4 lo = make_uint4(codes2<0x4140>(x0), codes2<0x4342>(x0),
-                                                codes2<0x4140>(x1), codes2<0x4342>(x1));
-                    const uint4 hi = make_uint4(codes2<0x4140>(x2), codes2<0x4342>(x2),
-                                                codes2<0x4140>(x3), codes2<0x4342>(x3));
-                    uint8_t* row = dst + (c >> 2) * F::SUB + r * 128;
-                    const int ch = 2 * (c & 3);
-                    *reinterpret_cast<uint4*>(row + (((ch + swap) ^ (r & 7)) << 4)) =
-                        swap ? hi : lo;
-                    *reinterpret_cast<uint4*>(row + (((ch + !swap) ^ (r & 7)) << 4)) =
-                        swap ? lo : hi;
+            if (*dead && lane == 0) {  // let issued copies land before the CTA leaves
+                for (int par = 0; par < 2; ++par) {
+                    for (int i = 0; i < F::NSC; ++i) mbar_wait(&sc_full[i], par);
+                    for (int i = 0; i < (F::kQ8 ? F::NR : NS); ++i)
+                        mbar_wait(F::kQ8 ? &raw_full[i] : &full[i], par);
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&ready[s]);
-                    mbar_arrive(&raw_empty[rs]);
-                }
+            }
+        } else if (warp == 1) {
+            // --------------------------------------------------------- MMA
+            // The whole warp runs this; an elected lane issues a group of MMAs
+            // in one branch (a predicate on each of them cost 4 %).
+            constexpr uint32_t fmt = F::kHalf ? 0u : 1u;
+            constexpr uint32_t id_s = idesc_f16(fmt, 128, KS);
+            constexpr uint32_t id_o = idesc_f16(fmt, 128, HD) | (1u << 16);  // B is MN-major
+            const uint32_t lead = elect_lane();
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint64_t dq0 = uniform(smem_desc_k_sw128(sQ));
+            const uint64_t dk0 = uniform(smem_desc_k_sw128(sRing));
+            const uint64_t dv0 = uniform(smem_desc_mn_sw128(sRing, F::SUB));
+            uint32_t it = 0, np[2] = {0, 0}, no[2] = {0, 0};  // no: segments of a stage
+            // slot of operand tile t once it is there, as descriptor offset
+            auto operand = [&](uint32_t t, uint32_t& off) -> bool {
+                const int s = t % NS;
+                // ready of a 16-bit ring only counts V tiles (odd t, even NSL)
+                uint64_t* b = F::kQ8 || (t & 1) ? &ready[s] : &full[s];
+                if (!ring_wait(b, (t / NS) & 1, dead)) return false;
+                tc_fence_after();
+                off = __shfl_sync(0xffffffffu, (uint32_t)s * (F::TILE >> 4), 0);
+                return true;
             };
-            uint32_t t = 0;
-            for (uint32_t u = 0; u <= (uint32_t)total; ++u) {
-                if (u < (uint32_t)total) {
-                    const int ss = u % F::NSC;
-                    ring_wait(&sc_full[ss], (u / F::NSC) & 1, dead);
-                    if (lane == 0) mbar_arrive(&sc_empty[ss]);
+            auto scores = [&](int i, uint32_t koff) {
+                const uint64_t dq = dq0 + i * (F::TILE >> 4), dk = dk0 + koff;
+                if (lead) {
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const int o = (k / 4) * (F::SUB >> 4) + 2 * (k % 4);
+                        umma_f16_ss(tm + i * 128, dq + o, dk + o, id_s, k != 0);
+                    }
+                    umma_commit(&s_full[i]);
                 }
-#pragma unroll 1
-                for (int v = 0; v < 2; ++v)
-                    if (v ? u > 0 : u < (uint32_t)total)
-                        convert(t++, v ? v_empty : k_empty, v ? v_ready : k_ready, v ? sV : sK,
-                                u - v);
+                __syncwarp();
+            };
+            PlanPos& p = wk.p;
+            for (int left = total; left > 0;) {
+                const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
+                const int m = min(tw.count - p.i, left);
+                const int stages = p.n * a.gqa - p.t * TR > 128 ? 2 : 1;
+                uint32_t koff, voff = 0;
+                bool on = operand(2 * it, koff);
+                for (int i = 0; on && i < stages; ++i) {
+                    on = ring_wait(&q_full[i], no[i] & 1, dead);
+                    if (!on) break;
+                    tc_fence_after();
+                    scores(i, koff);
+                    if (m == 1) commit_lead(&q_empty[i], lead);
+                }
+                if (!on) break;
+                commit_lead(&empty[2 * it % NS], lead);
+                for (int j = 0; j < m; ++j) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (i >= stages) break;
+                        on = ring_wait(&p_half[i], np[i] & 1, dead) &&
+                             (i != 0 || operand(2 * (it + j) + 1, voff)) &&
+                             (j != 0 || ring_wait(&o_empty[i], (no[i] & 1) ^ 1, dead));
+                        if (!on) break;
+                        tc_fence_after();
+                        const uint64_t dv = dv0 + voff;
+                        if (lead) {
+#pragma unroll
+                            for (int k = 0; k < KS / 32; ++k)
+                                umma_f16_ts(tm + 256 + i * 128, tm + i * 128 + 8 * k, dv + k * 128,
+                                            id_o, j != 0 || k != 0);
+                        }
+                        __syncwarp();
+                        on = ring_wait(&p_full[i], np[i]++ & 1, dead);
+                        if (!on) break;
+                        tc_fence_after();
+                        if (lead) {
+#pragma unroll
+                            for (int k = KS / 32; k < KS / 16; ++k)
+                                umma_f16_ts(tm + 256 + i * 128, tm + i * 128 + 8 * k, dv + k * 128,
+                                            id_o, 1);
+                        }
+                        __syncwarp();
+                        if (j + 1 < m) {
+                            on = i != 0 || operand(2 * (it + j + 1), koff);
+                            if (!on) break;
+                            scores(i, koff);
+                            if (j + 2 == m) commit_lead(&q_empty[i], lead);
+                        } else {
+                            commit_lead(&o_full[i], lead);
+                            ++no[i];
+                        }
+                    }
+                    if (!on) break;
+                    commit_lead(&empty[(2 * (it + j) + 1) % NS], lead);
+                    if (j + 1 < m) commit_lead(&empty[2 * (it + j + 1) % NS], lead);
+                }
+                if (!on) break;
+                it += m;
+                left -= m;
+                if (left > 0) P::next_tile(a, p);
             }
+            if (*dead) {  // nothing of this CTA may be in flight when it leaves
+                commit_lead(drain, lead);
+                mbar_wait_warp(drain, 0);
+            }
+            __syncwarp();
         } else {
+            // ------------------------------------------- operand preparation
+            // and each of the two warps brings the q rows of a stage
+            const int w = warp - 2;
+            uint32_t seg = 0, nq = 0;  // segments, and those with rows of this stage
             for (uint32_t u = 0; u < (uint32_t)total; ++u) {
-                const int ss = u % F::NSC, s = u % NS;
+                if (wk.first()) {
+                    const int pr0 = wk.p.t * TR + w * 128, rows = wk.p.n * a.gqa;
+                    if (pr0 < rows) {
+                        // (the last tile's scores are all done)
+                        if (!ring_wait(&q_empty[w], (nq & 1) ^ 1, dead)) break;
+                        ++nq;
+                        load_q<F>(a, wk.p, pr0, rows, sQ + w * F::TILE,
+                                  sC + ((seg & 3) * 2 + w) * 128);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&q_full[w]);
+                    }
+                    ++seg;
+                }
+                const int ss = u % F::NSC;
                 ring_wait(&sc_full[ss], (u / F::NSC) & 1, dead);
                 const int flag = sFlag[ss];
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sc_empty[ss]);
-                const int key0 = wk.key0();
-                const bool whole = flag == 15 && key0 + KS - 1 <= wk.tw.p_first &&
-                                   (a.window == 0 || wk.tw.p_last - key0 < a.window ||
-                                    key0 + KS - 1 < a.n_sink);
-                if (ring_wait(&v_full[s], (u / NS) & 1, dead)) {
-                    if (!whole) {
-                        constexpr uint32_t kInf = F::kHalf ? 0x7C007C00u : 0x7F807F80u;
-                        constexpr uint32_t kOne = F::kHalf ? 0x04000400u : 0x00800080u;
-                        uint4* v = reinterpret_cast<uint4*>(sV + s * F::TILE);
-#pragma unroll 4
-                        for (int q = w * 32 + lane; q < F::TILE / 16; q += 32 * F::NPREP) {
-                            uint4 x4 = v[q];
-                            uint32_t* x = reinterpret_cast<uint32_t*>(&x4);
-                            uint32_t z = 0;
+                if constexpr (F::kQ8) {
+#pragma unroll 1
+                    for (uint32_t t = 2 * u; t < 2 * u + 2; ++t) {
+                        const int rs = t % F::NR, s = t % NS;
+                        if (!ring_wait(&raw_full[rs], (t / F::NR) & 1, dead)) continue;
+                        if (!ring_wait(&empty[s], ((t / NS) & 1) ^ 1, dead)) continue;
+                        constexpr int LPR = HD / 16;       // lanes per row
+                        constexpr int RPI = 32 / LPR;      // rows per step
+                        constexpr int BATCH = 4;
+                        const int c = lane % LPR;          // 16 codes of a row
+                        const bool swap = (c >> 2) & 1;    // other bank half first
+                        const uint8_t* src = sRaw + rs * F::RAW + 16 * c;
+                        uint8_t* dst = sRing + s * F::TILE + (c >> 2) * F::SUB;
+#pragma unroll 1
+                        for (int r0 = w * (KS / F::NPREP) + lane / LPR;
+                             r0 < (w + 1) * (KS / F::NPREP); r0 += BATCH * RPI) {
+                            uint4 x[BATCH];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) z |= (x[i] & kInf) + kOne;
-                            if (z & 0x80008000u) {
+                            for (int i = 0; i < BATCH; ++i)
+                                x[i] = *reinterpret_cast<const uint4*>(src + (r0 + i * RPI) * HD);
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const uint32_t b = ((x[i] & kInf) + kOne) & 0x80008000u;
-                                    x[i] &= ~((b & 0x8000u ? 0xFFFFu : 0u) |
-                                              (b & 0x80000000u ? 0xFFFF0000u : 0u));
-                                }
-                                v[q] = x4;
-                                *odd = 1;
+                            for (int i = 0; i < BATCH; ++i) {
+                                const int r = r0 + i * RPI;
+                                const uint32_t x0 = x[i].x ^ 0x80808080u;
+                                const uint32_t x1 = x[i].y ^ 0x80808080u;
+                                const uint32_t x2 = x[i].z ^ 0x80808080u;
+                                const uint32_t x3 = x[i].w ^ 0x80808080u;
+                                const uint4 lo = make_uint4(codes2<0x4140>(x0), codes2<0x4342>(x0),
+                                                            codes2<0x4140>(x1), codes2<0x4342>(x1));
+                                const uint4 hi = make_uint4(codes2<0x4140>(x2), codes2<0x4342>(x2),
+                                                            codes2<0x4140>(x3), codes2<0x4342>(x3));
+                                const int ch = 2 * (c & 3);
+                                *reinterpret_cast<uint4*>(dst + r * 128 +
+                                                          (((ch + swap) ^ (r & 7)) << 4)) =
+                                    swap ? hi : lo;
+                                *reinterpret_cast<uint4*>(dst + r * 128 +
+                                                          (((ch + !swap) ^ (r & 7)) << 4)) =
+                                    swap ? lo : hi;
                             }
                         }
                         fence_proxy_async_smem();
                         __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(&ready[s]);
+                            mbar_arrive(&raw_empty[rs]);
+                        }
                     }
-                    if (lane == 0) mbar_arrive(&v_ready[s]);
+                } else {
+                    const uint32_t t = 2 * u + 1;
+                    const int s = t % NS;
+                    const int key0 = wk.key0();
+                    const bool whole = flag == 0xFF && key0 + KS - 1 <= wk.tw.p_first &&
+                                       (a.window == 0 || wk.tw.p_last - key0 < a.window ||
+                                        key0 + KS - 1 < a.n_sink);
+                    if (ring_wait(&full[s], (t / NS) & 1, dead)) {
+                        if (!whole) {
+                            constexpr uint32_t kInf = F::kHalf ? 0x7C007C00u : 0x7F807F80u;
+                            constexpr uint32_t kOne = F::kHalf ? 0x04000400u : 0x00800080u;
+                            uint4* v = reinterpret_cast<uint4*>(sRing + s * F::TILE);
+#pragma unroll 4
+                            for (int q = w * 32 + lane; q < F::TILE / 16; q += 32 * F::NPREP) {
+                                uint4 x4 = v[q];
+                                uint32_t* x = reinterpret_cast<uint32_t*>(&x4);
+                                uint32_t z = 0;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) z |= (x[i] & kInf) + kOne;
+                                if (z & 0x80008000u) {
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        const uint32_t b = ((x[i] & kInf) + kOne) & 0x80008000u;
+                                        x[i] &= ~((b & 0x8000u ? 0xFFFFu : 0u) |
+                                                  (b & 0x80000000u ? 0xFFFF0000u : 0u));
+                                    }
+                                    v[q] = x4;
+                                    *odd = 1;
+                                }
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                        }
+                        if (lane == 0) mbar_arrive(&ready[s]);
+                    }
                 }
                 wk.next(a);
             }
         }
     } else {
         // --------------------------------------------------------- softmax
-        const int st = warp >= 12 ? 1 : 0;
+        regs_inc<F::kRegsMany>();
+        const int st = warp >= 8 ? 1 : 0;
         const int r = (warp & 3) * 32 + lane;  // row of the stage, TMEM lane
-        const uint32_t tS0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + st * 128;
-        const uint32_t tO = tS0 + 256;
-        uint32_t u = 0, ns = 0, nd = 0, no = 0, seg = 0;
+        const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + st * 128;
+        const uint32_t tO = tS + 256;
+        uint32_t u = 0, sph = 0, no = 0, seg = 0;
         bool owner = false;
-        PlanPos& p = wk.p;
+        PlanPos p = *sPos;
         for (int left = total; left > 0; ++seg) {
             const TileWork<TR, KS> tw(a, p.n, p.len, p.t);
             const int m = min(tw.count - p.i, left);
@@ -797,69 +730,64 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                 const int ss = u % F::NSC;
                 ring_wait(&sc_full[ss], (u / F::NSC) & 1, dead);
                 if (active) {
-                    const int buf = ns & 1;
-                    const bool on = ring_wait(&s_full[2 * st + buf], (ns >> 1) & 1, dead);
-                    ++ns;
+                    const bool on = ring_wait(&s_full[st], sph & 1, dead);
+                    ++sph;
                     if (!on) continue;
-                    const uint32_t tS = tS0 + 64 * buf;
                     tc_fence_after();
+                    uint32_t s[4][32];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x32(tS + 32 * q, s[q]);
                     // (there are scores, so q and its factors were there; they
-                    // stay for four segments, scores come two chunks early)
+                    // stay for four segments, scores come a chunk early)
                     if (F::kRowScale && j == 0) c = sC[((seg & 3) * 2 + st) * 128 + r];
                     const int key0 = tw.key0(p.i + j);
                     const int flag = sFlag[ss];
                     const float4* ksc = reinterpret_cast<const float4*>(sScale + ss * 2 * KS);
                     const float4* vsc = ksc + KS / 4;
-                    const bool whole = flag == 15 && key0 + KS - 1 <= p_lo &&
+                    const bool whole = flag == 0xFF && key0 + KS - 1 <= p_lo &&
                                        (a.window == 0 || p_hi - key0 < a.window ||
                                         key0 + KS - 1 < a.n_sink);
-                    // Both passes are loops over 32 columns, read from tensor
-                    // memory twice: unrolled, with the scores in registers, the
-                    // roles' code no longer fits the SM's instruction cache
-                    // (77 % hits, the next level 74 % busy, twice the time).
-                    // ---- pass 1: the row's maximum; scaled and masked scores go back
-                    float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll 1
-                    for (int q = 0; q < KS / 32; ++q) {
-                        uint32_t s[32];
-                        tmem_ld_32x32b_x32(tS + 32 * q, s);
-                        tmem_ld_done(s);
-                        if constexpr (F::kQ8) {
-                            float4 k4[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) k4[i] = ksc[8 * q + i];
+                    for (int q = 0; q < 4; ++q) tmem_ld_done(s[q]);
+                    // ---- the row's scores and their maximum
+                    if constexpr (F::kQ8) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                scale2(s[4 * i], s[4 * i + 1], f2(k4[i].x, k4[i].y));
-                                scale2(s[4 * i + 2], s[4 * i + 3], f2(k4[i].z, k4[i].w));
-                            }
-                        }
-                        if (!whole) {
-                            const uint32_t seen = seen_bits(a, pos, key0, flag, q);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (!((seen >> i) & 1)) s[i] = 0xFF800000u;
-                        }
-                        if (F::kQ8 || !whole) tmem_st_x32(tS + 32 * q, s);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            m0 = max3n(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                            m1 = max3n(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                        for (int i = 0; i < 32; ++i) {
+                            const float4 k4 = ksc[i];
+                            uint32_t* x = &s[i / 8][4 * (i % 8)];
+                            scale2(x[0], x[1], f2(k4.x, k4.y));
+                            scale2(x[2], x[3], f2(k4.z, k4.w));
                         }
                     }
-                    if (F::kQ8 || !whole) tmem_st_wait();
-                    const float mx = max3n(m0, m1, m1) * c;
+                    if (!whole) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const uint32_t seen = seen_bits(a, pos, key0 + 32 * q, flag >> (2 * q));
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (!((seen >> i) & 1)) s[q][i] = 0xFF800000u;
+                        }
+                    }
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            m4[q] = max3n(m4[q], __uint_as_float(s[q][i]),
+                                          __uint_as_float(s[q][i + 1]));
+                    const float mx = max3n(max3n(m4[0], m4[1], m4[2]), m4[3], m4[3]) * c;
                     int Et = E;
                     if constexpr (F::kQ8) {
                         // V's largest scale in this chunk, of positions some row may see
-                        const float2 v2 = reinterpret_cast<const float2*>(vsc)[lane];
-                        const int n = ((flag >> (lane / 8)) & 1) ? tw.p_last - key0 - 2 * lane : -1;
+                        const float4 v4 = vsc[lane];
+                        const int n = ((flag >> (lane / 4)) & 1) ? tw.p_last - key0 - 4 * lane : -1;
                         auto bits = [&](float v, int at) {
                             const uint32_t b = __float_as_uint(fabsf(v));
                             return at <= n && b < 0x7F800000u ? b : 0u;
                         };
-                        const uint32_t top =
-                            __reduce_max_sync(0xffffffffu, max(bits(v2.x, 0), bits(v2.y, 1)));
+                        const uint32_t top = __reduce_max_sync(
+                            0xffffffffu, max(max(bits(v4.x, 0), bits(v4.y, 1)),
+                                             max(bits(v4.z, 2), bits(v4.w, 3))));
                         Et = max(E, min((int)(top >> 23) - 126, 126));
                     }
                     if (__any_sync(0xffffffffu, mx > M + 8.f || Et > E)) {
@@ -869,12 +797,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                         M = N;
                         E = Et;
                         l2 = f2mul(l2, f2(f, f));
-                        // PV of the last chunk (not every PV is waited for; the
-                        // two barriers in turn are at most one phase behind,
-                        // since S of the last chunk came after the PV before it)
-                        const uint32_t g = nd + j - 1;
-                        if (j > 0 && ring_wait(&pv_done[2 * st + (g & 1)], (g >> 1) & 1, dead)) {
-                            tc_fence_after();
+                        if (j > 0) {
 #pragma unroll 1
                             for (int q = 0; q < HD / 32; ++q) {
                                 uint32_t o[32];
@@ -887,57 +810,52 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                             }
                         }
                     }
-                    // ---- pass 2: weights 2^(z - D), packed over the scores; a
-                    // visible NaN makes all of them NaN
+                    // ---- weights 2^(z - D), packed over the scores; a visible NaN
+                    // makes all of them NaN
                     const float D = mx != mx ? mx
                                              : kUp - (M == -INFINITY ? 0.f : M) -
                                                    (float)(F::kQ8 ? E : 0);
                     const uint64_t c2 = f2(c, c), d2 = f2(D, D);
-#pragma unroll 1
-                    for (int q = 0; q < KS / 32; ++q) {
-                        uint32_t s[32], w[16];
-                        tmem_ld_32x32b_x32(tS + 32 * q, s);
-                        float4 v4[F::kQ8 ? 8 : 1];
-                        if constexpr (F::kQ8) {
+                    uint64_t lb = 0;
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) v4[i] = vsc[8 * q + i];
-                        }
-                        tmem_ld_done(s);
-                        uint64_t la = 0, lb = 0;
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t w[16];
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            const uint64_t z0 = f2fma(f2u(s[i], s[i + 1]), c2, d2);
-                            const uint64_t z1 = f2fma(f2u(s[i + 2], s[i + 3]), c2, d2);
+                            const uint64_t z0 = f2fma(f2u(s[q][i], s[q][i + 1]), c2, d2);
+                            const uint64_t z1 = f2fma(f2u(s[q][i + 2], s[q][i + 3]), c2, d2);
                             float w0 = ex2(f2lo(z0)), w1 = ex2(f2hi(z0));
                             float w2 = ex2(f2lo(z1)), w3 = ex2(f2hi(z1));
-                            la = f2add(la, f2(w0, w1));
+                            l2 = f2add(l2, f2(w0, w1));
                             lb = f2add(lb, f2(w2, w3));
                             if constexpr (F::kQ8) {
-                                scale2f(w0, w1, f2(v4[i / 4].x, v4[i / 4].y));
-                                scale2f(w2, w3, f2(v4[i / 4].z, v4[i / 4].w));
+                                const float4 v4 = vsc[8 * q + i / 4];
+                                scale2f(w0, w1, f2(v4.x, v4.y));
+                                scale2f(w2, w3, f2(v4.z, v4.w));
                             }
                             w[i / 2] = pack<OT>(w0, w1);
                             w[i / 2 + 1] = pack<OT>(w2, w3);
                         }
-                        l2 = f2add(l2, f2add(la, lb));
                         if (F::kQ8 && !whole) {  // a hidden position's scale may be anything
-                            const uint32_t seen = seen_bits(a, pos, key0, flag, q);
+                            const uint32_t seen = seen_bits(a, pos, key0 + 32 * q, flag >> (2 * q));
 #pragma unroll
                             for (int i = 0; i < 16; ++i)
                                 w[i] &= ((seen >> (2 * i)) & 1 ? 0xFFFFu : 0u) |
                                         ((seen >> (2 * i)) & 2 ? 0xFFFF0000u : 0u);
                         }
                         tmem_st_x16(tS + 16 * q, w);
+                        if (q & 1) {  // half of the keys: their products may begin
+                            tmem_st_wait();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(q == 1 ? &p_half[st] : &p_full[st]);
+                        }
                     }
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[2 * st + buf]);
+                    l2 = f2add(l2, lb);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sc_empty[ss]);
             }
-            if (active) nd += m - 1;  // the last PV of a segment answers on o_full
 
             // ---- the finished rows, or this piece of them
             if (active && ring_wait(&o_full[st], no++ & 1, dead)) {
@@ -946,48 +864,35 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                 const float l = f2lo(l2) + f2hi(l2);
                 // no finite score seen: zeros, unless it was a NaN
                 const float inv = piece ? 1.f : M == -INFINITY && l == l ? 0.f : 1.f / l;
-                const int64_t row0 =
-                    (2 * (int64_t)blockIdx.x + (cut_l ? 0 : 1)) * TR + st * 128 + (warp & 3) * 32;
-                if (piece) a.stat[row0 + lane] = make_float2(M + (float)(F::kQ8 ? E : 0), l);
-                const unsigned alive = __ballot_sync(0xffffffffu, live);
-                const int64_t off = (int64_t)(p.row + tok) * a.out_stride + (int64_t)h * HD;
-#pragma unroll 1
-                for (int q2 = 0; q2 < HD / 64; ++q2) {
-                    uint32_t y[32];  // 64 dimensions of this row, 16 bits each
-#pragma unroll 1
-                    for (int q = 2 * q2; q < 2 * q2 + 2; ++q) {
-                        uint32_t s[32];
-                        tmem_ld_32x32b_x32(tO + 32 * q, s);
-                        tmem_ld_done(s);
-                        if constexpr (!F::kQ8) {
-                            if (*odd && live) add_odd<F>(a, p, tw, m, pos, 32 * q, s);
-                        }
-                        if (piece) {
-                            turn8(s);
-                            float* o = a.part + (row0 + (lane & ~7)) * HD + 32 * q + 4 * (lane & 7);
+                const int64_t pslot = 2 * (int64_t)blockIdx.x + (cut_l ? 0 : 1);
+                float* part = a.part + (pslot * TR + st * 128 + r) * HD;
+                if (piece)
+                    a.stat[pslot * TR + st * 128 + r] =
+                        make_float2(M + (float)(F::kQ8 ? E : 0), l);
+                X* o = static_cast<X*>(a.out) + (int64_t)(p.row + tok) * a.out_stride +
+                       (int64_t)h * HD;
 #pragma unroll
-                            for (int k = 0; k < 8; ++k)
-                                *reinterpret_cast<uint4*>(o + k * HD) =
-                                    make_uint4(s[4 * k], s[4 * k + 1], s[4 * k + 2], s[4 * k + 3]);
-                        } else {
+                for (int q = 0; q < HD / 32; ++q) {
+                    uint32_t s[32];
+                    tmem_ld_32x32b_x32(tO + 32 * q, s);
+                    tmem_ld_done(s);
+                    if (!F::kQ8 && *odd && live)
+                        add_odd<F>(a, p, tw, m, pos, 32 * q, s);
+                    if (piece) {
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) {
-                                y[k] = y[16 + k];
-                                y[16 + k] = pack<X>(__uint_as_float(s[2 * k]) * inv,
-                                                    __uint_as_float(s[2 * k + 1]) * inv);
-                            }
-                        }
-                    }
-                    if (!piece) {
-                        turn8(y);
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4*>(part + 32 * q + i) =
+                                make_uint4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+                    } else if (live) {
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const int from = (lane & ~7) + k;
-                            const int64_t at = __shfl_sync(0xffffffffu, off, from);
-                            X* o = static_cast<X*>(a.out) + at + 64 * q2 + 8 * (lane & 7);
-                            if ((alive >> from) & 1)
-                                *reinterpret_cast<uint4*>(o) =
-                                    make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
+                        for (int i = 0; i < 32; i += 8) {
+                            uint32_t y[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                y[k] = pack<X>(__uint_as_float(s[i + 2 * k]) * inv,
+                                               __uint_as_float(s[i + 2 * k + 1]) * inv);
+                            *reinterpret_cast<uint4*>(o + 32 * q + i) =
+                                make_uint4(y[0], y[1], y[2], y[3]);
                         }
                     }
                 }
@@ -997,7 +902,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             }
             if (cut_r && !cut_l) {
                 owner = true;
-                if (threadIdx.x == 256) {
+                if (threadIdx.x == 128) {
                     const int64_t end = u0 + (total - left) + tw.count;
                     CutTile ct;
                     ct.pieces = (int)((end - 1) / L - blockIdx.x) + 1;
@@ -1011,7 +916,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             left -= m;
             if (left > 0) P::next_tile(a, p);
         }
-        if (!owner && threadIdx.x == 256) a.cut[blockIdx.x].pieces = 0;
+        if (!owner && threadIdx.x == 128) a.cut[blockIdx.x].pieces = 0;
     }
 
     tc_fence_before();
@@ -1042,7 +947,7 @@ int launch_tc(const PagedJob& j) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tk, tv, j.a, 4);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tk, tv, j.a, 2);
     if (e != cudaSuccess) return cuda_error(e, "launch paged_tc");
     return FTC_OK;
 }
