@@ -3,8 +3,7 @@
 // reading rows back.
 //
 // Both move every byte once and are bound by HBM, or for a decode step by
-// the launch: a thread takes 8 consecutive values of a row of K and the same
-// 8 of V (two 16-byte loads of fp32 each, both tensors' loads in flight
+// the launch: a piece of work is 8 values of a row of K and the same 8 of V (two 16-byte loads of fp32 each, both tensors' loads in flight
 // together), so a row of head_dim values is head_dim / 8 neighbouring lanes
 // and its maximum is a shuffle reduction inside a warp.
 #include <cuda_bf16.h>
@@ -77,17 +76,67 @@ namespace {
 
 constexpr int kRowThreads = 256;
 
-// 8 values in fp32 from / to a row of T
+// Where lane l's 8 values of a row lie: next to each other, or with fp32 rows
+// 4 in each half of the row, so that a warp's 16-byte accesses of the fp32 side
+// are whole sectors (8 neighbours made every store write half sectors).
+template <typename X, int HD>
+struct Spread {
+    static constexpr bool kSplit = sizeof(X) == 4;
+    static __device__ __forceinline__ int lo(int lane) { return (kSplit ? 4 : 8) * lane; }
+    static __device__ __forceinline__ int hi(int lane) {
+        return kSplit ? HD / 2 + 4 * lane : 8 * lane + 4;
+    }
+};
+
+// 8 values of a row of T as loaded, and in fp32
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+};
+
+// p: the row; S: the spread of the side whose type is X (T the type read)
+template <class S, typename T>
+__device__ __forceinline__ Raw8<T> load8(const T* p, int lane) {
+    Raw8<T> r;
     if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0];
-        const float4 b = reinterpret_cast<const float4*>(p)[1];
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-        x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        r.w[0] = *reinterpret_cast<const uint4*>(p + S::lo(lane));
+        r.w[1] = *reinterpret_cast<const uint4*>(p + S::hi(lane));
+    } else if constexpr (S::kSplit) {
+        const uint2 a = *reinterpret_cast<const uint2*>(p + S::lo(lane));
+        const uint2 b = *reinterpret_cast<const uint2*>(p + S::hi(lane));
+        r.w[0] = make_uint4(a.x, a.y, b.x, b.y);
     } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        r.w[0] = *reinterpret_cast<const uint4*>(p + S::lo(lane));
+    }
+    return r;
+}
+
+// 8 codes of a row
+template <class S>
+__device__ __forceinline__ uint2 load_codes(const int8_t* p, int lane) {
+    if constexpr (S::kSplit)
+        return make_uint2(*reinterpret_cast<const uint32_t*>(p + S::lo(lane)),
+                          *reinterpret_cast<const uint32_t*>(p + S::hi(lane)));
+    else return *reinterpret_cast<const uint2*>(p + S::lo(lane));
+}
+
+template <class S>
+__device__ __forceinline__ void store_codes(int8_t* p, int lane, uint2 c) {
+    if constexpr (S::kSplit) {
+        *reinterpret_cast<uint32_t*>(p + S::lo(lane)) = c.x;
+        *reinterpret_cast<uint32_t*>(p + S::hi(lane)) = c.y;
+    } else {
+        *reinterpret_cast<uint2*>(p + S::lo(lane)) = c;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void floats(const Raw8<T>& r, float (&x)[8]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+    } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (std::is_same<T, __half>::value) {
@@ -98,6 +147,23 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
                 x[2 * i + 1] = bf2f(w[i] >> 16);
             }
         }
+    }
+}
+
+// Bits of the largest |x| of the 8 (16-bit types: both halves of a word at once).
+template <typename T>
+__device__ __forceinline__ uint32_t top8(const Raw8<T>& r) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+    uint32_t t = 0;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t = max(t, w[i] & 0x7FFFFFFFu);
+        return t;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t = __vmaxu2(t, w[i] & 0x7FFF7FFFu);
+        t = max(t & 0xFFFFu, t >> 16);
+        return std::is_same<T, __half>::value ? __float_as_uint(h2f(t)) : t << 16;
     }
 }
 
@@ -112,35 +178,44 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+template <class S, typename T>
+__device__ __forceinline__ void store8(T* p, int lane, const float (&x)[8]) {
     if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        *reinterpret_cast<float4*>(p + S::lo(lane)) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(p + S::hi(lane)) = make_float4(x[4], x[5], x[6], x[7]);
     } else {
-        *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]),
-                                                  pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+        const uint2 a = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+        const uint2 b = make_uint2(pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+        if constexpr (S::kSplit) {
+            *reinterpret_cast<uint2*>(p + S::lo(lane)) = a;
+            *reinterpret_cast<uint2*>(p + S::hi(lane)) = b;
+        } else {
+            *reinterpret_cast<uint4*>(p + S::lo(lane)) = make_uint4(a.x, a.y, b.x, b.y);
+        }
     }
 }
 
-// The cache slot of this thread's row: CTA rows start at token t0.  The
-// CTA's first sequence is the number of sequences that end at or before t0
-// (one round of loads over all threads); a later row walks on from there.
+// The cache slot of a row.
 struct Slot {
     int page;  // -1: not mapped
     int slot;
     bool live;  // false: padding
 };
 
-__device__ __forceinline__ Slot find_slot(const PageView& b, int t0, int t) {
+// Sequences that end at or before token t0: where a CTA's rows begin to look
+// (one round of loads over all threads; a later row walks on from there).
+__device__ __forceinline__ int first_seq(const PageView& b, int t0) {
     int before = 0;
     for (int i0 = 0; i0 < b.n_seqs; i0 += kRowThreads) {
         const int i = i0 + (int)threadIdx.x;
         before += __syncthreads_count(i < b.n_seqs && b.start[i + 1] <= t0);
     }
+    return before;
+}
+
+__device__ __forceinline__ Slot find_slot(const PageView& b, int s, int t) {
     Slot r = {-1, 0, false};
     if (t >= b.n_tokens) return r;
-    int s = before;
     while (s < b.n_seqs && b.start[s + 1] <= t) ++s;
     if (s >= b.n_seqs) return r;
     int r0, n;
@@ -153,18 +228,33 @@ __device__ __forceinline__ Slot find_slot(const PageView& b, int t0, int t) {
     return r;
 }
 
+// Row and head of piece g of the batch's rows (32-bit arithmetic: a 64-bit
+// division a piece cost more than the piece).
+template <int HD>
+struct Piece {
+    int t, h, lane;
+    __device__ __forceinline__ Piece(const PageView& b, uint32_t g) {
+        constexpr uint32_t LANES = HD / 8;
+        const uint32_t row = g / LANES;
+        t = (int)(row / (uint32_t)b.n_kv);
+        h = (int)(row - (uint32_t)t * (uint32_t)b.n_kv);
+        lane = (int)(g % LANES);
+    }
+};
+
 // Row of 8-bit codes: d = max|x| / 127 and the codes of this thread's 8
 // values.  |x| is compared as integer bits, so a NaN wins over an infinity
 // and both over every finite value.  The code is the exactly rounded
-// quotient: c = rint(x * (1 / d)) is within one of it, and the residual
-// r = x - c d (one fused multiply-add, exact here: c d has at most 32 bits
-// and cancels to within d) says which side of the half it is on, so no
-// division per value.  Tiny d are scaled by 2^64 first to keep 1 / d finite.
+// quotient: c = x * (1 / d) rounded (by adding 1.5 * 2^23, whose low byte then
+// is the code) is within one of it, and the residual r = x - c d (one fused
+// multiply-add, exact here: c d has at most 32 bits and cancels to within d)
+// tells: |r| < d / 2 and c stands, else the half that it is on decides.  So no
+// division and no conversion per value.  Tiny d are scaled by 2^64 first, which
+// keeps 1 / d finite.
+// top: the bits of this thread's largest |x|.
 template <int LANES>
-__device__ __forceinline__ uint2 quantise8(const float (&x)[8], float& d) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+__device__ __forceinline__ uint2 quantise8(float (&x)[8], uint32_t top, float& d) {
+    constexpr float kRound = 12582912.f;
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (top >= 0x7F800000u) {
@@ -173,94 +263,161 @@ __device__ __forceinline__ uint2 quantise8(const float (&x)[8], float& d) {
     }
     d = __fdiv_rn(__uint_as_float(top), 127.f);
     if (d == 0.f) return make_uint2(0, 0);
-    const float up = d < 1e-30f ? 18446744073709551616.f : 1.f;
-    const float ds = d * up, inv = __frcp_rn(ds);
-    uint32_t w[2] = {0, 0};
+    float ds = d;
+    if (d < 1e-30f) {
+        ds = d * 18446744073709551616.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float xs = x[i] * up;
-        float c = rintf(xs * inv);
-        const float r2 = 2.f * fmaf(-c, ds, xs);
-        const bool odd = ((int)c & 1) != 0;
-        if (r2 > ds || (r2 == ds && odd)) c += 1.f;
-        else if (r2 < -ds || (r2 == -ds && odd)) c -= 1.f;
-        c = fminf(fmaxf(c, -127.f), 127.f);  // a subnormal d may be far below max|x| / 127
-        w[i >> 2] |= ((uint32_t)(int)c & 0xFFu) << (8 * (i & 3));
+        for (int i = 0; i < 8; ++i) x[i] *= 18446744073709551616.f;
     }
-    return make_uint2(w[0], w[1]);
+    const float inv = __frcp_rn(ds), half = 0.5f * ds;
+    uint32_t q[8];
+    float far = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const uint64_t v = f2(x[i], x[i + 1]);
+        const uint64_t t = f2add(f2mul(v, f2(inv, inv)), f2(kRound, kRound));
+        const uint64_t r = f2fma(f2add(f2(kRound, kRound), f2mul(t, f2(-1.f, -1.f))), f2(ds, ds), v);
+        q[i] = (uint32_t)t;
+        q[i + 1] = (uint32_t)(t >> 32);
+        far = fmaxf(far, fmaxf(fabsf(f2lo(r)), fabsf(f2hi(r))));
+    }
+    if (far >= half || d < 1e-30f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float c = __uint_as_float(q[i]) - kRound;
+            const float r = fmaf(-c, ds, x[i]);
+            const bool odd = q[i] & 1;
+            if (r > half || (r == half && odd)) c += 1.f;
+            else if (r < -half || (r == -half && odd)) c -= 1.f;
+            // (a subnormal d may be far below max|x| / 127)
+            c = fminf(fmaxf(c, -127.f), 127.f);
+            q[i] = __float_as_uint(c + kRound);
+        }
+    }
+    auto bytes = [](uint32_t a, uint32_t b, uint32_t c, uint32_t e) {
+        return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, e, 0x0040), 0x5410);
+    };
+    return make_uint2(bytes(q[0], q[1], q[2], q[3]), bytes(q[4], q[5], q[6], q[7]));
 }
 
-// C: cache element (__half, __nv_bfloat16 or int8_t), X: row element
-template <typename X, typename C, int HD>
+// C: cache element (__half, __nv_bfloat16 or int8_t), X: row element, R: pieces
+// per thread, kRowThreads apart.  The rows' loads are issued before the slots
+// are looked up (start, kv_len and the table hang on one another).
+template <typename X, typename C, int HD, int R>
 __global__ void __launch_bounds__(kRowThreads)
 kv_pages_write_kernel(const PageView b, const X* __restrict__ kx, const X* __restrict__ vx,
                       int64_t x_stride, C* kc, C* vc, float* ks, float* vs) {
+    using S = Spread<X, HD>;
     constexpr int LANES = HD / 8;
-    const int per_token = b.n_kv * LANES;  // threads
-    const int64_t g0 = (int64_t)blockIdx.x * kRowThreads;
-    const int64_t g = g0 + threadIdx.x;
-    const int t = (int)(g / per_token), rest = (int)(g - (int64_t)t * per_token);
-    const int h = rest / LANES, lane = rest % LANES;
-    const Slot at = find_slot(b, (int)(g0 / per_token), t);
-    float k[8] = {}, v[8] = {};
-    if (at.live) {
-        const int64_t off = (int64_t)t * x_stride + (int64_t)h * HD + 8 * lane;
-        load8(kx + off, k);
-        load8(vx + off, v);
-    }
-    const int64_t row = (int64_t)h * b.page_size + at.slot;
-    const int64_t dst = at.page * b.page_stride + row * HD + 8 * lane;
-    if constexpr (sizeof(C) == 1) {
-        float dk, dv;
-        const uint2 ck = quantise8<LANES>(k, dk), cv = quantise8<LANES>(v, dv);
-        if (at.page < 0) return;
-        *reinterpret_cast<uint2*>(kc + dst) = ck;
-        *reinterpret_cast<uint2*>(vc + dst) = cv;
-        if (lane == 0) {
-            ks[at.page * b.scale_stride + row] = dk;
-            vs[at.page * b.scale_stride + row] = dv;
+    const uint32_t g0 = blockIdx.x * (uint32_t)(kRowThreads * R);
+    Raw8<X> kr[R], vr[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const Piece<HD> p(b, g0 + i * kRowThreads + threadIdx.x);
+        if (p.t < b.n_tokens) {
+            const int64_t off = (int64_t)p.t * x_stride + (int64_t)p.h * HD;
+            kr[i] = load8<S>(kx + off, p.lane);
+            vr[i] = load8<S>(vx + off, p.lane);
+        } else {
+            kr[i] = {}, vr[i] = {};
         }
-    } else {
-        if (at.page < 0) return;
-        store8(kc + dst, k);
-        store8(vc + dst, v);
+    }
+    const int s0 = first_seq(b, Piece<HD>(b, g0).t);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const Piece<HD> p(b, g0 + i * kRowThreads + threadIdx.x);
+        const Slot at = find_slot(b, s0, p.t);
+        const int64_t row = (int64_t)p.h * b.page_size + at.slot;
+        const int64_t dst = at.page * b.page_stride + row * HD;
+        if constexpr (sizeof(C) == 1) {
+            float k[8], v[8], dk, dv;
+            floats(kr[i], k);
+            floats(vr[i], v);
+            const uint2 ck = quantise8<LANES>(k, top8(kr[i]), dk);
+            const uint2 cv = quantise8<LANES>(v, top8(vr[i]), dv);
+            if (at.page < 0) continue;
+            store_codes<S>(kc + dst, p.lane, ck);
+            store_codes<S>(vc + dst, p.lane, cv);
+            if (p.lane == 0) {
+                ks[at.page * b.scale_stride + row] = dk;
+                vs[at.page * b.scale_stride + row] = dv;
+            }
+        } else {
+            if (at.page < 0) continue;
+            if constexpr (std::is_same<X, C>::value) {
+                *reinterpret_cast<uint4*>(kc + dst + 8 * p.lane) = kr[i].w[0];
+                *reinterpret_cast<uint4*>(vc + dst + 8 * p.lane) = vr[i].w[0];
+            } else {
+                float k[8], v[8];
+                floats(kr[i], k);
+                floats(vr[i], v);
+                store8<S>(kc + dst, p.lane, k);
+                store8<S>(vc + dst, p.lane, v);
+            }
+        }
     }
 }
 
-template <typename X, typename C, int HD>
+template <typename X, typename C, int HD, int R>
 __global__ void __launch_bounds__(kRowThreads)
 kv_pages_read_kernel(const PageView b, X* __restrict__ kx, X* __restrict__ vx, int64_t x_stride,
-                     const C* kc, const C* vc, const float* ks, const float* vs) {
-    constexpr int LANES = HD / 8;
-    const int per_token = b.n_kv * LANES;
-    const int64_t g0 = (int64_t)blockIdx.x * kRowThreads;
-    const int64_t g = g0 + threadIdx.x;
-    const int t = (int)(g / per_token), rest = (int)(g - (int64_t)t * per_token);
-    const int h = rest / LANES, lane = rest % LANES;
-    const Slot at = find_slot(b, (int)(g0 / per_token), t);
-    if (!at.live) return;
-    float k[8] = {}, v[8] = {};
-    if (at.page >= 0) {
-        const int64_t row = (int64_t)h * b.page_size + at.slot;
-        const int64_t src = at.page * b.page_stride + row * HD + 8 * lane;
-        if constexpr (sizeof(C) == 1) {
-            const float dk = ks[at.page * b.scale_stride + row];
-            const float dv = vs[at.page * b.scale_stride + row];
-            const uint2 ck = *reinterpret_cast<const uint2*>(kc + src);
-            const uint2 cv = *reinterpret_cast<const uint2*>(vc + src);
+                     const C* __restrict__ kc, const C* __restrict__ vc,
+                     const float* __restrict__ ks, const float* __restrict__ vs) {
+    using S = Spread<X, HD>;
+    const uint32_t g0 = blockIdx.x * (uint32_t)(kRowThreads * R);
+    const int s0 = first_seq(b, Piece<HD>(b, g0).t);
+    // all pieces' loads in flight together
+    uint2 kq[R], vq[R];
+    Raw8<typename std::conditional<sizeof(C) == 1, __half, C>::type> kr[R], vr[R];
+    float dk[R], dv[R];
+    Slot at[R];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                k[i] = dk * (float)(int8_t)((i < 4 ? ck.x : ck.y) >> (8 * (i & 3)));
-                v[i] = dv * (float)(int8_t)((i < 4 ? cv.x : cv.y) >> (8 * (i & 3)));
+    for (int i = 0; i < R; ++i) {
+        const Piece<HD> p(b, g0 + i * kRowThreads + threadIdx.x);
+        at[i] = find_slot(b, s0, p.t);
+        const int64_t row = (int64_t)p.h * b.page_size + at[i].slot;
+        const int64_t src = at[i].page * b.page_stride + row * HD;
+        if constexpr (sizeof(C) == 1) {
+            kq[i] = vq[i] = make_uint2(0, 0);
+            dk[i] = dv[i] = 0.f;
+            if (at[i].page >= 0) {
+                kq[i] = load_codes<S>(kc + src, p.lane);
+                vq[i] = load_codes<S>(vc + src, p.lane);
+                dk[i] = ks[at[i].page * b.scale_stride + row];
+                dv[i] = vs[at[i].page * b.scale_stride + row];
             }
         } else {
-            load8(kc + src, k);
-            load8(vc + src, v);
+            kr[i] = {}, vr[i] = {};
+            if (at[i].page >= 0) {
+                kr[i] = load8<S>(kc + src, p.lane);
+                vr[i] = load8<S>(vc + src, p.lane);
+            }
         }
     }
-    const int64_t off = (int64_t)t * x_stride + (int64_t)h * HD + 8 * lane;
-    store8(kx + off, k);
-    store8(vx + off, v);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (!at[i].live) continue;
+        const Piece<HD> p(b, g0 + i * kRowThreads + threadIdx.x);
+        const int64_t off = (int64_t)p.t * x_stride + (int64_t)p.h * HD;
+        if constexpr (std::is_same<X, C>::value) {
+            *reinterpret_cast<uint4*>(kx + off + 8 * p.lane) = kr[i].w[0];
+            *reinterpret_cast<uint4*>(vx + off + 8 * p.lane) = vr[i].w[0];
+        } else {
+            float k[8], v[8];
+            if constexpr (sizeof(C) == 1) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    k[e] = dk[i] * (float)(int8_t)((e < 4 ? kq[i].x : kq[i].y) >> (8 * (e & 3)));
+                    v[e] = dv[i] * (float)(int8_t)((e < 4 ? vq[i].x : vq[i].y) >> (8 * (e & 3)));
+                }
+            } else {
+                floats(kr[i], k);
+                floats(vr[i], v);
+            }
+            store8<S>(kx + off, p.lane, k);
+            store8<S>(vx + off, p.lane, v);
+        }
+    }
 }
 
 struct RowCall {
@@ -272,31 +429,41 @@ struct RowCall {
     cudaStream_t st;
 };
 
-template <typename X, typename C, int HD>
+template <typename X, typename C, int HD, int R>
 int launch_rows(const RowCall& r) {
     const int64_t threads = (int64_t)r.b.n_tokens * r.b.n_kv * (HD / 8);
-    const int64_t grid64 = (threads + kRowThreads - 1) / kRowThreads;
-    FTC_REQUIRE(grid64 <= INT_MAX, FTC_E_UNSUPPORTED, "ftc_kv_pages: too many rows for one launch");
+    const int64_t grid64 = (threads + kRowThreads * R - 1) / (kRowThreads * R);
+    FTC_REQUIRE(threads <= INT_MAX - 65536, FTC_E_UNSUPPORTED,
+                "ftc_kv_pages: too many rows for one launch");
     const unsigned grid = (unsigned)grid64;
     C* kc = static_cast<C*>(r.c->k);
     C* vc = static_cast<C*>(r.c->v);
     X* k = static_cast<X*>(r.k);
     X* v = static_cast<X*>(r.v);
     if (r.write)
-        kv_pages_write_kernel<X, C, HD><<<grid, kRowThreads, 0, r.st>>>(
+        kv_pages_write_kernel<X, C, HD, R><<<grid, kRowThreads, 0, r.st>>>(
             r.b, k, v, r.stride, kc, vc, r.c->k_scale, r.c->v_scale);
     else
-        kv_pages_read_kernel<X, C, HD><<<grid, kRowThreads, 0, r.st>>>(
+        kv_pages_read_kernel<X, C, HD, R><<<grid, kRowThreads, 0, r.st>>>(
             r.b, k, v, r.stride, kc, vc, r.c->k_scale, r.c->v_scale);
     FTC_CUDA(cudaGetLastError());
     return FTC_OK;
 }
 
+// One piece a thread while that leaves SMs idle (latency counts), else four,
+// two of fp32 rows (bytes in flight count).
+template <typename X, typename C, int HD>
+int rows_pieces(const RowCall& r) {
+    const int64_t threads = (int64_t)r.b.n_tokens * r.b.n_kv * (HD / 8);
+    return threads < (int64_t)device_sms() * 2048 ? launch_rows<X, C, HD, 1>(r)
+                                                  : launch_rows<X, C, HD, sizeof(X) == 4 ? 2 : 4>(r);
+}
+
 template <typename X, typename C>
 int rows_hd(const RowCall& r) {
-    return r.c->head_dim == 64    ? launch_rows<X, C, 64>(r)
-           : r.c->head_dim == 128 ? launch_rows<X, C, 128>(r)
-                                  : launch_rows<X, C, 256>(r);
+    return r.c->head_dim == 64    ? rows_pieces<X, C, 64>(r)
+           : r.c->head_dim == 128 ? rows_pieces<X, C, 128>(r)
+                                  : rows_pieces<X, C, 256>(r);
 }
 
 template <typename X>

@@ -372,50 +372,68 @@ class PageBatch:
 
 
 class _PagedLaunch:
-    """Device guard and stream of a paged call: the current stream of the
-    cache's device unless one is given (a torch stream or its address)."""
+    """Device guard and stream of a paged call on another device than the
+    current one, or on a given stream (a torch stream or its address): buffers
+    made inside belong to the stream that the kernels run on."""
 
     def __init__(self, device, stream):
         import torch
-        self._guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index \
-            else None
-        self._given = stream
-        self._device = device
+        if stream is None:
+            stream = torch.cuda.current_stream(device)
+        elif isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream, device=device) if stream else \
+                torch.cuda.default_stream(device)
+        self.stream = stream.cuda_stream
+        self._guards = (torch.cuda.device(device), torch.cuda.stream(stream))
 
     def __enter__(self):
-        import torch
-        if self._guard is not None:
-            self._guard.__enter__()
-        if self._given is None:
-            self.stream, self.ctx = torch.cuda.current_stream(self._device).cuda_stream, None
-            return self
-        s = self._given
-        if isinstance(s, int):
-            s = torch.cuda.ExternalStream(s, device=self._device) if s else \
-                torch.cuda.default_stream(self._device)
-        # buffers made here belong to the stream that the kernels run on
-        self.stream, self.ctx = s.cuda_stream, torch.cuda.stream(s)
-        self.ctx.__enter__()
-        return self
+        for g in self._guards:
+            g.__enter__()
+        return self.stream
 
     def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+        for g in reversed(self._guards):
+            g.__exit__(*exc)
+
+
+class _HereLaunch:
+    """The same for the current stream of the current device: nothing to guard."""
+
+    def __init__(self, stream):
+        self.stream = stream
+
+    def __enter__(self):
+        return self.stream
+
+    def __exit__(self, *exc):
+        pass
+
+
+def _paged_launch(device, stream):
+    import torch
+    if stream is None and torch.cuda.current_device() == device.index:
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        return _HereLaunch(raw(device.index) if raw is not None
+                           else torch.cuda.current_stream(device).cuda_stream)
+    return _PagedLaunch(device, stream)
 
 
 def _paged_rows(x, pages, batch, width, what):
     """(FTC type, row stride) of rows [n_tokens, width] (or [n_tokens, heads,
     head_dim]); rows may be wider apart than they are long."""
-    if x.dim() == 3:
-        x = x.view(x.shape[0], x.shape[1] * x.shape[2])
-    if x.dtype not in _ROW_TYPES or x.dim() != 2 or x.shape[1] != width or \
-            x.shape[0] != batch.n_tokens or x.device != pages.device or \
-            (x.shape[0] and x.stride(1) != 1):
+    shape = x.shape
+    if len(shape) == 3:
+        x = x.view(shape[0], shape[1] * shape[2])
+        shape = x.shape
+    t = _ROW_TYPES.get(x.dtype)
+    if t is None or len(shape) != 2 or shape[1] != width or shape[0] != batch.n_tokens or \
+            x.device != pages.device:
         raise ValueError(f"{what}: rows must be [{batch.n_tokens}, {width}] float32, float16 or "
-                         "bfloat16 on the cache's device, values of a row next to each other")
-    return _ROW_TYPES[x.dtype], x.stride(0) if x.shape[0] > 1 else width
+                         "bfloat16 on the cache's device")
+    stride = x.stride()
+    if shape[0] and stride[1] != 1:
+        raise ValueError(f"{what}: the values of a row must lie next to each other")
+    return t, stride[0] if shape[0] > 1 else width
 
 
 def _paged_args(pages, batch, what):
@@ -429,12 +447,12 @@ def kv_pages_write(pages, k_new, v_new, batch, stream=None):
     (ftc_kv_pages_write)."""
     _paged_args(pages, batch, "kv_pages_write")
     width = pages.n_head_kv * pages.head_dim
-    t, ld = _paged_rows(k_new, pages, batch, width, "kv_pages_write")
-    if (t, ld) != _paged_rows(v_new, pages, batch, width, "kv_pages_write"):
+    rows = _paged_rows(k_new, pages, batch, width, "kv_pages_write")
+    if rows != _paged_rows(v_new, pages, batch, width, "kv_pages_write"):
         raise ValueError("kv_pages_write: k_new and v_new must have one type and row stride")
-    with _PagedLaunch(pages.device, stream) as on:
+    with _paged_launch(pages.device, stream) as st:
         check(lib().ftc_kv_pages_write(pages._ref, batch._ref, k_new.data_ptr(), v_new.data_ptr(),
-                                       t, ld, on.stream), "ftc_kv_pages_write")
+                                       *rows, st), "ftc_kv_pages_write")
 
 
 def kv_pages_read(pages, batch, k_out=None, v_out=None, out_dtype="F32", stream=None):
@@ -444,18 +462,22 @@ def kv_pages_read(pages, batch, k_out=None, v_out=None, out_dtype="F32", stream=
     torch = _torch_types()
     _paged_args(pages, batch, "kv_pages_read")
     width = pages.n_head_kv * pages.head_dim
-    with _PagedLaunch(pages.device, stream) as on:
-        if k_out is None or v_out is None:
-            if k_out is not None or v_out is not None:
-                raise ValueError("kv_pages_read: give both k_out and v_out, or none")
-            dt = getattr(torch, _TORCH_OUT[F.dtype_id(out_dtype)])
-            k_out = torch.empty((batch.n_tokens, width), dtype=dt, device=pages.device)
-            v_out = torch.empty_like(k_out)
-        t, ld = _paged_rows(k_out, pages, batch, width, "kv_pages_read")
-        if (t, ld) != _paged_rows(v_out, pages, batch, width, "kv_pages_read"):
-            raise ValueError("kv_pages_read: k_out and v_out must have one type and row stride")
+    with _paged_launch(pages.device, stream) as st:
+        if k_out is None and v_out is None:
+            t = F.dtype_id(out_dtype)
+            if t not in _TORCH_OUT:
+                raise ValueError('kv_pages_read: out_dtype must be "F32", "F16" or "BF16"')
+            k_out, v_out = torch.empty((2, batch.n_tokens, width), device=pages.device,
+                                       dtype=getattr(torch, _TORCH_OUT[t])).unbind(0)
+            rows = (t, width)
+        elif k_out is None or v_out is None:
+            raise ValueError("kv_pages_read: give both k_out and v_out, or none")
+        else:
+            rows = _paged_rows(k_out, pages, batch, width, "kv_pages_read")
+            if rows != _paged_rows(v_out, pages, batch, width, "kv_pages_read"):
+                raise ValueError("kv_pages_read: k_out and v_out must have one type and row stride")
         check(lib().ftc_kv_pages_read(pages._ref, batch._ref, k_out.data_ptr(), v_out.data_ptr(),
-                                      t, ld, on.stream), "ftc_kv_pages_read")
+                                      *rows, st), "ftc_kv_pages_read")
     return k_out, v_out
 
 
@@ -466,28 +488,29 @@ def attention_pages(q, n_head, pages, batch, window=0, n_sink=0, scale=None, out
     returns out of q's type.  ``window`` > 0: a row sees the last ``window``
     positions up to its own, and the first ``n_sink``.  ``scale`` defaults to
     1 / sqrt(head_dim).  ``ws``: uint8 workspace (allocated when None)."""
-    torch = _torch_types()
+    import torch
     _paged_args(pages, batch, "attention_pages")
     width = n_head * pages.head_dim
     t, ld = _paged_rows(q, pages, batch, width, "attention_pages")
     if scale is None:
         scale = pages.head_dim ** -0.5
-    with _PagedLaunch(pages.device, stream) as on:
+    with _paged_launch(pages.device, stream) as st:
         if out is None:
-            out = torch.empty((batch.n_tokens, width), dtype=q.dtype, device=pages.device)
-        to, ldo = _paged_rows(out, pages, batch, width, "attention_pages")
-        if to != t:
-            raise ValueError("attention_pages: out must have q's type")
-        need = lib().ftc_attention_pages_workspace_bytes(pages._ref, batch._ref, n_head, t)
-        if ws is None and need:
+            out, ldo = torch.empty((batch.n_tokens, width), dtype=q.dtype, device=pages.device), width
+        else:
+            to, ldo = _paged_rows(out, pages, batch, width, "attention_pages")
+            if to != t:
+                raise ValueError("attention_pages: out must have q's type")
+        if ws is None:
+            need = lib().ftc_attention_pages_workspace_bytes(pages._ref, batch._ref, n_head, t)
             ws = torch.empty(need, dtype=torch.uint8, device=pages.device)
-        if ws is not None and (ws.device != pages.device or not ws.is_contiguous()):
+        elif ws.device != pages.device or not ws.is_contiguous():
             raise ValueError("attention_pages: ws must be contiguous on the cache's device")
+        else:
+            need = ws.numel() * ws.element_size()
         check(lib().ftc_attention_pages(
             pages._ref, batch._ref, q.data_ptr(), t, ld, n_head, scale, window, n_sink,
-            out.data_ptr(), ldo, ws.data_ptr() if ws is not None else None,
-            ws.numel() * ws.element_size() if ws is not None else 0, on.stream),
-            "ftc_attention_pages")
+            out.data_ptr(), ldo, ws.data_ptr(), need, st), "ftc_attention_pages")
     return out
 
 
