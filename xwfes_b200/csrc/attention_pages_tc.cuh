@@ -376,8 +376,9 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
     grid_launch_dependents();
     __syncthreads();
 
-    const int64_t W = P::scan(a, sPre);
-    const int64_t L = plan_share(W, (int)gridDim.x, 1, least);
+    int64_t tiles;
+    const int64_t W = P::scan(a, sPre, tiles);
+    const int64_t L = plan_share(W, tiles, (int)gridDim.x, 1, least);
     const int64_t u0 = (int64_t)blockIdx.x * L;
     if (u0 >= W) {
         if (threadIdx.x == 0) a.cut[blockIdx.x].pieces = 0;

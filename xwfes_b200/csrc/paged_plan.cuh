@@ -104,13 +104,19 @@ struct Plan {
     }
 
     // Units before each sequence to pre[0 .. n_seqs) (shared memory), all
-    // units returned; every thread of the CTA calls it.
-    static __device__ int64_t scan(const PagedArgs& a, int64_t* pre) {
+    // units returned, and the tiles that they are of; every thread of the CTA
+    // calls it.
+    static __device__ int64_t scan(const PagedArgs& a, int64_t* pre, int64_t& n_tiles) {
         const int tid = threadIdx.x, nt = blockDim.x, warp = tid >> 5, lane = tid & 31;
+        unsigned long long* tiles = reinterpret_cast<unsigned long long*>(pre + kMaxSeqs + 1);
+        if (tid == 0) *tiles = 0;
+        __syncthreads();
+        int mine = 0;
         for (int s = tid; s < a.b.n_seqs; s += nt) {
             PlanPos p;
             p.s = s;
             load_seq(a, p);
+            mine += p.tiles;
             int64_t w = 0;
             if (p.tiles > 4) {
                 w = -1;  // a warp's work, below
@@ -119,6 +125,7 @@ struct Plan {
             }
             pre[s] = w;
         }
+        if (mine) atomicAdd(tiles, (unsigned long long)mine);
         __syncthreads();
         for (int s = warp; s < a.b.n_seqs; s += nt >> 5) {
             if (pre[s] >= 0) continue;
@@ -148,6 +155,7 @@ struct Plan {
             if (lane == 0) *total = sum;
         }
         __syncthreads();
+        n_tiles = (int64_t)*tiles * a.b.n_kv;
         return *total;
     }
 
@@ -204,11 +212,17 @@ struct Plan {
     }
 };
 
-// Units per CTA: an equal share of all, rounded up to `step`, at least
-// `least` (a shorter range costs more in joining than it saves).
-__device__ __forceinline__ int64_t plan_share(int64_t W, int G, int step, int least) {
+// Units per CTA: an equal share of all, rounded up to `step`.  A share below
+// `least` is raised to it (a shorter range costs more in joining than it
+// saves), but not past a tile: with little work, CTAs of their own for the
+// tiles beat one that takes several in turn (8 tiles of 60 positions: 21 us in
+// shares of four tiles, 10 us one by one).
+__device__ __forceinline__ int64_t plan_share(int64_t W, int64_t tiles, int G, int step,
+                                              int least) {
     const int64_t per = (W + G - 1) / G;
-    return max((per + step - 1) / step * step, (int64_t)least);
+    if (per >= least) return (per + step - 1) / step * step;
+    const int64_t tile = (W + tiles - 1) / max(tiles, (int64_t)1);
+    return max(per, min((int64_t)least, tile));
 }
 
 }  // namespace ftc
