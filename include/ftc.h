@@ -573,8 +573,8 @@ int ftc_kv_pages_read(const ftc_kv_pages* pages, const ftc_page_batch* batch, vo
                       void* v_out, int out_dtype, int64_t out_stride, void* stream);
 
 /* Bytes of workspace ftc_attention_pages needs (0: none, or bad arguments).
- * They depend on the device, the cache's and q's types and head layout and
- * n_tokens, not on the sequences. */
+ * They depend on the device, the cache's and q's types and head layout, n_seqs,
+ * n_tokens and max_new, not on the device arrays. */
 size_t ftc_attention_pages_workspace_bytes(const ftc_kv_pages* pages, const ftc_page_batch* batch,
                                            int64_t n_head, int q_dtype);
 

@@ -4,22 +4,31 @@
 //
 //   out = sum_j w_j v_j / sum_j w_j,  w_j = 2^(c q.k_j - M),  c = scale log2(e)
 // in one pass over the keys (running maximum M, running sum, the accumulator
-// rescaled when M grows).  A CTA is NW consumer warps and one producer warp.
-// The producer brings key chunks (KS positions of K and V, one box per page
-// and 128 bytes of head_dim, swizzled by TMA so that the matrix loads are free
-// of bank conflicts) into a ring of slots; a chunk of a page that is not
-// mapped is fetched out of bounds, which fills zeros.  A slot belongs to one
-// group of MW warps, warp i of the group taking packed rows 16 i .. 16 i + 15;
-// the groups take slots in turn, each with a softmax state of its own, and
-// meet only at a tile's end.  So decode (MW = 1, 16 packed rows) has 4
-// independent warps on one tile's keys, and chunks (MW = 4, 8) read each key
+// rescaled when M grows).  Both products are taken transposed, keys and then
+// dimensions as the 16 rows of an instruction (K and V are the A operands,
+// read with ldmatrix; q and the weights the B operands of 8 packed rows each),
+// so that a decode tile of one KV head's 4 or 8 query heads wastes little and
+// the weights go from one product to the next by movmatrix, in registers.
+//
+// A CTA is NW consumer warps and one producer warp.  The producer brings key
+// chunks (KS positions of K and V, one box per page and 128 bytes of head_dim,
+// swizzled by TMA so that the matrix loads are free of bank conflicts) into a
+// ring of slots; a chunk of a page that is not mapped is fetched out of bounds,
+// which fills zeros.  A slot belongs to one group of MW warps, warp i of the
+// group taking packed rows 8 NT i onwards; the groups take slots in turn, each
+// with a softmax state of its own, and meet only at a tile's end.  Decode (MW =
+// 1, 8 or 16 packed rows) has 4 independent warps on one tile's keys and its
+// next q prepared by the producer; chunks (MW = 4, 8: one group) read each key
 // once for 64 or 128 rows.
 //
-// Decode is bound by HBM: 2 (head_dim bytes) a position and KV head.  Why
-// matrix instructions for it: with 4 query heads on a KV head the CUDA cores
-// would need 8 multiply-adds a byte of cache, 1.5 times what they have at HBM
-// speed, and the 8-bit decode on top; as 16-row tiles the same work is a
-// fifth of the tensor rate.
+// Decode is bound by HBM: 2 (head_dim bytes) a position and KV head; 64
+// sequences of 100 to 16000 positions, 32 heads on 8, 8-bit: 203 us, 5.4 TB/s.
+// Why matrix instructions for it: with 4 query heads on a KV head the CUDA
+// cores would need 8 multiply-adds a byte of cache, 1.5 times what they have at
+// HBM speed, and the 8-bit decode on top.  A few sequences are bound by latency
+// (one of 517 positions: 17 us, the plan, a chunk and the join in turn), and
+// groups of 4 warps by it too: 40 fp32 rows over an f16 cache run at 1.2 TB/s,
+// 2.4 warps a scheduler, a third of the issue slots used.
 //
 // Types.  Operands are f16 for f16 and 8-bit caches, bf16 for bf16 caches; the
 // 8-bit codes are exact in f16 (byte -> 1024 + code + 128 in the mantissa, one

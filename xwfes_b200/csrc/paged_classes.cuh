@@ -11,9 +11,10 @@ namespace paged {
 template <typename X, int HD>
 constexpr bool kTc = sizeof(X) == 2 && HD < 256;
 
-// The class's shape elsewhere: 4 warps in turn on 8 rows and on 16, 4 warps
-// of 16 rows, and 8 warps of 16 rows (head_dim 256: 4, nine warps leave a
-// thread too few registers).
+// The class's shape elsewhere: 4 warps in turn on 8 rows and on 16, one group
+// of 4 warps of 16 rows, and of 8 (head_dim 256: 4, nine warps leave a thread
+// too few registers).  The tcgen05 kernel does not pay below 64 rows: 24 rows
+// of 8-bit cache 316 us there, 261 here; 16 rows 315 and 108.
 template <typename X, typename C, int HD, class Fn>
 auto with_class(int cls, Fn fn) {
     if (cls == 0) return fn((Cfg<X, C, HD, 1, 1, 4>*)nullptr);
