@@ -316,6 +316,16 @@ def test_attention_long_chunk(ftc, q, cache):
     attend(ftc, q, cache, 4, 1, 128, 64, [(700, 1500), (1, 800), (257, 257)], seed=10)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("q,cache", [("bf16", "bf16"), ("f16", "q8"), ("f16", "f16")])
+def test_attention_many_short_tiles(ftc, q, cache, hd):
+    """More tiles of a few chunks than the device has SMs: many short
+    sequences, and one prompt under a window."""
+    attend(ftc, q, cache, 32, 2, hd, 64,
+           [(16 - s % 3, 16 + (s * 389) % 1380) for s in range(80)], seed=hd)
+    attend(ftc, q, cache, 64, 4, hd, 16, [(641, 700)], window=200, sink=5, seed=hd + 1)
+
+
 @pytest.mark.parametrize("max_new", [0, 1])
 @pytest.mark.parametrize("q,cache", [("bf16", "q8"), ("f32", "f16")])
 def test_attention_does_not_lean_on_max_new(ftc, q, cache, max_new):

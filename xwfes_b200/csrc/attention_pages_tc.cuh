@@ -44,6 +44,11 @@
 namespace ftc {
 namespace paged {
 
+// Tiles of at most this many chunks are not cut when there is one for every
+// CTA: a cut tile's second start and its join cost more than an uneven share
+// (8191 rows under a window of 1024, 256 tiles of 10 chunks: 103 us cut, 90 whole).
+constexpr int kWholeTile = 12;
+
 template <typename X_, typename C_, int HD_>
 struct TcCfg {
     using X = X_;
@@ -377,15 +382,26 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
     __syncthreads();
 
     int64_t tiles;
-    const int64_t W = P::scan(a, sPre, tiles);
+    int largest;
+    const int64_t W = P::scan(a, sPre, tiles, largest);
     const int64_t L = plan_share(W, tiles, (int)gridDim.x, 1, least);
-    const int64_t u0 = (int64_t)blockIdx.x * L;
-    if (u0 >= W) {
+    int64_t u0 = min((int64_t)blockIdx.x * L, W), u1 = min(u0 + L, W);
+    if (largest <= kWholeTile && tiles >= gridDim.x) {  // the ranges go to the nearest tile edges
+        if (warp == 0) {
+            const int64_t e0 = P::nearest_edge(a, sPre, u0, W);
+            const int64_t e1 = P::nearest_edge(a, sPre, u1, W);
+            if (lane == 0) sPre[kMaxSeqs + 3] = e0, sPre[kMaxSeqs + 4] = e1;
+        }
+        __syncthreads();
+        u0 = sPre[kMaxSeqs + 3];
+        u1 = sPre[kMaxSeqs + 4];
+    }
+    if (u0 >= u1) {
         if (threadIdx.x == 0) a.cut[blockIdx.x].pieces = 0;
         if (a.second) grid_dependency_wait();
         return;
     }
-    const int total = (int)min(L, W - u0);
+    const int total = (int)(u1 - u0);
     if (warp == 0) {
         const PlanPos p = P::locate(a, sPre, u0);
         if (lane == 0) *sPos = p;

@@ -81,7 +81,7 @@ struct PlanPos {
 
 template <int TR, int KS>
 struct Plan {
-    static constexpr int kSmem = kMaxSeqs * 8 + 32;
+    static constexpr int kSmem = (kMaxSeqs + 5) * 8;  // sums, and five more words
 
     // The sequence's rows for this launch: 0 tiles when it is another's.
     static __device__ __forceinline__ void load_seq(const PagedArgs& a, PlanPos& p) {
@@ -92,26 +92,31 @@ struct Plan {
     }
 
     // Chunks of all tiles of one KV head of a sequence, lanes of a warp
-    // over the tiles.
+    // over the tiles; `most` grows to the largest tile that the lane sees.
     static __device__ __forceinline__ int64_t seq_chunks_warp(const PagedArgs& a,
-                                                              const PlanPos& p) {
+                                                              const PlanPos& p, int& most) {
         int64_t w = 0;
-        for (int t = threadIdx.x & 31; t < p.tiles; t += 32)
-            w += TileWork<TR, KS>(a, p.n, p.len, t).count;
+        for (int t = threadIdx.x & 31; t < p.tiles; t += 32) {
+            const int c = TileWork<TR, KS>(a, p.n, p.len, t).count;
+            w += c;
+            most = max(most, c);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
         return w;
     }
 
     // Units before each sequence to pre[0 .. n_seqs) (shared memory), all
-    // units returned, and the tiles that they are of; every thread of the CTA
-    // calls it.
-    static __device__ int64_t scan(const PagedArgs& a, int64_t* pre, int64_t& n_tiles) {
+    // units returned, the tiles that they are of and the largest tile's units;
+    // every thread of the CTA calls it.
+    static __device__ int64_t scan(const PagedArgs& a, int64_t* pre, int64_t& n_tiles,
+                                   int& largest) {
         const int tid = threadIdx.x, nt = blockDim.x, warp = tid >> 5, lane = tid & 31;
         unsigned long long* tiles = reinterpret_cast<unsigned long long*>(pre + kMaxSeqs + 1);
-        if (tid == 0) *tiles = 0;
+        int* top = reinterpret_cast<int*>(pre + kMaxSeqs + 2);
+        if (tid == 0) *tiles = 0, *top = 0;
         __syncthreads();
-        int mine = 0;
+        int mine = 0, most = 0;
         for (int s = tid; s < a.b.n_seqs; s += nt) {
             PlanPos p;
             p.s = s;
@@ -121,7 +126,11 @@ struct Plan {
             if (p.tiles > 4) {
                 w = -1;  // a warp's work, below
             } else {
-                for (int t = 0; t < p.tiles; ++t) w += TileWork<TR, KS>(a, p.n, p.len, t).count;
+                for (int t = 0; t < p.tiles; ++t) {
+                    const int c = TileWork<TR, KS>(a, p.n, p.len, t).count;
+                    w += c;
+                    most = max(most, c);
+                }
             }
             pre[s] = w;
         }
@@ -132,10 +141,11 @@ struct Plan {
             PlanPos p;
             p.s = s;
             load_seq(a, p);
-            const int64_t w = seq_chunks_warp(a, p);
+            const int64_t w = seq_chunks_warp(a, p, most);
             __syncwarp();
             if (lane == 0) pre[s] = w;
         }
+        if (most) atomicMax(top, most);
         __syncthreads();
         int64_t* total = pre + kMaxSeqs;
         if (warp == 0) {
@@ -156,6 +166,7 @@ struct Plan {
         }
         __syncthreads();
         n_tiles = (int64_t)*tiles * a.b.n_kv;
+        largest = *top;
         return *total;
     }
 
@@ -171,7 +182,8 @@ struct Plan {
         PlanPos p;
         p.s = lo;
         load_seq(a, p);
-        const int64_t per = p.tiles > 0 ? seq_chunks_warp(a, p) : 1;
+        int most = 0;
+        const int64_t per = p.tiles > 0 ? seq_chunks_warp(a, p, most) : 1;
         const int64_t rem = u - pre[lo];
         p.kvh = (int)(rem / per);
         int64_t left = rem - p.kvh * per;
@@ -196,6 +208,15 @@ struct Plan {
             left -= __shfl_sync(0xffffffffu, x, 31);
         }
         return p;
+    }
+
+    // The tile edge nearest to unit u of W (a whole warp calls it).
+    static __device__ int64_t nearest_edge(const PagedArgs& a, const int64_t* pre, int64_t u,
+                                           int64_t W) {
+        if (u >= W) return W;
+        const PlanPos p = locate(a, pre, u);
+        const int c = TileWork<TR, KS>(a, p.n, p.len, p.t).count;
+        return 2 * p.i < c ? u - p.i : u - p.i + c;
     }
 
     // To the first chunk of the next tile.
