@@ -84,9 +84,10 @@ struct JoinSet {
     const float2* stat;
     const float* part;
     int G, TR;
-    // a row per warp, or four in flight where tiles have many rows (256-row
-    // tiles, a prompt of 8191 under a window: 14 us instead of 30)
-    __host__ __device__ int rows_per_cta() const { return kJoinWarps * (TR >= 64 ? 4 : 1); }
+    // a row per warp, or four in flight where tiles have many rows and so few
+    // pieces (256-row tiles, a prompt of 8191 under a window, 14 us instead of
+    // 30; but a call of 64-row tiles in 5 pieces 115 us instead of 102)
+    __host__ __device__ int rows_per_cta() const { return kJoinWarps * (TR >= 128 ? 4 : 1); }
     __host__ __device__ int blocks() const { return (TR + rows_per_cta() - 1) / rows_per_cta(); }
 };
 
@@ -214,22 +215,24 @@ __device__ __forceinline__ void join_rows4(const JoinArgs& a, const JoinSet& s, 
         if (r + i < ct.rows) store_row<X, HD>(a, ct, r + i, acc[i], l[i]);
 }
 
-template <typename X, int HD>
+// kMany: a set has four rows a warp (the others keep the registers that it takes).
+template <typename X, int HD, bool kMany>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join(const JoinArgs a) {
     const int which = (int)blockIdx.x >= a.blocks0;
     const JoinSet& s = a.set[which];
     const int blk = blockIdx.x - (which ? a.blocks0 : 0);
-    const int b = blk / s.blocks(), rows = s.rows_per_cta() / kJoinWarps;
-    const int r = (blk - b * s.blocks()) * s.rows_per_cta() + (threadIdx.x >> 5) * rows;
+    const int rows = kMany ? s.rows_per_cta() / kJoinWarps : 1;
+    const int per = kMany ? s.blocks() : (s.TR + kJoinWarps - 1) / kJoinWarps;
+    const int b = blk / per, r = ((blk - b * per) * kJoinWarps + (threadIdx.x >> 5)) * rows;
     grid_dependency_wait();
     grid_launch_dependents();
     const CutTile ct = s.cut[b];
     if (ct.pieces == 0 || r >= ct.rows) return;
-    if (rows == 4 && ct.pieces <= 8) {
-        join_rows4<X, HD>(a, s, ct, b, r);
-    } else {  // lanes over the pieces' statistics
-        for (int i = 0; i < rows && r + i < ct.rows; ++i) join_row<X, HD>(a, s, ct, b, r + i);
+    if constexpr (kMany) {
+        if (rows == 4 && ct.pieces <= 8) return join_rows4<X, HD>(a, s, ct, b, r);
     }
+    // many pieces: lanes over their statistics
+    for (int i = 0; i < rows && r + i < ct.rows; ++i) join_row<X, HD>(a, s, ct, b, r + i);
 }
 
 template <typename X, int HD>
@@ -243,7 +246,9 @@ int launch_join(const JoinArgs& a, int blocks, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_join<X, HD>, a);
+    const bool many = a.set[0].rows_per_cta() > kJoinWarps || a.set[1].rows_per_cta() > kJoinWarps;
+    const cudaError_t e = many ? cudaLaunchKernelEx(&cfg, paged_join<X, HD, true>, a)
+                               : cudaLaunchKernelEx(&cfg, paged_join<X, HD, false>, a);
     if (e != cudaSuccess) return cuda_error(e, "launch paged_join");
     return FTC_OK;
 }

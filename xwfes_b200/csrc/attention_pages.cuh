@@ -396,7 +396,7 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
     // this CTA's share of the units
     int64_t tiles;
     int largest;
-    const int64_t W = P::scan(a, sPre, tiles, largest);
+    const int64_t W = P::template scan<false>(a, sPre, tiles, largest);
     const int64_t L = plan_share(W, tiles, (int)gridDim.x, NG, least);
     const int64_t u0 = (int64_t)blockIdx.x * L;
     if (u0 >= W) {

@@ -46,8 +46,9 @@ namespace paged {
 
 // Tiles of at most this many chunks are not cut when there is one for every
 // CTA: a cut tile's second start and its join cost more than an uneven share
-// (8191 rows under a window of 1024, 256 tiles of 10 chunks: 103 us cut, 90 whole).
-constexpr int kWholeTile = 12;
+// (256 tiles: of 10 chunks 103 us cut, 90 whole; of 16, 107 and 94; of 18, 129
+// and 113; of 5 to 32, 122 and 128).
+constexpr int kWholeTile = 20;
 
 template <typename X_, typename C_, int HD_>
 struct TcCfg {
@@ -383,7 +384,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
 
     int64_t tiles;
     int largest;
-    const int64_t W = P::scan(a, sPre, tiles, largest);
+    const int64_t W = P::template scan<true>(a, sPre, tiles, largest);
     const int64_t L = plan_share(W, tiles, (int)gridDim.x, 1, least);
     int64_t u0 = min((int64_t)blockIdx.x * L, W), u1 = min(u0 + L, W);
     if (largest <= kWholeTile && tiles >= gridDim.x) {  // the ranges go to the nearest tile edges

@@ -107,8 +107,9 @@ struct Plan {
     }
 
     // Units before each sequence to pre[0 .. n_seqs) (shared memory), all
-    // units returned, the tiles that they are of and the largest tile's units;
-    // every thread of the CTA calls it.
+    // units returned, the tiles that they are of and, when asked for, the
+    // largest tile's units; every thread of the CTA calls it.
+    template <bool kLargest>
     static __device__ int64_t scan(const PagedArgs& a, int64_t* pre, int64_t& n_tiles,
                                    int& largest) {
         const int tid = threadIdx.x, nt = blockDim.x, warp = tid >> 5, lane = tid & 31;
@@ -145,7 +146,7 @@ struct Plan {
             __syncwarp();
             if (lane == 0) pre[s] = w;
         }
-        if (most) atomicMax(top, most);
+        if (kLargest && most) atomicMax(top, most);
         __syncthreads();
         int64_t* total = pre + kMaxSeqs;
         if (warp == 0) {
@@ -166,7 +167,7 @@ struct Plan {
         }
         __syncthreads();
         n_tiles = (int64_t)*tiles * a.b.n_kv;
-        largest = *top;
+        largest = kLargest ? *top : 0;
         return *total;
     }
 
