@@ -316,6 +316,14 @@ def test_attention_long_chunk(ftc, q, cache):
     attend(ftc, q, cache, 4, 1, 128, 64, [(700, 1500), (1, 800), (257, 257)], seed=10)
 
 
+@pytest.mark.parametrize("q,cache", [("f32", "q8"), ("bf16", "bf16")])
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31, 2**40])
+def test_attention_widest_windows(ftc, q, cache, window):
+    """A window of all 31 bits, with rows before position 0 in the tile."""
+    attend(ftc, q, cache, 8, 2, 64, 16, [(40, 25), (3, 70), (1, 9)], window=window, sink=2**33,
+           seed=15)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("q,cache", [("bf16", "bf16"), ("f16", "q8"), ("f16", "f16")])
 def test_attention_many_short_tiles(ftc, q, cache, hd):

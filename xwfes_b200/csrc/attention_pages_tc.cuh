@@ -25,7 +25,7 @@
 //
 // What bounds it: per chunk and stage pair the tensor cores need 2048 clocks
 // at head_dim 128 and the exponentials, 16 a clock, as many; a chunk takes 2.4
-// times that (2048 bf16 rows of 32 heads on 16384 positions: 514 us, 1.0
+// times that (2048 bf16 rows of 32 heads on 16384 positions: 523 us, 0.98
 // PFLOP/s).  A stage's softmax (~2100 clocks) and its MMAs (a batch of 8 comes
 // back ~500 clocks after its last issue) stand one after the other, two stages
 // are what tensor memory holds, and the roles' code passes the SM's

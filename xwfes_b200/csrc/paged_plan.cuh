@@ -58,7 +58,8 @@ struct TileWork {
         p_last = len - n + r1 / a.gqa;
         const int cap = a.b.table_cols << a.b.page_shift;  // positions the table can name
         const int hi = min(p_last, cap - 1);
-        first = a.window > 0 ? max(p_first - a.window + 1, 0) / KS : 0;
+        // (rows before position 0 have no window; window may be INT_MAX)
+        first = a.window > 0 ? max(max(p_first, 0) - a.window + 1, 0) / KS : 0;
         n_sink_chunks = a.window > 0
                             ? min((int)(((int64_t)min(a.n_sink, hi + 1) + KS - 1) / KS), first)
                             : 0;
