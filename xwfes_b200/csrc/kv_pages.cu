@@ -7,7 +7,7 @@
 // tensors' loads in flight together, so a row of head_dim values is head_dim / 8
 // neighbouring lanes and its maximum is a shuffle reduction inside a warp.
 // Measured: 28004 rows of 8 KV heads of 128 read from 8 bits to fp32 49 us (5.9
-// TB/s); 8192 bf16 rows stored in 8 bits and read back, two launches, 31 us (2.7
+// TB/s); 8192 bf16 rows stored in 8 bits and read back, two launches, 28 us (3.0
 // TB/s); one row each of 48 sequences 5.6 us the pair.
 #include <cuda_bf16.h>
 
@@ -303,64 +303,55 @@ __device__ __forceinline__ uint2 quantise8(float (&x)[8], uint32_t top, float& d
     return make_uint2(bytes(q[0], q[1], q[2], q[3]), bytes(q[4], q[5], q[6], q[7]));
 }
 
-// C: cache element (__half, __nv_bfloat16 or int8_t), X: row element, R: pieces
-// per thread, kRowThreads apart.  The rows' loads are issued before the slots
-// are looked up (start, kv_len and the table hang on one another).
-template <typename X, typename C, int HD, int R>
+// C: cache element (__half, __nv_bfloat16 or int8_t), X: row element.  A
+// piece a thread; the rows' loads are issued before the slots are looked up
+// (start, kv_len and the table hang on one another).
+template <typename X, typename C, int HD>
 __global__ void __launch_bounds__(kRowThreads)
 kv_pages_write_kernel(const PageView b, const X* __restrict__ kx, const X* __restrict__ vx,
                       int64_t x_stride, C* kc, C* vc, float* ks, float* vs) {
     using S = Spread<X, HD>;
     constexpr int LANES = HD / 8;
-    const uint32_t g0 = blockIdx.x * (uint32_t)(kRowThreads * R);
-    Raw8<X> kr[R], vr[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const Piece<HD> p(b, g0 + i * kRowThreads + threadIdx.x);
-        if (p.t < b.n_tokens) {
-            const int64_t off = (int64_t)p.t * x_stride + (int64_t)p.h * HD;
-            kr[i] = load8<S>(kx + off, p.lane);
-            vr[i] = load8<S>(vx + off, p.lane);
-        } else {
-            kr[i] = {}, vr[i] = {};
-        }
+    const uint32_t g0 = blockIdx.x * (uint32_t)kRowThreads;
+    const Piece<HD> p(b, g0 + threadIdx.x);
+    Raw8<X> kr = {}, vr = {};
+    if (p.t < b.n_tokens) {
+        const int64_t off = (int64_t)p.t * x_stride + (int64_t)p.h * HD;
+        kr = load8<S>(kx + off, p.lane);
+        vr = load8<S>(vx + off, p.lane);
     }
-    const int s0 = first_seq(b, Piece<HD>(b, g0).t);
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const Piece<HD> p(b, g0 + i * kRowThreads + threadIdx.x);
-        const Slot at = find_slot(b, s0, p.t);
-        const int64_t row = (int64_t)p.h * b.page_size + at.slot;
-        const int64_t dst = at.page * b.page_stride + row * HD;
-        if constexpr (sizeof(C) == 1) {
-            float k[8], v[8], dk, dv;
-            floats(kr[i], k);
-            floats(vr[i], v);
-            const uint2 ck = quantise8<LANES>(k, top8(kr[i]), dk);
-            const uint2 cv = quantise8<LANES>(v, top8(vr[i]), dv);
-            if (at.page < 0) continue;
-            store_codes<S>(kc + dst, p.lane, ck);
-            store_codes<S>(vc + dst, p.lane, cv);
-            if (p.lane == 0) {
-                ks[at.page * b.scale_stride + row] = dk;
-                vs[at.page * b.scale_stride + row] = dv;
-            }
+    const Slot at = find_slot(b, first_seq(b, Piece<HD>(b, g0).t), p.t);
+    const int64_t row = (int64_t)p.h * b.page_size + at.slot;
+    const int64_t dst = at.page * b.page_stride + row * HD;
+    if constexpr (sizeof(C) == 1) {
+        float k[8], v[8], dk, dv;
+        floats(kr, k);
+        floats(vr, v);
+        const uint2 ck = quantise8<LANES>(k, top8(kr), dk);
+        const uint2 cv = quantise8<LANES>(v, top8(vr), dv);
+        if (at.page < 0) return;
+        store_codes<S>(kc + dst, p.lane, ck);
+        store_codes<S>(vc + dst, p.lane, cv);
+        if (p.lane == 0) {
+            ks[at.page * b.scale_stride + row] = dk;
+            vs[at.page * b.scale_stride + row] = dv;
+        }
+    } else {
+        if (at.page < 0) return;
+        if constexpr (std::is_same<X, C>::value) {
+            *reinterpret_cast<uint4*>(kc + dst + 8 * p.lane) = kr.w[0];
+            *reinterpret_cast<uint4*>(vc + dst + 8 * p.lane) = vr.w[0];
         } else {
-            if (at.page < 0) continue;
-            if constexpr (std::is_same<X, C>::value) {
-                *reinterpret_cast<uint4*>(kc + dst + 8 * p.lane) = kr[i].w[0];
-                *reinterpret_cast<uint4*>(vc + dst + 8 * p.lane) = vr[i].w[0];
-            } else {
-                float k[8], v[8];
-                floats(kr[i], k);
-                floats(vr[i], v);
-                store8<S>(kc + dst, p.lane, k);
-                store8<S>(vc + dst, p.lane, v);
-            }
+            float k[8], v[8];
+            floats(kr, k);
+            floats(vr, v);
+            store8<S>(kc + dst, p.lane, k);
+            store8<S>(vc + dst, p.lane, v);
         }
     }
 }
 
+// R: pieces per thread, kRowThreads apart.
 template <typename X, typename C, int HD, int R>
 __global__ void __launch_bounds__(kRowThreads)
 kv_pages_read_kernel(const PageView b, X* __restrict__ kx, X* __restrict__ vx, int64_t x_stride,
@@ -432,41 +423,40 @@ struct RowCall {
     cudaStream_t st;
 };
 
-template <typename X, typename C, int HD, int R>
+// Reads of 16-bit rows that fill the device have four pieces a thread in flight
+// (28004 rows from 8 bits 35 us, with one 39); fp32 rows (50 and 49 us), writes
+// (94 and 90) and small calls (4.7 and 3.5) take one.
+template <typename X, typename C, int HD>
 int launch_rows(const RowCall& r) {
     const int64_t threads = (int64_t)r.b.n_tokens * r.b.n_kv * (HD / 8);
-    const int64_t grid64 = (threads + kRowThreads * R - 1) / (kRowThreads * R);
     FTC_REQUIRE(threads <= INT_MAX - 65536, FTC_E_UNSUPPORTED,
                 "ftc_kv_pages: too many rows for one launch");
-    const unsigned grid = (unsigned)grid64;
+    auto grid = [&](int pieces) {
+        return (unsigned)((threads + kRowThreads * pieces - 1) / (kRowThreads * pieces));
+    };
     C* kc = static_cast<C*>(r.c->k);
     C* vc = static_cast<C*>(r.c->v);
     X* k = static_cast<X*>(r.k);
     X* v = static_cast<X*>(r.v);
+    constexpr int R = sizeof(X) == 2 ? 4 : 1;
     if (r.write)
-        kv_pages_write_kernel<X, C, HD, R><<<grid, kRowThreads, 0, r.st>>>(
+        kv_pages_write_kernel<X, C, HD><<<grid(1), kRowThreads, 0, r.st>>>(
+            r.b, k, v, r.stride, kc, vc, r.c->k_scale, r.c->v_scale);
+    else if (R == 1 || threads < (int64_t)device_sms() * 2048)
+        kv_pages_read_kernel<X, C, HD, 1><<<grid(1), kRowThreads, 0, r.st>>>(
             r.b, k, v, r.stride, kc, vc, r.c->k_scale, r.c->v_scale);
     else
-        kv_pages_read_kernel<X, C, HD, R><<<grid, kRowThreads, 0, r.st>>>(
+        kv_pages_read_kernel<X, C, HD, R><<<grid(R), kRowThreads, 0, r.st>>>(
             r.b, k, v, r.stride, kc, vc, r.c->k_scale, r.c->v_scale);
     FTC_CUDA(cudaGetLastError());
     return FTC_OK;
 }
 
-// One piece a thread while that leaves SMs idle (latency counts), else four,
-// two of fp32 rows (bytes in flight count).
-template <typename X, typename C, int HD>
-int rows_pieces(const RowCall& r) {
-    const int64_t threads = (int64_t)r.b.n_tokens * r.b.n_kv * (HD / 8);
-    return threads < (int64_t)device_sms() * 2048 ? launch_rows<X, C, HD, 1>(r)
-                                                  : launch_rows<X, C, HD, sizeof(X) == 4 ? 2 : 4>(r);
-}
-
 template <typename X, typename C>
 int rows_hd(const RowCall& r) {
-    return r.c->head_dim == 64    ? rows_pieces<X, C, 64>(r)
-           : r.c->head_dim == 128 ? rows_pieces<X, C, 128>(r)
-                                  : rows_pieces<X, C, 256>(r);
+    return r.c->head_dim == 64    ? launch_rows<X, C, 64>(r)
+           : r.c->head_dim == 128 ? launch_rows<X, C, 128>(r)
+                                  : launch_rows<X, C, 256>(r);
 }
 
 template <typename X>
