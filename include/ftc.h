@@ -584,7 +584,11 @@ size_t ftc_attention_pages_workspace_bytes(const ftc_kv_pages* pages, const ftc_
  * is mapped, and, with window > 0, p - j < window or j < n_sink (the first
  * n_sink positions stay visible).  Scores are scale * q . k, a row that sees
  * nothing gives zeros, and what stands at positions that a row does not see
- * (NaN, infinities) does not reach it.  q and out: [n_tokens][stride] of
+ * (NaN, infinities, values of any size) does not reach it.  Over an 8-bit
+ * cache a row's weights times V's scales are 16-bit floats relative to the
+ * largest product that the row's weights and the scales it sees allow: what is
+ * below 2^-31 of that (F32 q: 2^-38) counts as zero, and V above 2^100 in
+ * magnitude also costs the sum of weights its smallest terms.  q and out: [n_tokens][stride] of
  * q_dtype, head h at h * head_dim; query head h reads KV head
  * h / (n_head / n_head_kv).  q_dtype is FTC_F32 with any cache, or FTC_F16
  * with an FTC_F16 or FTC_KV_Q8 cache, or FTC_BF16 with an FTC_BF16 or

@@ -1,0 +1,119 @@
+"""Paged attention on the GPU where hidden positions hold anything that a float
+can be: every row stays within a bound that counts what the row sees alone."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import pages_ref as R  # noqa: E402
+import pages_seen as V  # noqa: E402
+from test_pages_gpu import (TYPES, agree, fill, ftc, gen, make_batch,  # noqa: E402,F401
+                            make_pages)
+
+Q8 = [("f32", "q8"), ("f16", "q8"), ("bf16", "q8")]
+
+
+def attend(ftc, q, cache, nh, nkv, hd, page, seqs, window=0, sink=0, seed=0, gain=1.5, edit=None,
+           spare=0):
+    """One call on random keys and values after ``edit(pages, table)``, with its
+    rows held to the bound; ``spare``: pages that belong to no sequence."""
+    g = gen(seed)
+    n_pages = sum(max(0, -(-length // page)) for _, length in seqs) + spare
+    pages = make_pages(ftc, cache, max(n_pages, 1), nkv, page, hd, g)
+    batch, start, lens, table = make_batch(ftc, seqs, page, max(n_pages, 1), g)
+    fill(pages, table, lens, g, gain)
+    if edit:
+        edit(pages, table)
+    x = torch.randn((batch.n_tokens, nh * hd), generator=g, device="cuda").to(TYPES[q])
+    got = ftc.attention_pages(x, nh, pages, batch, window=window, n_sink=sink)
+    torch.cuda.synchronize()
+    assert ftc.device_status() == 0
+    want, bound = V.attention(x, nh, pages, table, start, lens, window, sink)
+    agree(got, want, bound, list(range(batch.n_tokens)))
+    return got, want
+
+
+# sequences whose packed rows (4 query heads a KV head) are 4, 12, 40 and 360
+KINDS = {"decode": [(1, 500), (1, 131)], "verify": [(3, 500), (3, 131)],
+         "few": [(10, 500), (10, 131)], "chunk": [(90, 700), (90, 190)]}
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("junk", [1e3, 2.0 ** 20, 2.0 ** 31, 2.0 ** 40, 1e30])
+@pytest.mark.parametrize("q,cache", Q8)
+def test_scales_before_the_window(ftc, q, cache, junk, kind, page):
+    """8-bit codes of 127 with a large finite scale at every position between
+    the sinks and the oldest window of a call, the pages there all one page
+    that was never written."""
+    window, sink, seqs = 100, 5, KINDS[kind]
+    spare = []
+
+    def edit(pages, table):
+        junk_page = next(p for p in range(pages.k.shape[0])
+                         if not (table == p).any())
+        spare.append(junk_page)
+        for name in ("k", "v"):
+            getattr(pages, name)[junk_page] = 127
+            getattr(pages, name + "_scale")[junk_page] = junk
+        for s, (n, length) in enumerate(seqs):
+            first = length - n - window + 1  # the oldest position that a row's window holds
+            for j in range(sink, first):
+                c = j // page
+                if c * page >= sink and (c + 1) * page <= first:
+                    table[s, c] = junk_page
+                    continue
+                for name in ("k", "v"):
+                    getattr(pages, name)[int(table[s, c]), :, j % page] = 127
+                    getattr(pages, name + "_scale")[int(table[s, c]), :, j % page] = junk
+    attend(ftc, q, cache, 8, 2, 64, page, seqs, window=window, sink=sink, edit=edit, seed=71,
+           spare=1)
+    assert spare
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["verify", "few", "chunk"])
+@pytest.mark.parametrize("junk", [2.0 ** 20, 2.0 ** 31, 2.0 ** 40, 1e30])
+@pytest.mark.parametrize("q,cache", [("f32", "q8"), ("bf16", "q8")])  # f16 cannot hold the results
+def test_scales_of_later_tokens(ftc, q, cache, junk, kind, hd):
+    """The values of a call's later tokens grow from one to the next: no row
+    loses anything to the tokens after it in its tile."""
+    seqs = KINDS[kind]
+
+    def edit(pages, table):
+        for s, (n, length) in enumerate(seqs):
+            for i in range(n // 3, n):
+                j = length - n + i
+                gain = junk ** ((i - n // 3 + 1) / (n - n // 3))
+                pages.v_scale[int(table[s, j // 16]), :, j % 16] *= gain
+    attend(ftc, q, cache, 8, 2, hd, 16, seqs, edit=edit, seed=73 + hd)
+
+
+@pytest.mark.parametrize("q", ["f32", "bf16"])
+def test_two_tokens(ftc, q):
+    """The first of two tokens has its own value back, whatever the second's is."""
+    def edit(pages, table):
+        pages.v_scale[int(table[0, 0]), :, 1] *= 2.0 ** 40
+    got, want = attend(ftc, q, "q8", 4, 1, 128, 16, [(2, 2)], edit=edit, seed=79)
+    assert (got[0].abs().amax() > 0.1) and math.isfinite(float(want.abs().max()))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["verify", "few", "chunk"])
+@pytest.mark.parametrize("junk", [2.0 ** 20, 2.0 ** 31, 2.0 ** 40, 1e30])
+@pytest.mark.parametrize("q,cache", [("f32", "q8"), ("bf16", "q8")])
+def test_scales_that_leave_the_window(ftc, q, cache, junk, kind, hd):
+    """Large values at the oldest positions of a call's windows, so that its
+    first rows see them and its last rows do not."""
+    window, seqs = 80, KINDS[kind]
+
+    def edit(pages, table):
+        for s, (n, length) in enumerate(seqs):
+            oldest = length - n - window + 1
+            for i in range(n // 2):
+                j = oldest + i
+                gain = junk ** (1 - i / n)
+                pages.v_scale[int(table[s, j // 16]), :, j % 16] *= gain
+    attend(ftc, q, cache, 8, 2, hd, 16, seqs, window=window, edit=edit, seed=83 + hd)

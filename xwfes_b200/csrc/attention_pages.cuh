@@ -37,8 +37,8 @@
 // f16 with a power-of-two scale per row; an fp32 q is 2 f16 pieces (scaled the
 // same way, 2^-22 kept) or 3 bf16 pieces.  Weights: fp32 q also splits them
 // (2 or 3 pieces), else they are rounded once to the operand type, 2^14 up in
-// f16 (and V's scale relative to its running maximum) so that weights 2^-38 of
-// the largest still count.  With fp32 q the matrix unit's own accumulation,
+// f16 (and V's scale relative to the running maximum of those that the row
+// sees, 2^E) so that weights 2^-38 of the largest still count.  With fp32 q the matrix unit's own accumulation,
 // which truncates, is kept to short chains that fp32 adds join.
 #pragma once
 
@@ -530,16 +530,20 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
         const int p_lo = p.len - p.n + pr / a.gqa;
         const int p_hi = wrows > 0 ? p.len - p.n + (pr + wrows - 1) / a.gqa : -1;
 
+        constexpr float kLeastE = -100.f;  // weights 2^(14 - E) fit fp32
         float O[DT][NT][4];  // dimensions g, g + 8 of a tile by rows 2 t4, 2 t4 + 1
         float M[NT][2], l[NT][2];
+        // 8-bit V: weights times scales, and with them both sums, are held
+        // relative to 2^E, the largest scale that this row sees
+        float E[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             M[n][0] = M[n][1] = -INFINITY;
             l[n][0] = l[n][1] = 0.f;
+            E[n][0] = E[n][1] = kLeastE;
 #pragma unroll
             for (int d = 0; d < DT; ++d) O[d][n][0] = O[d][n][1] = O[d][n][2] = O[d][n][3] = 0.f;
         }
-        int E = -126;  // 8-bit V: the accumulator's unit is 2^E
 
         for (int j = grp; j < m; j += NG) {
             const uint32_t k = it + j;
@@ -621,10 +625,11 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
 
             // ---- the 8-bit scales of this lane's keys, 16 kt + g and + 8
             float vsc[KT][2];
-            float mul = 1.f;  // what E's growth does to the accumulator
+            float Ec[NT][2];  // of this chunk
             if constexpr (F::kQ8) {
                 const float* ksc = sScale + (s * 2) * KS;
-                uint32_t top = 0;
+                auto exponent = [](uint32_t bits) { return (float)((int)(bits >> 23) - 126); };
+                uint32_t sb[KT][2];
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -637,22 +642,38 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                             S[kt][n][2 * h] *= kf;
                             S[kt][n][2 * h + 1] *= kf;
                         }
-                        // (hidden slots may hold anything)
-                        uint32_t b = __float_as_uint(fabsf(vsc[kt][h]));
-                        if (!whole && !(((flag >> (kk / (KS / 2))) & 1) && key0 + kk <= p_hi &&
-                                        b < 0x7F800000u))
-                            b = 0;
-                        top = max(top, b);
+                        sb[kt][h] = __float_as_uint(fabsf(vsc[kt][h]));
+                        if (sb[kt][h] >= 0x7F800000u) sb[kt][h] = 0;
                     }
-                top = __reduce_max_sync(0xffffffffu, top);
-                const int Ek = min(max((int)(top >> 23) - 126, -126), 126);
-                if (Ek > E) {
-                    mul = E - Ek < -126 ? 0.f : pow2(E - Ek);
-                    E = Ek;
-                }
-                const float f = pow2(-E);
+                if (whole) {
+                    uint32_t t = 0;
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) vsc[kt][0] *= f, vsc[kt][1] *= f;
+                    for (int kt = 0; kt < KT; ++kt) t = max(t, max(sb[kt][0], sb[kt][1]));
+                    const float x = exponent(__reduce_max_sync(0xffffffffu, t));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) Ec[n][0] = Ec[n][1] = x;
+                } else {
+                    // (a slot hidden from a row may hold any scale)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint32_t t = 0;
+#pragma unroll
+                            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const int kk = 16 * kt + 8 * h + g;
+                                    if (((flag >> (kk / (KS / 2))) & 1) &&
+                                        vis(key0 + kk, pos[n][e]))
+                                        t = max(t, sb[kt][h]);
+                                }
+                            t = max(t, __shfl_xor_sync(0xffffffffu, t, 4));
+                            t = max(t, __shfl_xor_sync(0xffffffffu, t, 8));
+                            t = max(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                            Ec[n][e] = exponent(t);
+                        }
+                }
             }
 
             // ---- softmax: new maxima, weights (2^14 up in f16), sums
@@ -688,9 +709,16 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                     const float N = fmaxf(M[n][e], mx * c[n][e]);
                     const float R = N == -INFINITY ? 0.f : N;
-                    al[n][e] = ex2(M[n][e] - R);  // 0 while M is -inf
+                    al[n][e] = M[n][e] - R;
                     M[n][e] = N;
                     D[n][e] = kUp - R;
+                    if constexpr (F::kQ8) {
+                        const float En = fmaxf(E[n][e], Ec[n][e]);
+                        al[n][e] += E[n][e] - En;
+                        D[n][e] -= En;
+                        E[n][e] = En;
+                    }
+                    al[n][e] = ex2(al[n][e]);  // 0 while M is -inf
                 }
             uint32_t pb[KT][NT][NP][2];  // weights as B operand: keys by rows
 #pragma unroll
@@ -718,10 +746,7 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                         for (int q = 0; q < NP; ++q) pb[kt][n][q][h] = movm_t(x[q]);
                     }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    l[n][e] = fmaf(l[n][e], al[n][e], sum[e]);
-                    if constexpr (F::kQ8) al[n][e] *= mul;
-                }
+                for (int e = 0; e < 2; ++e) l[n][e] = fmaf(l[n][e], al[n][e], sum[e]);
             }
 
             // ---- weighted V, dimensions by rows: V is the A operand.  16-bit
@@ -852,13 +877,9 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
 
         // ---- join the groups, halving their number per round
         if constexpr (F::kQ8) {
-            const float f = pow2(E);
+            // (sums stand relative to 2^(M + E) from here on)
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) O[d][n][i] *= f;
+            for (int n = 0; n < NT; ++n) M[n][0] += E[n][0], M[n][1] += E[n][1];
         }
         if constexpr (NG > 1) {
             constexpr int PER = F::PER;

@@ -21,7 +21,8 @@
 // V elements that are not finite out (0 x inf would reach every row), which the
 // rows that see them get back at the end; between tiles each fetches the q rows
 // of a stage.  8-bit scales stay in fp32: K's multiplies S, V's multiplies P,
-// relative to its running maximum 2^E.
+// relative to the running maximum 2^E of those that the row sees (in a chunk
+// that some row does not see whole, each thread looks over its own row's).
 //
 // What bounds it: per chunk and stage pair the tensor cores need 2048 clocks
 // at head_dim 128 and the exponentials, 16 a clock, as many; a chunk takes 2.4
@@ -775,16 +776,33 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                     const float mx = max3n(max3n(m4[0], m4[1], m4[2]), m4[3], m4[3]) * c;
                     int Et = E;
                     if constexpr (F::kQ8) {
-                        // V's largest scale in this chunk, of positions some row may see
-                        const float4 v4 = vsc[lane];
-                        const int n = ((flag >> (lane / 4)) & 1) ? tw.p_last - key0 - 4 * lane : -1;
-                        auto bits = [&](float v, int at) {
+                        // V's largest finite scale of the positions that this row sees
+                        // (a hidden position may hold any): in a whole chunk of all
+                        uint32_t top = 0;
+                        auto take = [&](float v, bool on) {
                             const uint32_t b = __float_as_uint(fabsf(v));
-                            return at <= n && b < 0x7F800000u ? b : 0u;
+                            if (on && b < 0x7F800000u) top = max(top, b);
                         };
-                        const uint32_t top = __reduce_max_sync(
-                            0xffffffffu, max(max(bits(v4.x, 0), bits(v4.y, 1)),
-                                             max(bits(v4.z, 2), bits(v4.w, 3))));
+                        if (whole) {
+                            const float4 v4 = vsc[lane];
+                            take(v4.x, true), take(v4.y, true);
+                            take(v4.z, true), take(v4.w, true);
+                            top = __reduce_max_sync(0xffffffffu, top);
+                        } else {
+#pragma unroll 1
+                            for (int q = 0; q < 4; ++q) {
+                                const uint32_t seen =
+                                    seen_bits(a, pos, key0 + 32 * q, flag >> (2 * q));
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const float4 v4 = vsc[8 * q + i];
+                                    take(v4.x, (seen >> (4 * i)) & 1);
+                                    take(v4.y, (seen >> (4 * i)) & 2);
+                                    take(v4.z, (seen >> (4 * i)) & 4);
+                                    take(v4.w, (seen >> (4 * i)) & 8);
+                                }
+                            }
+                        }
                         Et = max(E, min((int)(top >> 23) - 126, 126));
                     }
                     if (__any_sync(0xffffffffu, mx > M + 8.f || Et > E)) {
