@@ -117,3 +117,26 @@ def test_scales_that_leave_the_window(ftc, q, cache, junk, kind, hd):
                 gain = junk ** (1 - i / n)
                 pages.v_scale[int(table[s, j // 16]), :, j % 16] *= gain
     attend(ftc, q, cache, 8, 2, hd, 16, seqs, window=window, edit=edit, seed=83 + hd)
+
+
+@pytest.mark.parametrize("n", [1, 3, 10, 90])
+@pytest.mark.parametrize("q,cache", Q8)
+def test_visible_value_row_that_is_not_a_number(ftc, q, cache, n):
+    """A row of V that was stored as NaN makes the rows that see it NaN, also where
+    its weight is too small for fp32; the rows before it stay as they are."""
+    length = 30 + n
+    pos = length - n // 2 - 1
+
+    g = gen(89)
+    pages = make_pages(ftc, cache, 10, 1, 16, 64, g)
+    batch, start, lens, table = make_batch(ftc, [(n, length)], 16, 10, g)
+    fill(pages, table, lens, g, 1.0)
+    p, slot = int(table[0, pos // 16]), pos % 16
+    pages.k[p, 0, slot], pages.k_scale[p, 0, slot] = -127, 1.0
+    pages.v_scale[p, 0, slot] = math.nan
+    x = torch.ones((n, 4 * 64), device="cuda").to(TYPES[q])  # the position's score: -1016
+    got = ftc.attention_pages(x, 4, pages, batch)
+    want, bound = V.attention(x, 4, pages, table, start, lens)
+    agree(got, want, bound, list(range(n)))
+    sees = torch.arange(length - n, length, device="cuda") >= pos
+    assert torch.isnan(got[sees]).all() and torch.isfinite(got[~sees]).all() and sees.any()

@@ -38,8 +38,9 @@
 // same way, 2^-22 kept) or 3 bf16 pieces.  Weights: fp32 q also splits them
 // (2 or 3 pieces), else they are rounded once to the operand type, 2^14 up in
 // f16 (and V's scale relative to the running maximum of those that the row
-// sees, 2^E) so that weights 2^-38 of the largest still count.  With fp32 q the matrix unit's own accumulation,
-// which truncates, is kept to short chains that fp32 adds join.
+// sees, 2^E) so that weights 2^-38 of the largest still count.  With fp32 q the
+// matrix unit's own accumulation, which truncates, is kept to short chains that
+// fp32 adds join.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -732,13 +733,11 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const float sv = S[kt][n][2 * h + e];
-                            w[e] = ex2(fmaf(sv, c[n][e], D[n][e]));
-                            if (!whole && __float_as_uint(sv) == 0xFFFFDEADu) w[e] = 0.f;
+                            const bool hid = !whole && __float_as_uint(sv) == 0xFFFFDEADu;
+                            w[e] = hid ? 0.f : ex2(fmaf(sv, c[n][e], D[n][e]));
                             sum[e] += w[e];
-                            if constexpr (F::kQ8) {
-                                const float v = w[e] * vsc[kt][h];
-                                w[e] = !whole && w[e] == 0.f ? 0.f : v;
-                            }
+                            // (a scale that is not finite reaches who sees it at any weight)
+                            if constexpr (F::kQ8) w[e] = hid ? 0.f : w[e] * vsc[kt][h];
                         }
                         uint32_t x[NP];
                         split<OT, NP>(w[0], w[1], x);
