@@ -584,7 +584,9 @@ size_t ftc_attention_pages_workspace_bytes(const ftc_kv_pages* pages, const ftc_
  * is mapped, and, with window > 0, p - j < window or j < n_sink (the first
  * n_sink positions stay visible).  Scores are scale * q . k, a row that sees
  * nothing gives zeros, and what stands at positions that a row does not see
- * (NaN, infinities, values of any size) does not reach it.  Over an 8-bit
+ * (NaN, infinities, values of any size) does not reach it.  A key that is
+ * infinite is a score of +inf (its rows are NaN) or of -inf (it has no weight;
+ * a row with no other score is NaN).  Over an 8-bit
  * cache a row's weights times V's scales are 16-bit floats relative to the
  * largest product that the row's weights and the scales it sees allow: what is
  * below 2^-31 of that (F32 q: 2^-38) counts as zero, and V above 2^100 in

@@ -36,6 +36,7 @@ def attention(q, n_head, pages, table, start, kv_len, window=0, n_sink=0, scale=
         at = [x for x in at if x[1] >= 0]
         if not at:
             out[start[s]:start[s + 1]] = 0
+            bound[start[s]:start[s + 1]] = 1e-30
             continue
         j = torch.tensor([x[0] for x in at], device=q.device)
         ids = torch.tensor([x[1] for x in at], device=q.device)

@@ -140,3 +140,49 @@ def test_visible_value_row_that_is_not_a_number(ftc, q, cache, n):
     agree(got, want, bound, list(range(n)))
     sees = torch.arange(length - n, length, device="cuda") >= pos
     assert torch.isnan(got[sees]).all() and torch.isfinite(got[~sees]).all() and sees.any()
+
+
+WIDE = [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")]
+
+
+@pytest.mark.parametrize("n", [1, 3, 10, 90])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+@pytest.mark.parametrize("q,cache", WIDE)
+def test_visible_key_infinity(ftc, q, cache, bad, n):
+    """A key element that overflowed its type: a score of -inf has no weight, one of
+    +inf makes its row NaN, in chunks that every row sees whole and in others."""
+    if (q, cache, n) == ("f32", "bf16", 10):
+        n = 20  # 80 packed rows
+    length = 300 + n
+
+    def edit(pages, table):
+        for pos, d in ((70, 3), (length - n // 2 - 1, 5)):
+            pages.k[int(table[0, pos // 16]), 0, pos % 16, d] = bad
+    got, want = attend(ftc, q, cache, 4, 1, 64, 16, [(n, length)], edit=edit, seed=97)
+    # (every score at position 70 is infinite)
+    heads = got.view(n, 4, 64)
+    assert torch.equal(torch.isnan(heads).all(-1), torch.isnan(heads).any(-1))
+    assert n == 1 or (torch.isnan(heads).any() and torch.isfinite(heads).any())
+
+
+@pytest.mark.parametrize("n", [1, 3, 10, 90])
+@pytest.mark.parametrize("q,cache", WIDE)
+def test_scores_of_minus_infinity_alone(ftc, q, cache, n):
+    """A row whose visible scores are all -inf has no weights: NaN.  It is no row that
+    sees nothing, which gives zeros."""
+    if (q, cache, n) == ("f32", "bf16", 10):
+        n = 20
+    g = gen(101)
+    pages = make_pages(ftc, cache, 30, 1, 16, 64, g)
+    seqs = [(n, n + 130), (n, n // 2)]
+    batch, start, lens, table = make_batch(ftc, seqs, 16, 30, g)
+    fill(pages, table, lens, g)
+    x = torch.randn((2 * n, 4 * 64), generator=g, device="cuda").to(TYPES[q])
+    x.view(2 * n, 4, 64)[:, :, 7] = 1.0
+    for j in range(lens[0] - n // 2):
+        pages.k[int(table[0, j // 16]), 0, j % 16, 7] = -math.inf
+    got = ftc.attention_pages(x, 4, pages, batch)
+    want, bound = V.attention(x, 4, pages, table, start, lens)
+    agree(got, want, bound, list(range(2 * n)))
+    assert torch.isnan(got[:n - n // 2]).all() and torch.isfinite(got[n - n // 2:n]).all()
+    assert (got[n:2 * n - n // 2] == 0).all() and torch.isfinite(got[n:]).all()

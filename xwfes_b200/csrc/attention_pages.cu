@@ -99,15 +99,16 @@ struct JoinArgs {
     int gqa;
 };
 
-// The lane's dimensions of a joined row, divided by its sum of weights.
+// The lane's dimensions of a joined row, divided by its sum of weights (no
+// maximum: the row sees nothing).
 template <typename X, int HD>
 __device__ __forceinline__ void store_row(const JoinArgs& a, const CutTile& ct, int r,
-                                          const float* acc, float l) {
+                                          const float* acc, float M, float l) {
     constexpr int E = HD / 32;
     const int pr = ct.r0 + r, t = pr / a.gqa, h = ct.kvh * a.gqa + pr - t * a.gqa;
     X* o = static_cast<X*>(a.out) + (int64_t)(ct.row + t) * a.out_stride + (int64_t)h * HD +
            E * (threadIdx.x & 31);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = M == -INFINITY && l == l ? 0.f : 1.f / l;
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
         if constexpr (sizeof(X) == 4)
@@ -173,7 +174,7 @@ __device__ __forceinline__ void join_row(const JoinArgs& a, const JoinSet& s, co
             }
         }
     }
-    store_row<X, HD>(a, ct, r, acc, l);
+    store_row<X, HD>(a, ct, r, acc, M, l);
 }
 
 // Rows r to r + 3 at once, for few pieces: their loads in flight together, the
@@ -212,7 +213,7 @@ __device__ __forceinline__ void join_rows4(const JoinArgs& a, const JoinSet& s, 
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (r + i < ct.rows) store_row<X, HD>(a, ct, r + i, acc[i], l[i]);
+        if (r + i < ct.rows) store_row<X, HD>(a, ct, r + i, acc[i], M[i], l[i]);
 }
 
 // kMany: a set has four rows a warp (the others keep the registers that it takes).

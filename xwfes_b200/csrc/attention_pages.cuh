@@ -45,6 +45,7 @@
 
 #include <cuda_bf16.h>
 
+#include <cfloat>
 #include <type_traits>
 
 #include "paged_plan.cuh"
@@ -270,6 +271,22 @@ struct Vis {
         return key <= p && (window == 0 || p - key < window || key < n_sink);
     }
 };
+
+// Whether a row at `pos` sees a position of chunks p.i to p.i + m - 1 of its
+// tile (for rows that end without a maximum: the loop over keys has no part
+// in it).
+template <int KS, class Tile>
+__device__ __noinline__ bool sees_any(const PagedArgs& a, const PlanPos& p, const Tile& tw, int m,
+                                      int pos) {
+    for (int j = 0; j < m; ++j) {
+        const int key0 = tw.key0(p.i + j);
+        for (int k = key0; k < key0 + KS && k <= pos; k += 16)
+            if ((a.window == 0 || pos - min(k + 15, pos) < a.window || k < a.n_sink) &&
+                page_of(a.b, p.s, k) >= 0)
+                return true;
+    }
+    return false;
+}
 
 // Where the packed row pr of a tile's sequence comes from and goes to.
 struct RowRef {
@@ -621,7 +638,12 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) S[kt][n][i] += lo[kt][n][i];
+                        for (int i = 0; i < 4; ++i) {
+                            // (an infinite key times a lower piece that is 0 or of the
+                            // other sign: the first piece says what the score is)
+                            const float x = S[kt][n][i] + lo[kt][n][i];
+                            S[kt][n][i] = x == x ? x : S[kt][n][i];
+                        }
             }
 
             // ---- the 8-bit scales of this lane's keys, 16 kt + g and + 8
@@ -943,6 +965,11 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                     sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                     const int r = 8 * n + 2 * t4 + e;
                     if (r >= wrows) continue;
+                    // a row that sees nothing has no maximum and gives zeros; one
+                    // whose scores are all -inf has no weights either: NaN
+                    if (M[n][e] == -INFINITY && sum == 0.f &&
+                        sees_any<F::KS>(a, p, tw, m, pos[n][e]))
+                        M[n][e] = -FLT_MAX;
                     if (piece) {
                         const int64_t row = pslot * TR + mt * F::WR + r;
                         if (g == 0) a.stat[row] = make_float2(M[n][e], sum);
@@ -958,8 +985,7 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                             }
                         }
                     } else {
-                        // a row that sees nothing has no sum: zeros
-                        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                        const float inv = M[n][e] == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;
                         const RowRef rr(a, p, pr + r);
                         X* o = static_cast<X*>(a.out) + (int64_t)(p.row + rr.tok) * a.out_stride +
                                (int64_t)rr.head * HD;

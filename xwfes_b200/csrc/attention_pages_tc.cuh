@@ -877,7 +877,8 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                 tc_fence_after();
                 const bool piece = cut_l || cut_r;
                 const float l = f2lo(l2) + f2hi(l2);
-                // no finite score seen: zeros, unless it was a NaN
+                // nothing seen: zeros.  (Scores of -inf alone, and NaN: no zeros)
+                if (M == -INFINITY && l == 0.f && sees_any<KS>(a, p, tw, m, pos)) M = -FLT_MAX;
                 const float inv = piece ? 1.f : M == -INFINITY && l == l ? 0.f : 1.f / l;
                 const int64_t pslot = 2 * (int64_t)blockIdx.x + (cut_l ? 0 : 1);
                 float* part = a.part + (pslot * TR + st * 128 + r) * HD;
