@@ -186,3 +186,48 @@ def test_scores_of_minus_infinity_alone(ftc, q, cache, n):
     agree(got, want, bound, list(range(2 * n)))
     assert torch.isnan(got[:n - n // 2]).all() and torch.isfinite(got[n - n // 2:n]).all()
     assert (got[n:2 * n - n // 2] == 0).all() and torch.isfinite(got[n:]).all()
+
+
+def device_ms(call):
+    """Least of five times of a captured call."""
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    times = []
+    for _ in range(5):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
+
+
+@pytest.mark.parametrize("q,cache", [("bf16", "bf16"), ("f16", "f16")])
+def test_one_request_with_nan_leaves_the_others(ftc, q, cache):
+    """A NaN among one request's values changes no bit of the others' results, nor
+    their time by more than that request's own tile."""
+    g = gen(103)
+    seqs = [(64, 64)] + [(64, 16384)] * 47
+    page = 64
+    n_pages = 1 + 47 * 256
+    pages = make_pages(ftc, cache, n_pages, 2, page, 128, g)
+    for x in (pages.k, pages.v):
+        x.normal_(generator=g)
+    batch, start, lens, table = make_batch(ftc, seqs, page, n_pages, g)
+    x = torch.randn((batch.n_tokens, 8 * 128), generator=g, device="cuda").to(TYPES[q])
+    out = torch.empty_like(x)
+
+    def call():
+        ftc.attention_pages(x, 8, pages, batch, out=out)
+    quick = device_ms(call)
+    plain = out.clone()
+    pages.v[int(table[0, 0]), :, 30, 5] = math.nan
+    slow = device_ms(call)
+    assert ftc.device_status() == 0
+    assert torch.equal(out[64:], plain[64:]) and torch.equal(out[:30], plain[:30])
+    assert torch.isnan(out[30:64].view(34, 8, 128)[:, :, 5]).all()
+    # its own tile: 64 positions that 256 threads read one by one
+    assert slow < 3 * quick, (slow, quick)

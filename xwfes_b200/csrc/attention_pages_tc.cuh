@@ -199,8 +199,26 @@ __device__ __forceinline__ void commit_lead(uint64_t* bar, uint32_t lead) {
         : "memory");
 }
 
+// Bits 15 and 31: the 16-bit value in that half is not finite (a full exponent
+// field carries into the sign's place).
+template <typename OT>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    constexpr bool half = std::is_same<OT, __half>::value;
+    return ((w & (half ? 0x7C007C00u : 0x7F807F80u)) + (half ? 0x04000400u : 0x00800080u)) &
+           0x80008000u;
+}
+
+// Whether every row of a tile sees all of the chunk from key0 on, mapped or not.
+template <class F>
+__device__ __forceinline__ bool covered(const PagedArgs& a, const TileWork<F::TR, F::KS>& tw,
+                                        int key0) {
+    return key0 + F::KS - 1 <= tw.p_first &&
+           (a.window == 0 || tw.p_last - key0 < a.window || key0 + F::KS - 1 < a.n_sink);
+}
+
 // V elements that are not finite, of the positions that a row sees, added to
-// 32 dimensions of its sum.
+// 32 dimensions of its sum.  Chunks that all rows see whole went through the
+// product as they are.
 template <class F>
 __device__ __noinline__ void add_odd(const PagedArgs& a, const PlanPos& p,
                                      const TileWork<F::TR, F::KS>& tw, int m, int pos, int d0,
@@ -208,19 +226,32 @@ __device__ __noinline__ void add_odd(const PagedArgs& a, const PlanPos& p,
     using OT = typename F::OT;
     for (int j = 0; j < m; ++j) {
         const int key0 = tw.key0(p.i + j);
+        bool whole = covered<F>(a, tw, key0);
+        for (int k = key0; whole && k < key0 + F::KS; k += a.b.page_size)
+            whole = page_of(a.b, p.s, k) >= 0;
+        if (whole) continue;
+        int pg = -1;
         for (int key = key0; key < key0 + F::KS && key <= pos; ++key) {
-            const int pg = page_of(a.b, p.s, key);
+            if (key % 16 == 0) pg = page_of(a.b, p.s, key);
             if (pg < 0 || !(a.window == 0 || pos - key < a.window || key < a.n_sink)) continue;
-            const uint32_t* v = reinterpret_cast<const uint32_t*>(
+            const uint4* v = reinterpret_cast<const uint4*>(
                 static_cast<const OT*>(a.v) + (int64_t)pg * a.b.page_stride +
                 ((int64_t)p.kvh * a.b.page_size + (key & (a.b.page_size - 1))) * F::HD + d0);
+            uint4 x4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x4[i] = v[i];
+            const uint32_t* x = reinterpret_cast<const uint32_t*>(x4);
+            uint32_t z = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) z |= not_finite<OT>(x[i]);
+            if (z == 0) continue;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float2 x = unpack<OT>(v[i]);
-                if (!(fabsf(x.x) < INFINITY))
-                    s[2 * i] = __float_as_uint(__uint_as_float(s[2 * i]) + x.x);
-                if (!(fabsf(x.y) < INFINITY))
-                    s[2 * i + 1] = __float_as_uint(__uint_as_float(s[2 * i + 1]) + x.y);
+                const float2 y = unpack<OT>(x[i]);
+                if (!(fabsf(y.x) < INFINITY))
+                    s[2 * i] = __float_as_uint(__uint_as_float(s[2 * i]) + y.x);
+                if (!(fabsf(y.y) < INFINITY))
+                    s[2 * i + 1] = __float_as_uint(__uint_as_float(s[2 * i + 1]) + y.y);
             }
         }
     }
@@ -342,11 +373,13 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
     uint64_t* o_empty = o_full + 2;
     uint64_t* drain = o_empty + 2;
     volatile int* dead = reinterpret_cast<volatile int*>(drain + 1);
-    volatile int* odd = dead + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(dead) + 2);
-    int* sFlag = const_cast<int*>(dead) + 4;  // [NSC]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(dead) + 1);
+    // [stage][4][2] the stage's segment (from 1 on) in which a preparing warp
+    // took V elements out; no warp is four segments ahead of another
+    volatile int* odd = dead + 2;
+    int* sFlag = const_cast<int*>(dead) + 18;  // [NSC]
     PlanPos* sPos = reinterpret_cast<PlanPos*>(sFlag + F::NSC);
-    static_assert((3 * NS + 2 * F::NR + 2 * F::NSC + 15) * 8 + 16 + 4 * F::NSC +
+    static_assert((3 * NS + 2 * F::NR + 2 * F::NSC + 15) * 8 + 72 + 4 * F::NSC +
                           (int)sizeof(PlanPos) <= 1024, "control block");
     int64_t* sPre = reinterpret_cast<int64_t*>(sRing);
 
@@ -376,7 +409,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
         }
         mbar_init(drain, 1);
         *dead = 0;
-        *odd = 0;
+        for (int i = 0; i < 16; ++i) odd[i] = 0;
         mbar_fence_init();
     }
     if (!a.second) grid_dependency_wait();  // as paged_mma
@@ -587,10 +620,14 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             // ------------------------------------------- operand preparation
             // and each of the two warps brings the q rows of a stage
             const int w = warp - 2;
-            uint32_t seg = 0, nq = 0;  // segments, and those with rows of this stage
+            // segments, those with rows of this stage, and of the second
+            uint32_t seg = 0, nq = 0, seg1 = 0;
+            bool both = false;  // this one has
             for (uint32_t u = 0; u < (uint32_t)total; ++u) {
                 if (wk.first()) {
                     const int pr0 = wk.p.t * TR + w * 128, rows = wk.p.n * a.gqa;
+                    both = wk.p.t * TR + 128 < rows;
+                    seg1 += both;
                     if (pr0 < rows) {
                         // (the last tile's scores are all done)
                         if (!ring_wait(&q_empty[w], (nq & 1) ^ 1, dead)) break;
@@ -659,13 +696,9 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                     const uint32_t t = 2 * u + 1;
                     const int s = t % NS;
                     const int key0 = wk.key0();
-                    const bool whole = flag == 0xFF && key0 + KS - 1 <= wk.tw.p_first &&
-                                       (a.window == 0 || wk.tw.p_last - key0 < a.window ||
-                                        key0 + KS - 1 < a.n_sink);
+                    const bool whole = flag == 0xFF && covered<F>(a, wk.tw, key0);
                     if (ring_wait(&full[s], (t / NS) & 1, dead)) {
                         if (!whole) {
-                            constexpr uint32_t kInf = F::kHalf ? 0x7C007C00u : 0x7F807F80u;
-                            constexpr uint32_t kOne = F::kHalf ? 0x04000400u : 0x00800080u;
                             uint4* v = reinterpret_cast<uint4*>(sRing + s * F::TILE);
 #pragma unroll 4
                             for (int q = w * 32 + lane; q < F::TILE / 16; q += 32 * F::NPREP) {
@@ -673,16 +706,17 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                                 uint32_t* x = reinterpret_cast<uint32_t*>(&x4);
                                 uint32_t z = 0;
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) z |= (x[i] & kInf) + kOne;
-                                if (z & 0x80008000u) {
+                                for (int i = 0; i < 4; ++i) z |= not_finite<OT>(x[i]);
+                                if (z != 0) {
 #pragma unroll
                                     for (int i = 0; i < 4; ++i) {
-                                        const uint32_t b = ((x[i] & kInf) + kOne) & 0x80008000u;
+                                        const uint32_t b = not_finite<OT>(x[i]);
                                         x[i] &= ~((b & 0x8000u ? 0xFFFFu : 0u) |
                                                   (b & 0x80000000u ? 0xFFFF0000u : 0u));
                                     }
                                     v[q] = x4;
-                                    *odd = 1;
+                                    odd[2 * (seg & 3) + w] = (int)seg;
+                                    if (both) odd[8 + 2 * (seg1 & 3) + w] = (int)seg1;
                                 }
                             }
                             fence_proxy_async_smem();
@@ -876,6 +910,8 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             if (active && ring_wait(&o_full[st], no++ & 1, dead)) {
                 tc_fence_after();
                 const bool piece = cut_l || cut_r;
+                const volatile int* o2 = odd + 8 * st + 2 * (no & 3);
+                const bool with_odd = !F::kQ8 && live && (o2[0] == (int)no || o2[1] == (int)no);
                 const float l = f2lo(l2) + f2hi(l2);
                 // nothing seen: zeros.  (Scores of -inf alone, and NaN: no zeros)
                 if (M == -INFINITY && l == 0.f && sees_any<KS>(a, p, tw, m, pos)) M = -FLT_MAX;
@@ -892,8 +928,7 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                     uint32_t s[32];
                     tmem_ld_32x32b_x32(tO + 32 * q, s);
                     tmem_ld_done(s);
-                    if (!F::kQ8 && *odd && live)
-                        add_odd<F>(a, p, tw, m, pos, 32 * q, s);
+                    if (with_odd) add_odd<F>(a, p, tw, m, pos, 32 * q, s);
                     if (piece) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
