@@ -11,6 +11,13 @@ namespace paged {
 template <typename X, int HD>
 constexpr bool kTc = sizeof(X) == 2 && HD < 256;
 
+// fp32 queries over a bf16 cache of head_dim 64 have no 64-row shape: one of
+// this type with several groups of warps (not in the tree) stopped with an
+// illegal access that reading did not explain, and a shape that no test had run
+// is not the place to look for it.  17 to 64 rows take the 128-row shape.
+template <typename X, typename C, int HD>
+constexpr bool kNo64 = sizeof(X) == 4 && std::is_same<C, __nv_bfloat16>::value && HD == 64;
+
 // The class's shape elsewhere: 4 warps in turn on 8 rows and on 16, one group
 // of 4 warps of 16 rows, and of 8 (head_dim 256: 4, nine warps leave a thread
 // too few registers).  The tcgen05 kernel does not pay below 64 rows: 24 rows
@@ -19,7 +26,9 @@ template <typename X, typename C, int HD, class Fn>
 auto with_class(int cls, Fn fn) {
     if (cls == 0) return fn((Cfg<X, C, HD, 1, 1, 4>*)nullptr);
     if (cls == 1) return fn((Cfg<X, C, HD, 2, 1, 4>*)nullptr);
-    if (cls == 2 || HD == 256) return fn((Cfg<X, C, HD, 2, 4, 4>*)nullptr);
+    if constexpr (!kNo64<X, C, HD>) {
+        if (cls == 2 || HD == 256) return fn((Cfg<X, C, HD, 2, 4, 4>*)nullptr);
+    }
     constexpr int big = HD == 256 || kTc<X, HD> ? 4 : 8;
     return fn((Cfg<X, C, HD, 2, big, big>*)nullptr);
 }
