@@ -231,3 +231,58 @@ def test_one_request_with_nan_leaves_the_others(ftc, q, cache):
     assert torch.isnan(out[30:64].view(34, 8, 128)[:, :, 5]).all()
     # its own tile: 64 positions that 256 threads read one by one
     assert slow < 3 * quick, (slow, quick)
+
+
+COMBOS = Q8 + WIDE
+# sequences whose packed rows (4 query heads a KV head) need tiles of 16 rows, and of 64
+ROWS = {"16 rows": [(4, 300), (3, 70), (3, 3)], "64 rows": [(10, 300), (16, 70), (5, 5)],
+        "64 rows beside decode": [(1, 200), (10, 300), (1, 17), (16, 16)]}
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("window,sink", [(0, 0), (50, 0), (40, 70)])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("q,cache", COMBOS)
+def test_a_few_tokens(ftc, q, cache, hd, rows, window, sink, page):
+    attend(ftc, q, cache, 8, 2, hd, page, ROWS[rows], window, sink, seed=107 + hd)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("q,cache", COMBOS)
+def test_a_few_tokens_with_pages_that_are_not_mapped(ftc, q, cache, hd, rows):
+    def edit(pages, table):
+        table[0, 3] = -1
+        table[1, 0] = pages.k.shape[0]
+        table[2, :] = -9
+    got, want = attend(ftc, q, cache, 8, 2, hd, 16, ROWS[rows], seed=109 + hd, edit=edit)
+    n = [n for n, _ in ROWS[rows]]
+    assert (got[n[0] + n[1]:n[0] + n[1] + n[2]] == 0).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("q,cache", COMBOS)
+def test_a_few_tokens_with_values_that_are_not_finite(ftc, q, cache, hd, rows, bad):
+    """In K and V before the window and behind a row's position, and in V where
+    rows see it."""
+    seqs, window = ROWS[rows], 60
+    n0, len0 = max(seqs, key=lambda x: x[1] if x[0] > 1 else 0)
+    s0 = seqs.index((n0, len0))
+
+    def edit(pages, table):
+        last = len0 - 1  # the last row alone sees this one
+        hidden = [0, 100, len0 - n0 - window]  # no row does
+        for j in hidden + [last, len0 - n0 - 20]:
+            p, slot = int(table[s0, j // 16]), j % 16
+            names = ("k", "v") if j in hidden else ("v",)
+            for name in names:
+                if cache == "q8":
+                    getattr(pages, name + "_scale")[p, 0, slot] = math.nan
+                else:
+                    getattr(pages, name)[p, 0, slot, 11] = bad
+    got, want = attend(ftc, q, cache, 8, 2, hd, 16, seqs, window=window, seed=113 + hd, edit=edit)
+    assert not torch.isfinite(got).all()
+    assert torch.isfinite(got.view(len(got), 2, -1)[:, 1]).all()  # the other KV head
