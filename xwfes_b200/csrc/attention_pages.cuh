@@ -59,6 +59,7 @@ struct Cfg {
     using C = C_;
     static constexpr int HD = HD_, NT = NT_, MW = MW_, NW = NW_;
     static constexpr int NG = NW / MW;      // warp groups
+    static_assert(MW == 1 || NG == 1, "one group of several warps, or groups of one");
     static constexpr int WR = 8 * NT;       // packed rows per warp
     static constexpr int TR = WR * MW;      // packed rows per tile
     using OT = typename std::conditional<std::is_same<C, __nv_bfloat16>::value, __nv_bfloat16,
@@ -78,7 +79,7 @@ struct Cfg {
     static constexpr int QB1 = MW * NT * NP * (HD / 16) * 256;
     static constexpr int QB = NQB * QB1;
     static constexpr int PER = HD / 4 * NT + 4 * NT;   // floats a lane hands over in a join
-    static constexpr int XB = NG > 1 ? (NG / 2) * MW * 32 * PER * 4 : 0;
+    static constexpr int XB = NG > 1 ? (NG / 2) * 32 * PER * 4 : 0;
     static constexpr int CTL = 1536;                   // barriers, flags, row factors
     static constexpr int kFixed = 1024 /* alignment */ + QB + XB + CTL;
     static constexpr int SLOT_ALL = SLOT + (kQ8 ? 2 * KS * 4 : 0);
@@ -355,7 +356,7 @@ __device__ __forceinline__ void prepare_q(const PagedArgs& a, const PlanPos& p, 
     }
 }
 
-template <typename X, class F>
+template <typename X>
 __device__ __forceinline__ void store1(X* o, float v) {
     if constexpr (sizeof(X) == 4) *o = v;
     else if constexpr (std::is_same<X, __half>::value) *o = __float2half_rn(v);
@@ -908,7 +909,7 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
             for (int h = NG / 2; h >= 1; h >>= 1) {
                 // rounds after the first write where this warp has read
                 if (grp >= h && grp < 2 * h) {
-                    float* x = sX + (((h == NG / 2 ? grp - h : grp) * MW + mt) * PER) * 32 + lane;
+                    float* x = sX + ((h == NG / 2 ? grp - h : grp) * PER) * 32 + lane;
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -925,8 +926,7 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
                 }
                 named_barrier(1, F::NW * 32);
                 if (grp < h) {
-                    const float* x =
-                        sX + (((h == NG / 2 ? grp : grp + h) * MW + mt) * PER) * 32 + lane;
+                    const float* x = sX + ((h == NG / 2 ? grp : grp + h) * PER) * 32 + lane;
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         float fa[2], fb[2];
@@ -992,11 +992,11 @@ paged_mma(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtens
 #pragma unroll
                         for (int d = 0; d < DT; ++d) {
                             if constexpr (F::kQ8) {
-                                store1<X, F>(o + 16 * d + 2 * g, O[d][n][e] * inv);
-                                store1<X, F>(o + 16 * d + 2 * g + 1, O[d][n][2 + e] * inv);
+                                store1<X>(o + 16 * d + 2 * g, O[d][n][e] * inv);
+                                store1<X>(o + 16 * d + 2 * g + 1, O[d][n][2 + e] * inv);
                             } else {
-                                store1<X, F>(o + 16 * d + g, O[d][n][e] * inv);
-                                store1<X, F>(o + 16 * d + 8 + g, O[d][n][2 + e] * inv);
+                                store1<X>(o + 16 * d + g, O[d][n][e] * inv);
+                                store1<X>(o + 16 * d + 8 + g, O[d][n][2 + e] * inv);
                             }
                         }
                     }

@@ -19,18 +19,21 @@ template <typename X, typename C, int HD>
 constexpr bool kNo64 = sizeof(X) == 4 && std::is_same<C, __nv_bfloat16>::value && HD == 64;
 
 // The class's shape elsewhere: 4 warps in turn on 8 rows and on 16, one group
-// of 4 warps of 16 rows, and of 8 (head_dim 256: 4, nine warps leave a thread
-// too few registers).  The tcgen05 kernel does not pay below 64 rows: 24 rows
+// of 4 warps of 16 rows, and of 8 (head_dim 256: 4 again, nine warps leave a
+// thread too few registers).  The tcgen05 kernel does not pay below 64 rows: 24 rows
 // of 8-bit cache 316 us there, 261 here; 16 rows 315 and 108.
 template <typename X, typename C, int HD, class Fn>
 auto with_class(int cls, Fn fn) {
     if (cls == 0) return fn((Cfg<X, C, HD, 1, 1, 4>*)nullptr);
     if (cls == 1) return fn((Cfg<X, C, HD, 2, 1, 4>*)nullptr);
-    if constexpr (!kNo64<X, C, HD>) {
-        if (cls == 2 || HD == 256) return fn((Cfg<X, C, HD, 2, 4, 4>*)nullptr);
+    if constexpr (HD == 256 || kTc<X, HD>) {
+        return fn((Cfg<X, C, HD, 2, 4, 4>*)nullptr);
+    } else {
+        if constexpr (!kNo64<X, C, HD>) {
+            if (cls == 2) return fn((Cfg<X, C, HD, 2, 4, 4>*)nullptr);
+        }
+        return fn((Cfg<X, C, HD, 2, 8, 8>*)nullptr);
     }
-    constexpr int big = HD == 256 || kTc<X, HD> ? 4 : 8;
-    return fn((Cfg<X, C, HD, 2, big, big>*)nullptr);
 }
 
 template <typename X, typename C, int HD>
