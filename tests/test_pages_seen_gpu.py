@@ -286,3 +286,60 @@ def test_a_few_tokens_with_values_that_are_not_finite(ftc, q, cache, hd, rows, b
     got, want = attend(ftc, q, cache, 8, 2, hd, 16, seqs, window=window, seed=113 + hd, edit=edit)
     assert not torch.isfinite(got).all()
     assert torch.isfinite(got.view(len(got), 2, -1)[:, 1]).all()  # the other KV head
+
+
+@pytest.mark.parametrize("n", [1, 10, 90])
+@pytest.mark.parametrize("sink", [0, 3, 40])
+@pytest.mark.parametrize("q,cache", [("f32", "q8"), ("f32", "f16"), ("bf16", "bf16"), ("f16", "q8")])
+def test_windows_past_the_table(ftc, q, cache, sink, n):
+    """Positions far past the table, up to the last that 31 bits hold: windows over
+    nothing, sinks that are there."""
+    g = gen(127)
+    pages = make_pages(ftc, cache, 12, 2, 16, 64, g)
+    batch, start, lens, table = make_batch(ftc, [(n, 64), (n, 64), (n, 64)], 16, 12, g)
+    fill(pages, table, lens, g)
+    far = [2 ** 31 - 1, 2 ** 31 - 120, 64 + n // 2 + 30]
+    batch.kv_len.copy_(torch.tensor(far))
+    x = torch.randn((3 * n, 8 * 64), generator=g, device="cuda").to(TYPES[q])
+    got = ftc.attention_pages(x, 8, pages, batch, window=30, n_sink=sink)
+    assert ftc.device_status() == 0
+    # the far rows see the sinks alone: as rows at position 64 + 30 and later do
+    near = [64 + 30 + n] * 2 + far[2:]
+    want, bound = V.attention(x, 8, pages, table, start, near, 30, sink)
+    agree(got, want, bound, list(range(3 * n)))
+    assert sink or (got[:2 * n] == 0).all()
+
+
+@pytest.mark.parametrize("q,cache", COMBOS)
+def test_rows_before_the_first_sequence(ftc, q, cache):
+    """Rows before start[0] and behind the last sequence are padding; sequences
+    without rows lie between others."""
+    g = gen(131)
+    pages = make_pages(ftc, cache, 20, 2, 16, 64, g)
+    batch, start, lens, table = make_batch(ftc, [(0, 5), (4, 40), (0, 9), (6, 6), (0, 0)], 16, 20, g,
+                                           tail=9)
+    fill(pages, table, lens, g)
+    start = [a + 3 for a in start]
+    batch.start.copy_(torch.tensor(start))
+    T = batch.n_tokens
+    inside = torch.arange(T, device="cuda")
+    inside = (inside >= 3) & (inside < 13)
+    x = torch.randn((T, 8 * 64), generator=g, device="cuda").to(TYPES[q])
+    kn, vn = (torch.randn((T, 2 * 64), generator=g, device="cuda") for _ in range(2))
+    kn[~inside], vn[~inside] = math.nan, math.nan
+    ftc.kv_pages_write(pages, kn, vn, batch)
+    out = torch.full_like(x, 7.0)
+    ftc.attention_pages(x, 8, pages, batch, out=out)
+    want, bound = V.attention(x, 8, pages, table, start, lens)
+    agree(out, want, bound, list(range(3, 13)))
+    assert (out[~inside] == 7.0).all()
+    k, v = (torch.full((T, 128), 7.0, device="cuda") for _ in range(2))
+    ftc.kv_pages_read(pages, batch, k, v)
+    for got, new in ((k, kn), (v, vn)):
+        y = new[inside].view(-1, 2, 64)
+        if cache == "q8":
+            c, d = R.quantise(y)
+            y = c.float() * d[..., None]
+        else:
+            y = y.to(TYPES[cache]).float()
+        assert torch.equal(got[inside], y.view(-1, 128)) and (got[~inside] == 7.0).all()
