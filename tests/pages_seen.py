@@ -77,4 +77,4 @@ def attention(q, n_head, pages, table, start, kv_len, window=0, n_sink=0, scale=
         bound[start[s]:start[s + 1]] = b.permute(2, 0, 1, 3).reshape(n, n_head, hd)
     if q.dtype == torch.float16:
         bound += 2.0 ** -25  # half a step of its subnormals
-    return out.view(len(q), -1), bound.view(len(q), -1)
+    return out.flatten(1), bound.flatten(1)

@@ -909,9 +909,22 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
             // ---- the finished rows, or this piece of them
             if (active && ring_wait(&o_full[st], no++ & 1, dead)) {
                 tc_fence_after();
+                if constexpr (!F::kQ8) {
+                    const volatile int* o2 = odd + 8 * st + 2 * (no & 3);
+                    if (o2[0] == (int)no || o2[1] == (int)no) {
+#pragma unroll 1
+                        for (int q = 0; q < HD / 32; ++q) {
+                            uint32_t s[32];
+                            tmem_ld_32x32b_x32(tO + 32 * q, s);
+                            tmem_ld_done(s);
+                            if (live) add_odd<F>(a, p, tw, m, pos, 32 * q, s);
+                            __syncwarp();
+                            tmem_st_x32(tO + 32 * q, s);
+                        }
+                        tmem_st_wait();
+                    }
+                }
                 const bool piece = cut_l || cut_r;
-                const volatile int* o2 = odd + 8 * st + 2 * (no & 3);
-                const bool with_odd = !F::kQ8 && live && (o2[0] == (int)no || o2[1] == (int)no);
                 const float l = f2lo(l2) + f2hi(l2);
                 // nothing seen: zeros.  (Scores of -inf alone, and NaN: no zeros)
                 if (M == -INFINITY && l == 0.f && sees_any<KS>(a, p, tw, m, pos)) M = -FLT_MAX;
@@ -928,7 +941,6 @@ paged_tc(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtenso
                     uint32_t s[32];
                     tmem_ld_32x32b_x32(tO + 32 * q, s);
                     tmem_ld_done(s);
-                    if (with_odd) add_odd<F>(a, p, tw, m, pos, 32 * q, s);
                     if (piece) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
