@@ -590,7 +590,11 @@ size_t ftc_attention_pages_workspace_bytes(const ftc_kv_pages* pages, const ftc_
  * cache a row's weights times V's scales are 16-bit floats relative to the
  * largest product that the row's weights and the scales it sees allow: what is
  * below 2^-31 of that (F32 q: 2^-38) counts as zero, and V above 2^100 in
- * magnitude also costs the sum of weights its smallest terms.  q and out: [n_tokens][stride] of
+ * magnitude also costs the sum of weights its smallest terms.  An element of V
+ * that is not finite makes that element of the rows that see it infinite or
+ * NaN.  Weights are fp32 with FTC_F32 q; with 16-bit q they are rounded to
+ * f16 (bf16 over an FTC_BF16 cache) before they meet V, about as much error
+ * again as the rounding of out; sums are fp32.  q and out: [n_tokens][stride] of
  * q_dtype, head h at h * head_dim; query head h reads KV head
  * h / (n_head / n_head_kv).  q_dtype is FTC_F32 with any cache, or FTC_F16
  * with an FTC_F16 or FTC_KV_Q8 cache, or FTC_BF16 with an FTC_BF16 or

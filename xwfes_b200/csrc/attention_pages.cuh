@@ -22,21 +22,29 @@
 // once for 64 or 128 rows.
 //
 // Decode is bound by HBM: 2 (head_dim bytes) a position and KV head; 64
-// sequences of 100 to 16000 positions, 32 heads on 8, 8-bit: 203 us, 5.4 TB/s.
+// sequences of 100 to 16000 positions, 32 heads on 8, 8-bit: 202 us, 5.5 TB/s.
 // Why matrix instructions for it: with 4 query heads on a KV head the CUDA
 // cores would need 8 multiply-adds a byte of cache, 1.5 times what they have at
 // HBM speed, and the 8-bit decode on top.  A few sequences are bound by latency
 // (one of 517 positions: 17 us, the plan, a chunk and the join in turn), and
-// groups of 4 warps by it too: 40 fp32 rows over an f16 cache run at 1.2 TB/s,
-// 2.4 warps a scheduler, a third of the issue slots used.
+// groups of 4 warps by it too: 40 fp32 rows over an f16 cache (8 sequences of
+// 900 to 6000) take 106 us, 1.1 TB/s, 2.4 warps a scheduler, a third of the
+// issue slots used.  fp32 queries in chunks stay on this path: 1024 tokens on
+// 8192, 32 heads, 1.11 ms over 8 bits, 1.42 over f16, 1.70 over bf16 (2 or 3
+// pieces of q and of the weights: 2 or 3 times the products); so does head_dim
+// 256, 2.14 ms with bf16.  fp32 instances spill: at head_dim 128 over 8 bits
+// 34 to 142 bytes, over 16 bits 4 to 50.
 //
 // Types.  Operands are f16 for f16 and 8-bit caches, bf16 for bf16 caches; the
 // 8-bit codes are exact in f16 (byte -> 1024 + code + 128 in the mantissa, one
 // subtraction), their scales stay outside: K's multiplies the score, V's the
 // weight.  q: a 16-bit q is one operand; a bf16 q over an 8-bit cache becomes
 // f16 with a power-of-two scale per row; an fp32 q is 2 f16 pieces (scaled the
-// same way, 2^-22 kept) or 3 bf16 pieces.  Weights: fp32 q also splits them
-// (2 or 3 pieces), else they are rounded once to the operand type, 2^14 up in
+// same way, 2^-22 kept: one bit or two short of fp32's own) or 3 bf16 pieces.
+// Weights: fp32 q also splits them (2 or 3 pieces), else they are rounded once
+// to the operand type, which a 16-bit result tolerates (an f16 result of a chunk
+// is 0.00029 from exact where fp32 weights give 0.00021, a bf16 one 0.0023 and
+// 0.0017, relative to the results) and saves half of PV's products; 2^14 up in
 // f16 (and V's scale relative to the running maximum of those that the row
 // sees, 2^E) so that weights 2^-38 of the largest still count.  With fp32 q the
 // matrix unit's own accumulation, which truncates, is kept to short chains that

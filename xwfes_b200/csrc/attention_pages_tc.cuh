@@ -19,18 +19,19 @@
 // registers (these warps get 216, the others 72); 2 and 3 turn 8-bit codes
 // into f16 tiles, and in chunks where some row's mask hides something they take
 // V elements that are not finite out (0 x inf would reach every row), which the
-// rows that see them get back at the end; between tiles each fetches the q rows
+// rows that see them get back before the epilogue; between tiles each fetches the q rows
 // of a stage.  8-bit scales stay in fp32: K's multiplies S, V's multiplies P,
 // relative to the running maximum 2^E of those that the row sees (in a chunk
 // that some row does not see whole, each thread looks over its own row's).
 //
 // What bounds it: per chunk and stage pair the tensor cores need 2048 clocks
-// at head_dim 128 and the exponentials, 16 a clock, as many; a chunk takes 2.4
-// times that (2048 bf16 rows of 32 heads on 16384 positions: 523 us, 0.98
-// PFLOP/s).  A stage's softmax (~2100 clocks) and its MMAs (a batch of 8 comes
-// back ~500 clocks after its last issue) stand one after the other, two stages
-// are what tensor memory holds, and the roles' code passes the SM's
-// instruction cache.  Tried and not kept, with the time of the same call: two S
+// at head_dim 128 and the exponentials, 16 a clock, as many; both are busy for
+// 53 % of the time (2048 bf16 rows of 32 heads on 16384 positions: 488 us, 1.06
+// PFLOP/s).  A stage's softmax and its MMAs stand one after the other, two
+// stages are what tensor memory holds at head_dim 128 (at 64, 128 columns and 90
+// KB of shared memory are free and not used), its warps wait for tensor
+// memory and barriers, and 44 to 72 bytes of registers spill.  Tried and not kept,
+// with the time of the same call, then 520 us: two S
 // buffers of 64 keys, scores a chunk early (820 us: what is done once per chunk
 // weighs double); 16 warps, q fetched by two of their own (668 us); a part of
 // the exponentials as polynomials on the FMA pipe (720 us: no one waits for the

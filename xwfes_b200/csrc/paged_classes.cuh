@@ -20,8 +20,11 @@ constexpr bool kNo64 = sizeof(X) == 4 && std::is_same<C, __nv_bfloat16>::value &
 
 // The class's shape elsewhere: 4 warps in turn on 8 rows and on 16, one group
 // of 4 warps of 16 rows, and of 8 (head_dim 256: 4 again, nine warps leave a
-// thread too few registers).  The tcgen05 kernel does not pay below 64 rows: 24 rows
-// of 8-bit cache 316 us there, 261 here; 16 rows 315 and 108.
+// thread too few registers).  Below 64 rows the tcgen05 kernel does not pay
+// over an 8-bit cache (32 sequences of 900 to 6000, 32 heads on 8 of 128, bf16
+// q: 24 rows 303 us there, 202 here; 64 rows 316 and 209).  Over 16 bits it
+// would (24 rows 151 and 229, 64 rows 164 and 237; head_dim 64 114 and 124, 119
+// and 130); one rule for all caches stands for now.
 template <typename X, typename C, int HD, class Fn>
 auto with_class(int cls, Fn fn) {
     if (cls == 0) return fn((Cfg<X, C, HD, 1, 1, 4>*)nullptr);
